@@ -303,7 +303,9 @@ cudaError_t kvf_b200_describe_path(const kvf_args *a, int fmt, int d, int ord, i
  * shared-memory barrier wait in a decode kernel ran out of time (the kernel
  * abandoned the step and its output is not valid). Bit 1: a cross-GPU wait
  * of kvf_b200_decode_exchange ran out of time (the affected output slices are
- * zero). Bit 2: kvf_b200_append met a token outside the cache (not written).
+ * zero). Bit 2: kvf_b200_append, kvf_b200_append_rope, kvf_b200_norm_rope or
+ * kvf_b200_gather met a token outside the cache or the rotation table (not
+ * written).
  * 0 = no error. This call synchronises with the device. */
 unsigned kvf_b200_device_errors(void);
 
@@ -327,11 +329,96 @@ cudaError_t kvf_b200_quantize(int fmt, int d, int group, const float *x, long lo
  * each sequence, usually its length so far; the caller then raises its
  * seq_lens by t_new. For a paged cache the block table must already map every
  * block the new tokens fall in. A token at or past n, or in a block past
- * max_blocks, is skipped and sets bit 2 of kvf_b200_device_errors(). No
+ * max_blocks or mapped to a negative page, is skipped and sets bit 2 of kvf_b200_device_errors(). No
  * reference counterpart: the reference places a whole cache on the host
  * (upload_cache, kvf_host.h:149-195). */
 cudaError_t kvf_b200_append(const kvf_args *a, int fmt, int d, int ord, int paged, const float *k_new,
                             const float *v_new, int t_new, const int *pos, cudaStream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Around the decode step: what a model's projections leave goes into the cache
+ * (kvf_b200_norm_rope, kvf_b200_append_rope), comes back as values
+ * (kvf_b200_gather), and chunks of new tokens attend to the cache
+ * (kvf_b200_chunk_attention). No reference counterpart: its host prepares the
+ * whole cache (upload_cache, runtime/kvf_host.h:149-195) and decodes one token.
+ *
+ * These calls take padded batches: T tokens of each of B sequences, of which
+ * sequence b uses the first lens[b] (device int[B], NULL = all T; outside
+ * [0, T] it is taken as the nearer end). Rows of tokens past lens[b] are not
+ * read, and in the outputs they are left as they were. The caches are those
+ * that kvf_b200_decode reads: f16, int8 with groups of 64 or 128, int4 with
+ * groups of 32, 64 or 128, d 64 or 128, any placement. A NULL pointer that
+ * is needed, a shape or type outside these rules is cudaErrorInvalidValue; a
+ * pointer off its element's alignment (16 bytes for cache payloads and the
+ * tables of kvf_rope) is cudaErrorMisalignedAddress. */
+
+/* Types of a model's activations. */
+enum { KVF_DT_F32 = 0, KVF_DT_F16 = 1, KVF_DT_BF16 = 2 };
+
+/* Head vectors of a padded batch: channel c of head h of token t of sequence b
+ * is element p[b * stride_b + t * stride_t + h * stride_h + c] (strides in
+ * elements), so heads sliced out of one projection's output need no copy.
+ * Rows on 16-byte boundaries are read and written in 16-byte pieces, others
+ * element by element. */
+typedef struct kvf_heads {
+  void *p;
+  int dtype; /* KVF_DT_* */
+  int heads;
+  long long stride_b, stride_t, stride_h;
+} kvf_heads;
+
+/* Rotation by position: cos and sin are fp32 [positions][rot / 2], 16-byte
+ * aligned. The first rot channels of a head (a multiple of 16, at most d) turn
+ * in pairs, pair i by angle i of its token's position: channels (i, i + rot/2),
+ * or (2i, 2i + 1) where `interleaved` is 1:
+ *   (a, b) -> (a cos - b sin, a sin + b cos). */
+typedef struct kvf_rope {
+  const float *cos, *sin;
+  int positions, rot, interleaved;
+} kvf_rope;
+
+/* RMS norm of one head vector: x / sqrt(mean(x^2) + eps) * weight, weight [d]
+ * of any KVF_DT_*. */
+typedef struct kvf_norm {
+  const void *weight;
+  int dtype;
+  float eps;
+} kvf_norm;
+
+/* out = rotate(norm(x)) for every head of every token, in one pass; rope or
+ * norm may be NULL, not both. Token t of sequence b stands at position
+ * pos[b] + t (device int[B]; may be NULL without rope). fp32 arithmetic, every
+ * operation rounded to nearest, the squares added as a tree of neighbours,
+ * rounded once to out's type, which is x's. out may be x itself. A token
+ * whose position is outside the table is not written and sets bit 2 of
+ * kvf_b200_device_errors(). */
+cudaError_t kvf_b200_norm_rope(const kvf_heads *x, const kvf_heads *out, int B, int T, int d, const kvf_rope *rope,
+                               const kvf_norm *norm, const int *pos, const int *lens, cudaStream_t stream);
+
+/* Appends T tokens to every sequence as a model's projections leave them: keys
+ * are normed (k_norm, NULL = no norm) and rotated (rope, NULL = no rotation),
+ * values taken as they are, and both are stored exactly as kvf_b200_quantize
+ * stores their fp32 rows, at tokens pos[b] .. pos[b] + lens[b] - 1 of the cache
+ * `a` describes (the fields that kvf_b200_append reads). q (NULL = none) takes
+ * the same tokens' query heads through q_norm and the rotation into q_out in
+ * the same launch. k, v, q and q_out have one type. A token at or past n, past
+ * max_blocks, in a block mapped to a negative page, or outside the rotation
+ * table is not written and sets bit 2 of kvf_b200_device_errors(). Two tokens
+ * of one call that fall on the same physical row (a page that two sequences
+ * share) leave it undefined. */
+cudaError_t kvf_b200_append_rope(const kvf_args *a, int fmt, int d, int ord, int paged, const kvf_heads *k,
+                                 const kvf_heads *v, int T, const kvf_rope *rope, const kvf_norm *k_norm,
+                                 const int *pos, const int *lens, const kvf_heads *q, const kvf_heads *q_out,
+                                 const kvf_norm *q_norm, cudaStream_t stream);
+
+/* Reads rows of the cache back as values (zero + scale * code, rounded once to
+ * the outputs' type): tokens pos[b] .. pos[b] + lens[b] - 1 of every sequence
+ * (pos NULL = from token 0) into k_out and v_out, which have Hkv heads and one
+ * type. Tokens at or past a->seq_lens[b] (where given) are left as they were;
+ * a token at or past n, past max_blocks or in a block mapped to a negative page
+ * too, and it sets bit 2 of kvf_b200_device_errors(). */
+cudaError_t kvf_b200_gather(const kvf_args *a, int fmt, int d, int ord, int paged, int T, const int *pos,
+                            const int *lens, const kvf_heads *k_out, const kvf_heads *v_out, cudaStream_t stream);
 
 /* Bytes of device scratch behind kvf_b200_decode_noalloc (8 MiB). */
 #define KVF_B200_NOALLOC_SCRATCH_BYTES (8u << 20)

@@ -15,6 +15,7 @@ LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libkvforge_b200.so"
 
 FMT_F16, FMT_INT8, FMT_INT4 = 0, 1, 2
 ORD_HEAD, ORD_TOKEN = 0, 1
+DT_F32, DT_F16, DT_BF16 = 0, 1, 2
 FMT_NAMES = {"f16": FMT_F16, "int8": FMT_INT8, "int4": FMT_INT4}
 
 
@@ -46,6 +47,25 @@ class KvfArgs(ctypes.Structure):
         ("split_sem", c_void_p),
         ("lse", c_void_p),
     ]
+
+
+class KvfHeads(ctypes.Structure):
+    """Mirror of kvf_heads: head vectors of a padded batch (strides in elements)."""
+
+    _fields_ = [("p", c_void_p), ("dtype", c_int), ("heads", c_int), ("stride_b", c_longlong),
+                ("stride_t", c_longlong), ("stride_h", c_longlong)]
+
+
+class KvfRope(ctypes.Structure):
+    """Mirror of kvf_rope: the rotation table."""
+
+    _fields_ = [("cos", c_void_p), ("sin", c_void_p), ("positions", c_int), ("rot", c_int), ("interleaved", c_int)]
+
+
+class KvfNorm(ctypes.Structure):
+    """Mirror of kvf_norm: the weight and epsilon of an RMS norm over a head."""
+
+    _fields_ = [("weight", c_void_p), ("dtype", c_int), ("eps", c_float)]
 
 
 class KvfError(RuntimeError):
@@ -100,6 +120,14 @@ SIGNATURES = [
     ("kvf_b200_quantize", c_int, [c_int, c_int, c_int, c_void_p, c_longlong, c_void_p, c_void_p, c_void_p]),
     ("kvf_b200_append", c_int, [ctypes.POINTER(KvfArgs), c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int,
                                  c_void_p, c_void_p]),
+    ("kvf_b200_norm_rope", c_int, [ctypes.POINTER(KvfHeads), ctypes.POINTER(KvfHeads), c_int, c_int, c_int,
+                                   ctypes.POINTER(KvfRope), ctypes.POINTER(KvfNorm), c_void_p, c_void_p, c_void_p]),
+    ("kvf_b200_append_rope", c_int, [ctypes.POINTER(KvfArgs), c_int, c_int, c_int, c_int, ctypes.POINTER(KvfHeads),
+                                     ctypes.POINTER(KvfHeads), c_int, ctypes.POINTER(KvfRope),
+                                     ctypes.POINTER(KvfNorm), c_void_p, c_void_p, ctypes.POINTER(KvfHeads),
+                                     ctypes.POINTER(KvfHeads), ctypes.POINTER(KvfNorm), c_void_p]),
+    ("kvf_b200_gather", c_int, [ctypes.POINTER(KvfArgs), c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p,
+                                ctypes.POINTER(KvfHeads), ctypes.POINTER(KvfHeads), c_void_p]),
     ("kvf_b200_version", c_char_p, []),
 ]
 

@@ -18,7 +18,8 @@ import numpy as np
 import torch
 
 from . import layout
-from ._native import FMT_F16, FMT_INT4, FMT_INT8, KvfArgs, check, lib
+from ._native import (DT_BF16, DT_F16, DT_F32, FMT_F16, FMT_INT4, FMT_INT8, KvfArgs, KvfError, KvfHeads, KvfNorm, KvfRope,
+                      check, lib)
 from .layout import Placement
 
 LOG2E = 1.4426950408889634
@@ -235,6 +236,214 @@ def append(cache: KVCache, k_new: torch.Tensor, v_new: torch.Tensor, pos: Option
         cache.seq_lens.add_(t_new)
 
 
+DTYPES = {torch.float32: DT_F32, torch.float16: DT_F16, torch.bfloat16: DT_BF16}  # KVF_DT_*
+
+
+@dataclass(frozen=True)
+class Rope:
+    """Rotation by position (kvf_rope): float32 cos, sin [positions][rot / 2].
+
+    The first rot channels of a head (a multiple of 16) turn in pairs (i, i +
+    rot / 2), or (2i, 2i + 1) if `interleaved`. Any schedule of angles works;
+    `build` makes the plain one."""
+
+    cos: torch.Tensor
+    sin: torch.Tensor
+    interleaved: bool = False
+
+    def __post_init__(self):
+        c, s = self.cos, self.sin
+        if c.dim() != 2 or c.shape != s.shape or c.dtype != torch.float32 or s.dtype != torch.float32:
+            raise ValueError("cos and sin must be float32 tensors [positions][rot / 2]")
+        if not (c.is_cuda and c.device == s.device and c.is_contiguous() and s.is_contiguous()):
+            raise ValueError("cos and sin must be contiguous on one CUDA device")
+        object.__setattr__(self, "struct", KvfRope(c.data_ptr(), s.data_ptr(), c.shape[0], 2 * c.shape[1],
+                                                   int(self.interleaved)))
+
+    @classmethod
+    def build(cls, positions: int, rot: int, *, base: float = 10000.0, interleaved: bool = False,
+              device="cuda") -> "Rope":
+        """Angle i of position p is p * base^(-2i / rot), worked out in 64 bits."""
+        inv = base ** (-torch.arange(0, rot, 2, dtype=torch.float64, device=device) / rot)
+        angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * inv
+        return cls(angle.cos().float(), angle.sin().float(), interleaved)
+
+
+def _launch(fn: str, device: torch.device, stream, *args) -> None:
+    """Calls an entry point on `stream` (default: the current one of the
+    tensors' device), with that device current."""
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _launch(fn, device, stream, *args)
+    s = stream if stream is not None else torch.cuda.current_stream(device)
+    check(fn, getattr(lib(), fn)(*args, s.cuda_stream))
+
+
+def _heads(x: torch.Tensor, what: str, device: torch.device, shape=None) -> KvfHeads:
+    if x.dim() != 4 or (shape is not None and tuple(x.shape) != tuple(shape)):
+        raise ValueError(f"{what} must be [B][T][heads][D]" + (f" = {tuple(shape)}" if shape is not None else ""))
+    if x.dtype not in DTYPES or x.device != device or not x.is_cuda:
+        raise ValueError(f"{what} must be float32, float16 or bfloat16 on {device}")
+    st = x.stride()
+    if st[3] != 1 and x.shape[3] > 1:
+        raise ValueError(f"{what}: the channels of a head must be adjacent")
+    return KvfHeads(x.data_ptr(), DTYPES[x.dtype], x.shape[2], st[0], st[1], st[2])
+
+
+def _per_sequence(x: Optional[torch.Tensor], what: str, B: int, device: torch.device) -> Optional[int]:
+    """Address of an int32 [B] tensor, or None."""
+    if x is None:
+        return None
+    if x.dtype != torch.int32 or x.numel() != B or x.device != device or not x.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous int32 tensor of B entries on {device}")
+    return x.data_ptr()
+
+
+def _rope(rope: Optional[Rope], device: torch.device):
+    if rope is None:
+        return None
+    if rope.cos.device != device:
+        raise ValueError(f"the rotation table must be on {device}")
+    return ctypes.byref(rope.struct)
+
+
+def _norm(weight: Optional[torch.Tensor], what: str, d: int, eps: float, device: torch.device):
+    if weight is None:
+        return None
+    if weight.dtype not in DTYPES or weight.shape != (d,) or weight.device != device or not weight.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous tensor [{d}] on {device}")
+    return ctypes.byref(KvfNorm(weight.data_ptr(), DTYPES[weight.dtype], eps))
+
+
+def _output(like: torch.Tensor, shape, dtype, stream) -> torch.Tensor:
+    """A fresh output; zeros, since rows past a sequence's length are left as they are."""
+    out = torch.zeros(shape, dtype=dtype, device=like.device)
+    if stream is not None:
+        cur = torch.cuda.current_stream(like.device)
+        if stream != cur:
+            stream.wait_stream(cur)
+            out.record_stream(stream)
+    return out
+
+
+def _cache_args(cache: "KVCache") -> KvfArgs:
+    """The cache's half of an argument block."""
+    a = KvfArgs()
+    a.k = cache.k.data_ptr()
+    a.v = cache.v.data_ptr()
+    if cache.k_meta is not None:
+        a.k_meta = cache.k_meta.data_ptr()
+        a.v_meta = cache.v_meta.data_ptr()
+        a.group_shift = cache.group.bit_length() - 1
+    if cache.place.paged:
+        a.block_table = cache.block_table.data_ptr()
+        a.block_shift = cache.place.block_tokens.bit_length() - 1
+        a.max_blocks = cache.max_blocks
+    a.B, a.H, a.Hkv, a.n = cache.B, cache.Hkv, cache.Hkv, cache.n
+    if cache.seq_lens is not None:
+        a.seq_lens = cache.seq_lens.data_ptr()
+    return a
+
+
+def norm_rope(x: torch.Tensor, pos: Optional[torch.Tensor], rope: Optional[Rope] = None, *,
+              weight: Optional[torch.Tensor] = None, eps: float = 1e-6, lens: Optional[torch.Tensor] = None,
+              out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+    """RMS norm (if weight [D] is given) and rotation (if rope is) of every head
+    vector of x [B][T][heads][D], in one pass (kvf_b200_norm_rope).
+
+    x may be float32, float16 or bfloat16 with any strides between rows; token
+    t of sequence b stands at position pos[b] + t (int32 [B]; None without
+    rope). lens (int32 [B]) gives the tokens that are there: rows past it are
+    not read, and in `out` left as they were. out (default: a new tensor,
+    zero there) may be x. A position outside the table leaves its rows unwritten
+    and sets bit 2 of device_errors()."""
+    xs = _heads(x, "x", x.device)
+    B, T, H, d = x.shape
+    if weight is None and rope is None:
+        raise ValueError("nothing to do: neither weight nor rope is given")
+    if rope is not None and pos is None:
+        raise ValueError("pos is required to rotate")
+    if out is None:
+        out = _output(x, x.shape, x.dtype, stream)
+    elif out.dtype != x.dtype:
+        raise ValueError("out must have x's type")
+    _launch("kvf_b200_norm_rope", x.device, stream, ctypes.byref(xs), ctypes.byref(_heads(out, "out", x.device, x.shape)),
+            B, T, d, _rope(rope, x.device), _norm(weight, "weight", d, eps, x.device),
+            _per_sequence(pos, "pos", B, x.device), _per_sequence(lens, "lens", B, x.device))
+    return out
+
+
+def append_rope(cache: KVCache, k: torch.Tensor, v: torch.Tensor, rope: Optional[Rope] = None, *,
+                pos: Optional[torch.Tensor] = None, lens: Optional[torch.Tensor] = None,
+                k_weight: Optional[torch.Tensor] = None, q: Optional[torch.Tensor] = None,
+                q_weight: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                stream=None) -> Optional[torch.Tensor]:
+    """Appends T tokens of every sequence to `cache` as a model's projections
+    leave them (kvf_b200_append_rope): k, v [B][T][Hkv][D] (float32, float16 or
+    bfloat16, any strides between rows); keys normed (k_weight [D]) and rotated
+    (rope), both stored exactly as quantize() stores their float32 rows, at
+    tokens pos[b] .. pos[b] + lens[b] - 1.
+
+    q [B][T][H][D] takes the same tokens' query heads through q_weight and the
+    rotation in the same launch; returned (q_out, or a new tensor), else None.
+    lens (int32 [B]) defaults to all T. pos (int32 [B]) defaults to
+    cache.seq_lens, which is then raised by what was appended (on the call's
+    stream); a given pos leaves seq_lens alone. Tokens outside the cache or the
+    table are skipped and set bit 2 of device_errors()."""
+    dev = cache.k.device
+    if k.dim() != 4 or (k.shape[0], k.shape[2], k.shape[3]) != (cache.B, cache.Hkv, cache.d):
+        raise ValueError(f"k must be [B][T][Hkv][D] with B={cache.B}, Hkv={cache.Hkv}, D={cache.d}")
+    B, T, Hkv, d = k.shape
+    ks, vs = _heads(k, "k", dev), _heads(v, "v", dev, k.shape)
+    if v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
+        raise ValueError("q, k and v must have one type")
+    bump = pos is None
+    if bump:
+        if cache.seq_lens is None:
+            raise ValueError("pos is required for a cache without seq_lens")
+        pos = cache.seq_lens
+    qs = qo = None
+    if q is not None:
+        if q.dim() != 4 or (q.shape[0], q.shape[1], q.shape[3]) != (B, T, d):
+            raise ValueError("q must be [B][T][H][D] of the same tokens")
+        if q_out is None:
+            q_out = _output(q, q.shape, q.dtype, stream)
+        elif q_out.dtype != q.dtype:
+            raise ValueError("q_out must have q's type")
+        qs, qo = ctypes.byref(_heads(q, "q", dev)), ctypes.byref(_heads(q_out, "q_out", dev, q.shape))
+    elif q_weight is not None or q_out is not None:
+        raise ValueError("q_weight and q_out go with q")
+    _launch("kvf_b200_append_rope", dev, stream, ctypes.byref(_cache_args(cache)), cache.fmt, d, cache.place.order,
+            int(cache.place.paged), ctypes.byref(ks), ctypes.byref(vs), T, _rope(rope, dev),
+            _norm(k_weight, "k_weight", d, eps, dev), _per_sequence(pos, "pos", B, dev),
+            _per_sequence(lens, "lens", B, dev), qs, qo, _norm(q_weight, "q_weight", d, eps, dev))
+    if bump:
+        with torch.cuda.stream(stream):
+            cache.seq_lens.add_(T if lens is None else lens.clamp(0, T))
+    return q_out
+
+
+def gather(cache: KVCache, T: int, *, pos: Optional[torch.Tensor] = None, lens: Optional[torch.Tensor] = None,
+           dtype: torch.dtype = torch.float32, out=None, stream=None):
+    """Tokens pos[b] .. pos[b] + lens[b] - 1 of every sequence read back from the
+    cache as values (kvf_b200_gather): (k, v), each [B][T][Hkv][D] of `dtype`,
+    or of out = (k, v), which may have any strides between rows. pos defaults to
+    0 and lens to T. Rows past lens, or at or past cache.seq_lens, are left as
+    they were (zero in new tensors)."""
+    dev = cache.k.device
+    shape = (cache.B, T, cache.Hkv, cache.d)
+    if out is None:
+        out = tuple(_output(cache.k, shape, dtype, stream) for _ in range(2))
+    k, v = out
+    if k.dtype != v.dtype:
+        raise ValueError("both outputs must have one type")
+    _launch("kvf_b200_gather", dev, stream, ctypes.byref(_cache_args(cache)), cache.fmt, cache.d, cache.place.order,
+            int(cache.place.paged), T, _per_sequence(pos, "pos", cache.B, dev),
+            _per_sequence(lens, "lens", cache.B, dev), ctypes.byref(_heads(k, "out[0]", dev, shape)),
+            ctypes.byref(_heads(v, "out[1]", dev, shape)))
+    return k, v
+
+
 PATHS = {"auto": 0, "mma": 1, "tc": 2}  # KVF_PATH_AUTO / KVF_PATH_MMA / KVF_PATH_TC
 # Scheduling flags (KVF_FLAG_*), OR'ed into the path value: how the mma.sync
 # launch merges its splits and whether it balances ragged batches; the output
@@ -396,5 +605,6 @@ def device_errors() -> int:
 
 
 __all__ = ["KVCache", "Workspace", "Decoder", "decode", "PATHS", "FLAG_MERGE_KERNEL", "FLAG_GRID_MERGE",
-           "FLAG_NO_BALANCE", "merge_states", "quantize", "append", "suggest_splits", "make_args", "describe",
+           "FLAG_NO_BALANCE", "merge_states", "quantize", "append", "Rope", "norm_rope", "append_rope", "gather",
+           "suggest_splits", "make_args", "describe",
            "device_errors", "row_bytes", "groups_per_row", "scale_log2", "FMT_F16", "FMT_INT8", "FMT_INT4"]

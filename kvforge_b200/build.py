@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import concurrent.futures as cf
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -27,7 +28,7 @@ OBJ = PKG / "_build"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", f"-I{INCLUDE}"]
-LIB_SOURCES = ["decode.cu", "registry.cu", "quantize.cu", "exchange.cu"]
+LIB_SOURCES = ["decode.cu", "registry.cu", "quantize.cu", "exchange.cu", "heads.cu"]
 
 
 def nvcc() -> str:
@@ -38,7 +39,14 @@ def nvcc() -> str:
 
 
 def _deps(src: Path) -> list[Path]:
-    return [src] + sorted(CSRC.glob("*.cuh")) + sorted(INCLUDE.glob("*.h"))
+    """A source, the public headers and the csrc headers it includes."""
+    found, todo = [src], [src]
+    while todo:
+        for name in re.findall(r'^#include "(\w+\.cuh)"', todo.pop().read_text(), re.M):
+            if CSRC / name not in found and (CSRC / name).exists():
+                found.append(CSRC / name)
+                todo.append(CSRC / name)
+    return found + sorted(INCLUDE.glob("*.h"))
 
 
 def _stale(out: Path, deps: list[Path]) -> bool:

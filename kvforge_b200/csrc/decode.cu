@@ -1155,6 +1155,7 @@ extern "C" int kvf_b200_suggest_splits_ragged(int B, int H, int Hkv, int n, int 
 
 namespace kvfb {
 unsigned take_append_errors();  // quantize.cu
+unsigned take_heads_errors();   // heads.cu
 }
 
 extern "C" unsigned kvf_b200_device_errors(void) {
@@ -1165,6 +1166,7 @@ extern "C" unsigned kvf_b200_device_errors(void) {
   }
   if (v) cudaMemcpyToSymbol(g_kvfb_error, &zero, sizeof(zero));
   if (kvfb::take_append_errors()) v |= 4u;  // an appended row fell outside the cache
+  if (kvfb::take_heads_errors()) v |= 4u;   // a token outside the cache or the rotation table
   return v;
 }
 

@@ -1,0 +1,496 @@
+// heads.cu - what lies between a model's projections and its KV cache, and back:
+// RMS norm and rotation of head vectors, the append of rotated keys and of
+// values to the cache, and rows of the cache read back as values.
+//
+//   norm    y = x * (1 / sqrt(mean(x^2) + eps)) * w        over the D channels of a head
+//   rotate  (a, b) -> (a cos - b sin, a sin + b cos)       for pairs (c, c + rot/2) or (2c, 2c + 1)
+//   store   the rounding of the cache's format (quantize.cuh), at the token's physical row
+//   read    zero + scale * code
+//
+// All of it is fp32, every operation rounded to nearest and none contracted,
+// and the squares are added in a fixed tree (channels 2i and 2i + 1, then
+// pairs of those, ...), so the result is the same however the work is spread
+// and what lands in a quantized cache is, bit for bit, kvf_b200_quantize of
+// the rotated row.
+#include "heads.cuh"
+#include "quantize.cuh"
+
+#include <algorithm>
+
+namespace kvfb {
+
+// A token of a call in this file fell outside the cache or the rotation table
+// (reported as bit 2 of kvf_b200_device_errors).
+__device__ unsigned g_kvfb_heads_error;
+
+namespace {
+
+struct Rows {
+  uint8_t *p;
+  long long sb, st, sh;  // strides in bytes
+  int heads;
+  int vec;               // rows start on 16-byte boundaries
+};
+
+struct Norm {
+  const void *w;
+  int dtype;
+  float eps;
+};
+
+struct HeadsArgs {
+  Rows q, q_out, k, v;   // heads = 0: not part of the call
+  Norm qn, kn;           // w = NULL: no norm
+  const float *cos, *sin;
+  int rot, positions, interleaved;
+  const int *pos, *lens;
+  int B, T, units;       // units: warps per token
+  CacheRows cache;
+  uint8_t *kd, *vd;
+  void *km, *vm;
+  int fmt, group;
+};
+
+__device__ __forceinline__ void load_weight8(const Norm &n, int li, float (&w)[8]) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const int c = 8 * li + k;
+    w[k] = n.dtype == KVF_DT_F32   ? __ldg(reinterpret_cast<const float *>(n.w) + c)
+           : n.dtype == KVF_DT_F16 ? __half2float(__ldg(reinterpret_cast<const __half *>(n.w) + c))
+                                   : __bfloat162float(__ldg(reinterpret_cast<const __nv_bfloat16 *>(n.w) + c));
+  }
+}
+
+// One warp takes R * (32 / (D / 8)) head vectors of one token, R per group of
+// D / 8 lanes, so the token's angles are read once for R heads and R rows are
+// in flight per lane. Rows are numbered query heads, then KV heads of k, then of v.
+template <int DT, int D, int R>
+__global__ void __launch_bounds__(256) heads_kernel(const HeadsArgs a) {
+  constexpr int LPR = D / 8;     // lanes per row
+  constexpr int RPW = 32 / LPR;  // rows per warp at a time
+  const int lane = threadIdx.x & 31;
+  const int li = lane % LPR;
+  const long long wid = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  const long long token = wid / a.units;
+  if (token >= (long long)a.B * a.T) return;
+  const int b = (int)(token / a.T), j = (int)(token - (long long)b * a.T);
+  if (a.lens && j >= a.lens[b]) return;
+  const int r0 = (int)(wid - token * a.units) * (R * RPW) + lane / LPR;
+  const int rows = a.q.heads + a.k.heads + a.v.heads;
+  const long long t = a.pos ? (long long)a.pos[b] + j : j;
+  const bool bad_pos = t < 0 || (a.rot && t >= a.positions);
+
+  float e[R][8];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    int r = r0 + i * RPW;
+    const Rows *src = &a.q;
+    if (r >= a.q.heads) {
+      r -= a.q.heads;
+      src = &a.k;
+      if (r >= a.k.heads) {
+        r -= a.k.heads;
+        src = &a.v;
+      }
+    }
+    if (r0 + i * RPW < rows) {
+      load8<DT>(src->p + b * src->sb + j * src->st + r * src->sh + 8 * li * dtype_bytes(DT), src->vec, e[i]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) e[i][k] = 0.f;
+    }
+  }
+
+  // Angles of this lane's channels. Half-split pairs: channel c < rot/2 turns
+  // with c + rot/2, rot/16 lanes further; both halves use angle c mod rot/2.
+  float cs[8], sn[8];
+  const bool turns = a.rot && !bad_pos && 8 * li < a.rot;
+  const int half = a.rot >> 1;
+  if (turns) {
+    const float *c = a.cos + t * half, *s = a.sin + t * half;
+    if (a.interleaved) {
+      const float4 c4 = *reinterpret_cast<const float4 *>(c + 4 * li), s4 = *reinterpret_cast<const float4 *>(s + 4 * li);
+      cs[0] = c4.x; cs[1] = c4.y; cs[2] = c4.z; cs[3] = c4.w;
+      sn[0] = s4.x; sn[1] = s4.y; sn[2] = s4.z; sn[3] = s4.w;
+    } else {
+      const int at = 8 * li < half ? 8 * li : 8 * li - half;
+      load8<KVF_DT_F32>(c + at, true, cs);
+      load8<KVF_DT_F32>(s + at, true, sn);
+    }
+  }
+  const bool low = 8 * li < half;
+  const int partner = (lane & ~(LPR - 1)) + (turns ? (low ? li + (a.rot >> 4) : li - (a.rot >> 4)) : li);
+
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int row = r0 + i * RPW;
+    const int cls = row < a.q.heads ? 0 : row < a.q.heads + a.k.heads ? 1 : 2;
+    if (__all_sync(0xffffffffu, row >= rows)) break;
+    float x[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = e[i][k];
+
+    const Norm &nm = cls == 0 ? a.qn : a.kn;
+    const bool normed = cls < 2 && nm.w;
+    if (__any_sync(0xffffffffu, normed)) {
+      float s[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s[k] = __fmul_rn(x[k], x[k]);
+      float sum = __fadd_rn(__fadd_rn(__fadd_rn(s[0], s[1]), __fadd_rn(s[2], s[3])),
+                            __fadd_rn(__fadd_rn(s[4], s[5]), __fadd_rn(s[6], s[7])));
+#pragma unroll
+      for (int off = 1; off < LPR; off <<= 1) sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, off));
+      if (normed) {
+        const float inv = __fdiv_rn(1.f, __fsqrt_rn(__fadd_rn(__fmul_rn(sum, 1.f / D), nm.eps)));
+        float w[8];
+        load_weight8(nm, li, w);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = __fmul_rn(__fmul_rn(x[k], inv), w[k]);
+      }
+    }
+    if (a.rot) {
+      if (a.interleaved) {
+        if (turns && cls < 2) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float u = x[2 * k], w = x[2 * k + 1];
+            x[2 * k] = __fsub_rn(__fmul_rn(u, cs[k]), __fmul_rn(w, sn[k]));
+            x[2 * k + 1] = __fadd_rn(__fmul_rn(u, sn[k]), __fmul_rn(w, cs[k]));
+          }
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float o = __shfl_sync(0xffffffffu, x[k], partner);
+          if (turns && cls < 2)
+            x[k] = low ? __fsub_rn(__fmul_rn(x[k], cs[k]), __fmul_rn(o, sn[k]))
+                       : __fadd_rn(__fmul_rn(o, sn[k]), __fmul_rn(x[k], cs[k]));
+        }
+      }
+    }
+
+    const bool live = row < rows;
+    if (live && cls == 0) {
+      if (bad_pos) {
+        if (li == 0) atomicOr(&g_kvfb_heads_error, 1u);
+      } else {
+        store8<DT>(a.q_out.p + b * a.q_out.sb + j * a.q_out.st + row * a.q_out.sh + 8 * li * dtype_bytes(DT),
+                   a.q_out.vec, x);
+      }
+    }
+    if (!__any_sync(0xffffffffu, live && cls > 0)) continue;
+    const int h = cls == 1 ? row - a.q.heads : row - a.q.heads - a.k.heads;
+    long long dr = -1;
+    if (live && cls > 0) {
+      dr = bad_pos ? -1 : a.cache.row(b, h, t);
+      if (dr < 0 && li == 0) atomicOr(&g_kvfb_heads_error, 1u);
+    }
+    uint8_t *data = cls == 1 ? a.kd : a.vd;
+    if (a.fmt == KVF_FMT_F16) {
+      if (dr >= 0) store8<KVF_DT_F16>(data + (dr * D + 8 * li) * 2, true, x);
+      continue;
+    }
+    const GroupScale g = group_scale8(x, li, a.group, a.fmt == KVF_FMT_INT8 ? 255 : 15);
+    if (dr >= 0) {
+      const int lpg = a.group >> 3;
+      if ((li & (lpg - 1)) == 0)
+        reinterpret_cast<uint32_t *>(cls == 1 ? a.km : a.vm)[dr * (D / a.group) + li / lpg] = g.word;
+      if (a.fmt == KVF_FMT_INT8)
+        store_codes8<KVF_FMT_INT8>(x, g, data + dr * D, li);
+      else
+        store_codes8<KVF_FMT_INT4>(x, g, data + dr * (D / 2), li);
+    }
+  }
+}
+
+template <int DT, int D>
+cudaError_t launch_heads(HeadsArgs a, cudaStream_t st) {
+  constexpr int RPW = 32 / (D / 8);
+  const int rows = a.q.heads + a.k.heads + a.v.heads;
+  const long long tokens = (long long)a.B * a.T;
+  const int r = tokens * ((rows + RPW - 1) / RPW) >= 4 * 148 * 16 ? 4 : 1;
+  a.units = (rows + r * RPW - 1) / (r * RPW);
+  const long long blocks = (tokens * a.units + 7) / 8;
+  if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+  if (r == 4)
+    heads_kernel<DT, D, 4><<<(unsigned)blocks, 256, 0, st>>>(a);
+  else
+    heads_kernel<DT, D, 1><<<(unsigned)blocks, 256, 0, st>>>(a);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_heads(const HeadsArgs &a, int dtype, int d, cudaStream_t st) {
+  if (d == 128)
+    return dtype == KVF_DT_F32   ? launch_heads<KVF_DT_F32, 128>(a, st)
+           : dtype == KVF_DT_F16 ? launch_heads<KVF_DT_F16, 128>(a, st)
+                                 : launch_heads<KVF_DT_BF16, 128>(a, st);
+  return dtype == KVF_DT_F32   ? launch_heads<KVF_DT_F32, 64>(a, st)
+         : dtype == KVF_DT_F16 ? launch_heads<KVF_DT_F16, 64>(a, st)
+                               : launch_heads<KVF_DT_BF16, 64>(a, st);
+}
+
+Rows rows_of(const kvf_heads *r) {
+  if (!r) return Rows{nullptr, 0, 0, 0, 0, 0};
+  const long long e = dtype_bytes(r->dtype);
+  return Rows{reinterpret_cast<uint8_t *>(r->p), r->stride_b * e, r->stride_t * e, r->stride_h * e, r->heads,
+              rows_aligned(*r) ? 1 : 0};
+}
+
+cudaError_t check_norm(const kvf_norm *n, Norm &out) {
+  out = Norm{nullptr, 0, 0.f};
+  if (!n) return cudaSuccess;
+  if (!n->weight || n->dtype < KVF_DT_F32 || n->dtype > KVF_DT_BF16 || !(n->eps >= 0.f)) return cudaErrorInvalidValue;
+  if (reinterpret_cast<uintptr_t>(n->weight) & (uintptr_t)(dtype_bytes(n->dtype) - 1)) return cudaErrorMisalignedAddress;
+  out = Norm{n->weight, n->dtype, n->eps};
+  return cudaSuccess;
+}
+
+cudaError_t check_rope(const kvf_rope *r, int d, HeadsArgs &a) {
+  if (!r) return cudaSuccess;
+  if (!r->cos || !r->sin || r->positions <= 0 || r->rot <= 0 || r->rot > d || r->rot % 16 ||
+      (r->interleaved != 0 && r->interleaved != 1))
+    return cudaErrorInvalidValue;
+  if ((reinterpret_cast<uintptr_t>(r->cos) | reinterpret_cast<uintptr_t>(r->sin)) & 15u)
+    return cudaErrorMisalignedAddress;
+  a.cos = r->cos;
+  a.sin = r->sin;
+  a.rot = r->rot;
+  a.positions = r->positions;
+  a.interleaved = r->interleaved;
+  return cudaSuccess;
+}
+
+// The cache half of a call's arguments: placement, payload and metadata, in
+// the formats that kvf_b200_decode reads.
+cudaError_t check_cache(const kvf_args *a, int fmt, int d, int ord, int paged, CacheRows &rows, int &group) {
+  if (!a || (d != 64 && d != 128) || fmt < 0 || fmt > 2 || (ord != KVF_ORD_HEAD && ord != KVF_ORD_TOKEN) ||
+      (paged != 0 && paged != 1) || a->B < 0 || a->Hkv <= 0 || a->n <= 0)
+    return cudaErrorInvalidValue;
+  group = 0;
+  if (fmt != KVF_FMT_F16) {
+    if (a->group_shift < 5 || a->group_shift > 7) return cudaErrorInvalidValue;
+    group = 1 << a->group_shift;
+    if (group > d || (fmt == KVF_FMT_INT8 && group < 64)) return cudaErrorInvalidValue;
+  }
+  if (paged && (a->block_shift < 0 || a->block_shift > 20 || a->max_blocks <= 0)) return cudaErrorInvalidValue;
+  if (a->B == 0) return cudaSuccess;
+  if (!a->k || !a->v || (group && (!a->k_meta || !a->v_meta)) || (paged && !a->block_table))
+    return cudaErrorInvalidValue;
+  if ((reinterpret_cast<uintptr_t>(a->k) | reinterpret_cast<uintptr_t>(a->v)) & 15u) return cudaErrorMisalignedAddress;
+  if (group && ((reinterpret_cast<uintptr_t>(a->k_meta) | reinterpret_cast<uintptr_t>(a->v_meta)) & 3u))
+    return cudaErrorMisalignedAddress;
+  rows = CacheRows{a->block_table, a->Hkv, a->n, ord == KVF_ORD_HEAD ? 1 : 0, paged, paged ? a->block_shift : 0,
+                   paged ? a->max_blocks : 0};
+  return cudaSuccess;
+}
+
+// ------------------------------------------------------------------ read back
+struct GatherArgs {
+  Rows k, v;
+  const int *pos, *lens, *seq_lens;
+  int B, T, units;
+  CacheRows cache;
+  const uint8_t *kd, *vd;
+  const uint32_t *km, *vm;
+  int gpr, group_shift;
+};
+
+// One warp takes R * RPW rows of one token, KV heads of k and then of v.
+template <int FMT, int DT, int D, int R>
+__global__ void __launch_bounds__(256) gather_kernel(const GatherArgs a) {
+  constexpr int LPR = D / 8;
+  constexpr int RPW = 32 / LPR;
+  const int lane = threadIdx.x & 31;
+  const int li = lane % LPR;
+  const long long wid = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  const long long token = wid / a.units;
+  if (token >= (long long)a.B * a.T) return;
+  const int b = (int)(token / a.T), j = (int)(token - (long long)b * a.T);
+  if (a.lens && j >= a.lens[b]) return;
+  const long long t = a.pos ? (long long)a.pos[b] + j : j;
+  if (a.seq_lens && t >= a.seq_lens[b]) return;
+  const int Hkv = a.k.heads;
+  const long long row0 = a.cache.row(b, 0, t);
+  if (row0 < 0) {
+    if (lane == 0) atomicOr(&g_kvfb_heads_error, 1u);
+    return;
+  }
+  // Heads of a token lie one row apart (token-major) or a whole sequence or page apart.
+  const long long hstep = !a.cache.head_major ? 1 : a.cache.paged ? 1ll << a.cache.bt_shift : a.cache.n;
+  const int r0 = (int)(wid - token * a.units) * (R * RPW) + lane / LPR;
+  uint4 raw[R];
+  uint32_t mw[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int r = r0 + i * RPW;
+    if (r >= 2 * Hkv) continue;
+    const bool isv = r >= Hkv;
+    const long long row = row0 + (isv ? r - Hkv : r) * hstep;
+    const uint8_t *data = isv ? a.vd : a.kd;
+    if (FMT == KVF_FMT_F16) {
+      raw[i] = __ldcs(reinterpret_cast<const uint4 *>(data + row * (2 * D)) + li);
+    } else {
+      if (FMT == KVF_FMT_INT8) {
+        const uint2 w = __ldcs(reinterpret_cast<const uint2 *>(data + row * D) + li);
+        raw[i].x = w.x;
+        raw[i].y = w.y;
+      } else {
+        raw[i].x = __ldcs(reinterpret_cast<const uint32_t *>(data + row * (D / 2)) + li);
+      }
+      mw[i] = (isv ? a.vm : a.km)[row * a.gpr + ((8 * li) >> a.group_shift)];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int r = r0 + i * RPW;
+    if (r >= 2 * Hkv) continue;
+    const bool isv = r >= Hkv;
+    float x[8];
+    if (FMT == KVF_FMT_F16) {
+      const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 f = widen2<KVF_DT_F16>(w[k]);
+        x[2 * k] = f.x;
+        x[2 * k + 1] = f.y;
+      }
+    } else {
+      const __half2 m = *reinterpret_cast<const __half2 *>(&mw[i]);
+      const float sc = __low2float(m), zero = __high2float(m);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t c = FMT == KVF_FMT_INT8 ? ((k < 4 ? raw[i].x : raw[i].y) >> (8 * (k & 3))) & 255u
+                                               : (raw[i].x >> (4 * k)) & 15u;
+        // the product is exact in fp32 (11 + 8 bits), so fused or not is the same
+        x[k] = __fmaf_rn((float)c, sc, zero);
+      }
+    }
+    const Rows &o = isv ? a.v : a.k;
+    store8<DT>(o.p + b * o.sb + j * o.st + (isv ? r - Hkv : r) * o.sh + 8 * li * dtype_bytes(DT), o.vec, x);
+  }
+}
+
+template <int FMT, int DT, int D>
+cudaError_t launch_gather(GatherArgs a, cudaStream_t st) {
+  constexpr int RPW = 32 / (D / 8), R = 4;
+  a.units = (2 * a.k.heads + R * RPW - 1) / (R * RPW);
+  const long long blocks = ((long long)a.B * a.T * a.units + 7) / 8;
+  if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+  gather_kernel<FMT, DT, D, R><<<(unsigned)blocks, 256, 0, st>>>(a);
+  return cudaGetLastError();
+}
+
+template <int FMT>
+cudaError_t launch_gather(const GatherArgs &a, int dtype, int d, cudaStream_t st) {
+  if (d == 128)
+    return dtype == KVF_DT_F32   ? launch_gather<FMT, KVF_DT_F32, 128>(a, st)
+           : dtype == KVF_DT_F16 ? launch_gather<FMT, KVF_DT_F16, 128>(a, st)
+                                 : launch_gather<FMT, KVF_DT_BF16, 128>(a, st);
+  return dtype == KVF_DT_F32   ? launch_gather<FMT, KVF_DT_F32, 64>(a, st)
+         : dtype == KVF_DT_F16 ? launch_gather<FMT, KVF_DT_F16, 64>(a, st)
+                               : launch_gather<FMT, KVF_DT_BF16, 64>(a, st);
+}
+
+} // namespace
+
+// Nonzero if a token fell outside since the last call (then cleared).
+unsigned take_heads_errors() {
+  unsigned v = 0, zero = 0;
+  if (cudaMemcpyFromSymbol(&v, g_kvfb_heads_error, sizeof(v)) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  if (v) cudaMemcpyToSymbol(g_kvfb_heads_error, &zero, sizeof(zero));
+  return v;
+}
+
+} // namespace kvfb
+
+using namespace kvfb;
+
+extern "C" cudaError_t kvf_b200_norm_rope(const kvf_heads *x, const kvf_heads *out, int B, int T, int d,
+                                          const kvf_rope *rope, const kvf_norm *norm, const int *pos, const int *lens,
+                                          cudaStream_t stream) {
+  if (B < 0 || T < 0 || (d != 64 && d != 128) || (!rope && !norm)) return cudaErrorInvalidValue;
+  if (B == 0 || T == 0) return cudaSuccess;
+  if (rope && !pos) return cudaErrorInvalidValue;
+  cudaError_t e;
+  if ((e = check_heads(x)) != cudaSuccess || (e = check_heads(out)) != cudaSuccess) return e;
+  if (x->dtype != out->dtype || x->heads != out->heads) return cudaErrorInvalidValue;
+  HeadsArgs a{};
+  if ((e = check_rope(rope, d, a)) != cudaSuccess || (e = check_norm(norm, a.qn)) != cudaSuccess) return e;
+  a.q = rows_of(x);
+  a.q_out = rows_of(out);
+  a.k = a.v = rows_of(nullptr);
+  a.pos = rope ? pos : nullptr;
+  a.lens = lens;
+  a.B = B;
+  a.T = T;
+  return launch_heads(a, x->dtype, d, stream);
+}
+
+extern "C" cudaError_t kvf_b200_append_rope(const kvf_args *args, int fmt, int d, int ord, int paged,
+                                            const kvf_heads *k, const kvf_heads *v, int T, const kvf_rope *rope,
+                                            const kvf_norm *k_norm, const int *pos, const int *lens,
+                                            const kvf_heads *q, const kvf_heads *q_out, const kvf_norm *q_norm,
+                                            cudaStream_t stream) {
+  HeadsArgs a{};
+  cudaError_t e;
+  if (T < 0) return cudaErrorInvalidValue;
+  if ((e = check_cache(args, fmt, d, ord, paged, a.cache, a.group)) != cudaSuccess) return e;
+  if (args->B == 0 || T == 0) return cudaSuccess;
+  if ((e = check_heads(k)) != cudaSuccess || (e = check_heads(v)) != cudaSuccess) return e;
+  if (!pos || k->heads != args->Hkv || v->heads != args->Hkv || k->dtype != v->dtype) return cudaErrorInvalidValue;
+  if ((q == nullptr) != (q_out == nullptr) || (!q && q_norm)) return cudaErrorInvalidValue;
+  if (q) {
+    if ((e = check_heads(q)) != cudaSuccess || (e = check_heads(q_out)) != cudaSuccess) return e;
+    if (q->dtype != k->dtype || q_out->dtype != q->dtype || q_out->heads != q->heads) return cudaErrorInvalidValue;
+  }
+  if ((e = check_rope(rope, d, a)) != cudaSuccess || (e = check_norm(k_norm, a.kn)) != cudaSuccess ||
+      (e = check_norm(q_norm, a.qn)) != cudaSuccess)
+    return e;
+  a.q = rows_of(q);
+  a.q_out = rows_of(q_out);
+  a.k = rows_of(k);
+  a.v = rows_of(v);
+  a.pos = pos;
+  a.lens = lens;
+  a.B = args->B;
+  a.T = T;
+  a.fmt = fmt;
+  a.kd = const_cast<uint8_t *>(args->k);
+  a.vd = const_cast<uint8_t *>(args->v);
+  a.km = const_cast<void *>(args->k_meta);
+  a.vm = const_cast<void *>(args->v_meta);
+  return launch_heads(a, k->dtype, d, stream);
+}
+
+extern "C" cudaError_t kvf_b200_gather(const kvf_args *args, int fmt, int d, int ord, int paged, int T, const int *pos,
+                                       const int *lens, const kvf_heads *k_out, const kvf_heads *v_out,
+                                       cudaStream_t stream) {
+  GatherArgs a{};
+  cudaError_t e;
+  int group = 0;
+  if (T < 0) return cudaErrorInvalidValue;
+  if ((e = check_cache(args, fmt, d, ord, paged, a.cache, group)) != cudaSuccess) return e;
+  if (args->B == 0 || T == 0) return cudaSuccess;
+  if ((e = check_heads(k_out)) != cudaSuccess || (e = check_heads(v_out)) != cudaSuccess) return e;
+  if (k_out->heads != args->Hkv || v_out->heads != args->Hkv || k_out->dtype != v_out->dtype)
+    return cudaErrorInvalidValue;
+  a.k = rows_of(k_out);
+  a.v = rows_of(v_out);
+  a.pos = pos;
+  a.lens = lens;
+  a.seq_lens = args->seq_lens;
+  a.B = args->B;
+  a.T = T;
+  a.kd = args->k;
+  a.vd = args->v;
+  a.km = reinterpret_cast<const uint32_t *>(args->k_meta);
+  a.vm = reinterpret_cast<const uint32_t *>(args->v_meta);
+  a.gpr = group ? d / group : 0;
+  a.group_shift = group ? args->group_shift : 0;
+  return fmt == KVF_FMT_F16    ? launch_gather<KVF_FMT_F16>(a, k_out->dtype, d, stream)
+         : fmt == KVF_FMT_INT8 ? launch_gather<KVF_FMT_INT8>(a, k_out->dtype, d, stream)
+                               : launch_gather<KVF_FMT_INT4>(a, k_out->dtype, d, stream);
+}

@@ -11,11 +11,7 @@
 // IEEE single precision with round-to-nearest (no contraction). The metadata
 // word is scale_h | zero_h << 16. int4 puts column c in byte c/2, odd columns
 // in the high nibble. f16 rows are the fp16 (round to nearest even) values.
-#include "kvforge_b200.h"
-
-#include <cuda_fp16.h>
-#include <cuda_runtime.h>
-#include <cstdint>
+#include "quantize.cuh"
 
 namespace kvfb {
 
@@ -24,8 +20,6 @@ namespace kvfb {
 __device__ unsigned g_kvfb_append_error;
 
 namespace {
-
-__device__ __forceinline__ uint16_t h_bits(__half h) { return __half_as_ushort(h); }
 
 // Destination row of source row r: the same row (kvf_b200_quantize), or the
 // physical cache row of an appended token (kvf_b200_append); < 0 = not written.
@@ -38,35 +32,17 @@ struct RowsSame {
 // runtime/kvf_kernels.cuh:51-64 (kvf_host.h:124-135).
 struct RowsAppend {
   const int *pos;
-  const int *table;
-  int Hkv, t_new, n, head_major, paged, bt_shift, max_blocks;
+  int t_new;
+  CacheRows cache;
   __device__ __forceinline__ long long operator()(long long r) const {
     const long long bh = r / t_new;
     const int j = (int)(r - bh * t_new);
-    const int h = (int)(bh % Hkv);
-    const int b = (int)(bh / Hkv);
+    const int h = (int)(bh % cache.Hkv);
+    const int b = (int)(bh / cache.Hkv);
     const int p0 = pos[b];
-    const long long t = (long long)p0 + j;
-    if (p0 < 0 || t >= n) return -1;
-    if (!paged) return head_major ? ((long long)b * Hkv + h) * n + t : ((long long)b * n + t) * Hkv + h;
-    const int blk = (int)(t >> bt_shift);
-    if (blk >= max_blocks) return -1;
-    const long long bt = 1ll << bt_shift, tl = t & (bt - 1);
-    const long long base = (long long)table[(long long)b * max_blocks + blk] * Hkv * bt;
-    return head_major ? base + (long long)h * bt + tl : base + tl * Hkv + h;
+    return p0 < 0 ? -1 : cache.row(b, h, (long long)p0 + j);
   }
 };
-
-// clamp(lround((x - zero) / sc), 0, levels) with the host's behaviour at the
-// edges: lround of a NaN, an infinity or a value of magnitude >= 2^63 yields
-// LONG_MIN on x86-64, which the clamp turns into 0 (this happens when a group
-// exceeds the fp16 range and zero becomes -inf).
-__device__ __forceinline__ int code(float x, float zero, float sc, int levels) {
-  const float t = __fdiv_rn(__fsub_rn(x, zero), sc);
-  if (!(t < 9.223372036854775808e18f && t > -9.223372036854775808e18f)) return 0;
-  const long long q = llroundf(t);
-  return q < 0 ? 0 : (q > levels ? levels : (int)q);
-}
 
 // One thread per (row, group).
 template <int FMT, class Dst>
@@ -173,26 +149,6 @@ __global__ void __launch_bounds__(256) quantize_rows(const float *__restrict__ x
   }
 }
 
-// code() without the division in the common case. With a = x - zero (fp32,
-// as the host computes it) and r = 1/sc rounded to nearest, t' = a * r is
-// within 3 * 2^-24 |t| of the host's t = a / sc (both correctly rounded), so
-// for |t'| < 1024 the two differ by less than 2^-12. When t' is further than
-// that from every half-integer, t lies strictly between the same two
-// half-integers as t', and round-half-away(t) = rint(t'); otherwise (and for
-// |t'| >= 1024, NaN or infinities, including sc = 0) the exact code() decides.
-__device__ __forceinline__ int code_fast(float x, float zero, float sc, float rsc, int levels) {
-  const float a = __fsub_rn(x, zero);
-  const float t = __fmul_rn(a, rsc);
-  if (fabsf(t) < 1024.f) {
-    const float q = rintf(t);
-    if (fabsf(__fsub_rn(t, q)) < 0.5f - 0x1p-12f) {
-      const int qi = (int)q;
-      return qi < 0 ? 0 : (qi > levels ? levels : qi);
-    }
-  }
-  return code(x, zero, sc, levels);
-}
-
 // quantize_rows with eight channels per lane (two 16-byte loads in flight,
 // one combining round fewer) and division-free codes, for groups of 8..D
 // channels (powers of two). Same bit-exact rules as quantize_rows.
@@ -218,51 +174,16 @@ __global__ void __launch_bounds__(256) quantize_rows8(const float *__restrict__ 
     e[0] = v0.x; e[1] = v0.y; e[2] = v0.z; e[3] = v0.w;
     e[4] = v1.x; e[5] = v1.y; e[6] = v1.z; e[7] = v1.w;
   }
-  const int lpg = group >> 3;  // lanes per group
-  const bool first = (li & (lpg - 1)) == 0;
-  float lo = first ? e[0] : INFINITY, hi = first ? e[0] : -INFINITY;
-#pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    if (k == 0 && first) continue;
-    lo = (e[k] < lo) ? e[k] : lo;
-    hi = (hi < e[k]) ? e[k] : hi;
-  }
-  for (int off = 1; off < lpg; off <<= 1) {
-    const float plo = __shfl_xor_sync(0xffffffffu, lo, off);
-    const float phi = __shfl_xor_sync(0xffffffffu, hi, off);
-    const bool earlier = (li & off) == 0;
-    const float alo = earlier ? lo : plo, blo = earlier ? plo : lo;
-    const float ahi = earlier ? hi : phi, bhi = earlier ? phi : hi;
-    lo = (blo < alo) ? blo : alo;
-    hi = (ahi < bhi) ? bhi : ahi;
-  }
-  const int levels = FMT == KVF_FMT_INT8 ? 255 : 15;
-  const __half zero_h = __float2half_rn(lo);
-  float scale = __fdiv_rn(__fsub_rn(hi, lo), (float)levels);
-  if (scale <= 0.f) scale = 1.f;
-  const __half scale_h = __float2half_rn(scale);
-  const float zero = __half2float(zero_h);
-  const float sc = __half2float(scale_h);
-  const float rsc = __frcp_rn(sc);
+  const GroupScale g = group_scale8(e, li, group, FMT == KVF_FMT_INT8 ? 255 : 15);
   if (!valid) return;
   const long long dr = dst(r);
   if (dr < 0) {
     if (li == 0) atomicOr(&g_kvfb_append_error, 1u);
     return;
   }
-  const int gpr = D / group;
-  if (first) meta[dr * gpr + li / lpg] = (uint32_t)h_bits(scale_h) | ((uint32_t)h_bits(zero_h) << 16);
-  uint32_t c[8];
-#pragma unroll
-  for (int k = 0; k < 8; ++k) c[k] = (uint32_t)code_fast(e[k], zero, sc, rsc, levels);
-  if (FMT == KVF_FMT_INT8) {
-    const uint2 w = make_uint2(c[0] | (c[1] << 8) | (c[2] << 16) | (c[3] << 24),
-                               c[4] | (c[5] << 8) | (c[6] << 16) | (c[7] << 24));
-    reinterpret_cast<uint2 *>(data + dr * D)[li] = w;
-  } else {
-    reinterpret_cast<uint32_t *>(data + dr * (D / 2))[li] =
-        c[0] | (c[1] << 4) | (c[2] << 8) | (c[3] << 12) | (c[4] << 16) | (c[5] << 20) | (c[6] << 24) | (c[7] << 28);
-  }
+  const int lpg = group >> 3;  // lanes per group
+  if ((li & (lpg - 1)) == 0) meta[dr * (D / group) + li / lpg] = g.word;
+  store_codes8<FMT>(e, g, data + dr * (FMT == KVF_FMT_INT8 ? D : D / 2), li);
 }
 
 template <class Dst>
@@ -376,8 +297,9 @@ extern "C" cudaError_t kvf_b200_append(const kvf_args *a, int fmt, int d, int or
   }
   if (paged && (!a->block_table || a->max_blocks <= 0 || a->block_shift < 0 || a->block_shift > 20))
     return cudaErrorInvalidValue;
-  const kvfb::RowsAppend dst{pos, a->block_table, a->Hkv, t_new, a->n, ord == KVF_ORD_HEAD ? 1 : 0, paged,
-                             paged ? a->block_shift : 0, paged ? a->max_blocks : 0};
+  const kvfb::RowsAppend dst{pos, t_new,
+                             {a->block_table, a->Hkv, a->n, ord == KVF_ORD_HEAD ? 1 : 0, paged,
+                              paged ? a->block_shift : 0, paged ? a->max_blocks : 0}};
   const long long rows = (long long)a->B * a->Hkv * t_new;
   cudaError_t e = kvfb::quantize_into(fmt, d, group, k_new, rows, const_cast<unsigned char *>(a->k),
                                       const_cast<void *>(a->k_meta), dst, stream);
