@@ -420,6 +420,31 @@ cudaError_t kvf_b200_append_rope(const kvf_args *a, int fmt, int d, int ord, int
 cudaError_t kvf_b200_gather(const kvf_args *a, int fmt, int d, int ord, int paged, int T, const int *pos,
                             const int *lens, const kvf_heads *k_out, const kvf_heads *v_out, cudaStream_t stream);
 
+/* Attention of T new tokens of every sequence over the cache `a` describes:
+ *   out[b][j][h] = sum_t softmax_t(scale q[b][j][h] . k_t) v_t,   t < seen
+ * with kv = a->seq_lens[b] (NULL = n; the new tokens' own keys and values
+ * are in the cache already) and ql = q_lens[b] (NULL = T) new tokens: token j
+ * is the sequence's token kv - ql + j and sees kv - ql + j + 1 tokens
+ * (causal = 1), or all kv (causal = 0: cross attention, or a chunk that sees
+ * itself whole). A row that sees nothing gets zeros. What lies in the cache
+ * at tokens a row does not see has no effect on it, infinities and NaN included.
+ * q and out have H heads and one type, any multiple of Hkv query heads, and
+ * may not overlap. Read from `a`: the cache, H, seq_lens, scale_log2, lse
+ * ([B][T][H], optional: log2 of each row's softmax denominator, -inf where it
+ * sees nothing), splits, and for splits > 1 the workspace part_o
+ * [B][T][H][splits][d] (16-byte aligned) and part_ml [B][T][H][splits][2].
+ * q, out, split_sem and max-splits rules of kvf_b200_decode do not apply. Blocks
+ * that hold seen tokens must be mapped (a negative page's tokens count as
+ * zero keys and values). Products of fp32 queries have fp32 accuracy (about
+ * 2^-21 relative). */
+cudaError_t kvf_b200_chunk_attention(const kvf_args *a, int fmt, int d, int ord, int paged, const kvf_heads *q,
+                                     const kvf_heads *out, int T, const int *q_lens, int causal, cudaStream_t stream);
+
+/* The splits of each sequence's tokens that kvf_b200_chunk_attention runs best
+ * with for this shape (dtype: KVF_DT_* of the queries; n: the longest
+ * sequence). At least 1. */
+int kvf_b200_chunk_splits(int B, int T, int H, int Hkv, int n, int fmt, int d, int dtype);
+
 /* Bytes of device scratch behind kvf_b200_decode_noalloc (8 MiB). */
 #define KVF_B200_NOALLOC_SCRATCH_BYTES (8u << 20)
 

@@ -128,6 +128,10 @@ SIGNATURES = [
                                      ctypes.POINTER(KvfHeads), ctypes.POINTER(KvfNorm), c_void_p]),
     ("kvf_b200_gather", c_int, [ctypes.POINTER(KvfArgs), c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p,
                                 ctypes.POINTER(KvfHeads), ctypes.POINTER(KvfHeads), c_void_p]),
+    ("kvf_b200_chunk_attention", c_int, [ctypes.POINTER(KvfArgs), c_int, c_int, c_int, c_int,
+                                         ctypes.POINTER(KvfHeads), ctypes.POINTER(KvfHeads), c_int, c_void_p, c_int,
+                                         c_void_p]),
+    ("kvf_b200_chunk_splits", c_int, [c_int] * 8),
     ("kvf_b200_version", c_char_p, []),
 ]
 

@@ -444,6 +444,77 @@ def gather(cache: KVCache, T: int, *, pos: Optional[torch.Tensor] = None, lens: 
     return k, v
 
 
+@dataclass
+class ChunkWorkspace:
+    """Split partials of chunk_attention: part_o [B][T][H][splits][D] and part_ml
+    [B][T][H][splits][2]. Calls that may overlap on the GPU need one each."""
+
+    splits: int
+    part_o: Optional[torch.Tensor]
+    part_ml: Optional[torch.Tensor]
+
+    @classmethod
+    def allocate(cls, cache: KVCache, T: int, H: int, dtype: torch.dtype, splits: Optional[int] = None) -> "ChunkWorkspace":
+        """For chunks of at most T tokens with H query heads of `dtype`; splits
+        defaults to kvf_b200_chunk_splits."""
+        dev, B, d = cache.k.device, cache.B, cache.d
+        if splits is None:
+            with torch.cuda.device(dev):
+                splits = int(lib().kvf_b200_chunk_splits(B, T, H, cache.Hkv, cache.n, cache.fmt, d, DTYPES[dtype]))
+        if splits <= 1:
+            return cls(1, None, None)
+        return cls(splits, torch.empty((B, T, H, splits, d), dtype=torch.float32, device=dev),
+                   torch.empty((B, T, H, splits, 2), dtype=torch.float32, device=dev))
+
+
+def chunk_attention(q: torch.Tensor, cache: KVCache, *, q_lens: Optional[torch.Tensor] = None, causal: bool = True,
+                    scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                    lse: Optional[torch.Tensor] = None, workspace: Optional[ChunkWorkspace] = None,
+                    stream=None) -> torch.Tensor:
+    """Attention of a chunk of new tokens over the cache (kvf_b200_chunk_attention).
+
+    q [B][T][H][D] (float32, float16 or bfloat16, any strides between rows, H a
+    multiple of Hkv) are the last q_lens[b] (int32 [B], default T) of the
+    cache.seq_lens[b] (default n) tokens stored, each of which sees the cache up
+    to itself (causal), or all of it (causal=False: cross attention). scale
+    defaults to 1 / sqrt(D). Returns out, of q's shape and type; rows past q_lens
+    are left as they were (zero in a new tensor), rows that see nothing are zero.
+    lse (float32 [B][T][H], contiguous) receives log2 of each softmax
+    denominator. workspace (ChunkWorkspace.allocate) saves its allocation here."""
+    dev = cache.k.device
+    qs = _heads(q, "q", dev)
+    B, T, H, d = q.shape
+    if (B, d) != (cache.B, cache.d) or H == 0 or H % cache.Hkv:
+        raise ValueError(f"q {tuple(q.shape)} does not go with the cache (B={cache.B}, Hkv={cache.Hkv}, D={cache.d})")
+    if out is None:
+        out = _output(q, q.shape, q.dtype, stream)
+    elif out.dtype != q.dtype:
+        raise ValueError("out must have q's type")
+    if lse is not None and (lse.dtype != torch.float32 or not lse.is_contiguous() or lse.numel() != B * T * H
+                            or lse.device != dev):
+        raise ValueError("lse must be a contiguous float32 tensor [B][T][H] on the cache's device")
+    a = _cache_args(cache)
+    a.H = H
+    a.scale_log2 = scale_log2(d) if scale is None else scale * LOG2E
+    if lse is not None:
+        a.lse = lse.data_ptr()
+    if workspace is None and B * T:
+        workspace = ChunkWorkspace.allocate(cache, T, H, q.dtype)
+        if stream is not None and workspace.part_o is not None:
+            workspace.part_o.record_stream(stream)
+            workspace.part_ml.record_stream(stream)
+    a.splits = workspace.splits if workspace is not None else 1
+    if a.splits > 1:
+        for x, e in ((workspace.part_o, d), (workspace.part_ml, 2)):
+            if x.device != dev or x.numel() < B * T * H * a.splits * e:
+                raise ValueError("workspace is too small for this chunk, or on another device")
+        a.part_o, a.part_ml = workspace.part_o.data_ptr(), workspace.part_ml.data_ptr()
+    _launch("kvf_b200_chunk_attention", dev, stream, ctypes.byref(a), cache.fmt, d, cache.place.order,
+            int(cache.place.paged), ctypes.byref(qs), ctypes.byref(_heads(out, "out", dev, q.shape)), T,
+            _per_sequence(q_lens, "q_lens", B, dev), int(causal))
+    return out
+
+
 PATHS = {"auto": 0, "mma": 1, "tc": 2}  # KVF_PATH_AUTO / KVF_PATH_MMA / KVF_PATH_TC
 # Scheduling flags (KVF_FLAG_*), OR'ed into the path value: how the mma.sync
 # launch merges its splits and whether it balances ragged batches; the output
@@ -605,6 +676,6 @@ def device_errors() -> int:
 
 
 __all__ = ["KVCache", "Workspace", "Decoder", "decode", "PATHS", "FLAG_MERGE_KERNEL", "FLAG_GRID_MERGE",
-           "FLAG_NO_BALANCE", "merge_states", "quantize", "append", "Rope", "norm_rope", "append_rope", "gather",
+           "FLAG_NO_BALANCE", "merge_states", "quantize", "append", "Rope", "norm_rope", "append_rope", "gather", "ChunkWorkspace", "chunk_attention",
            "suggest_splits", "make_args", "describe",
            "device_errors", "row_bytes", "groups_per_row", "scale_log2", "FMT_F16", "FMT_INT8", "FMT_INT4"]

@@ -1,0 +1,164 @@
+// chunk.cu - attention of a chunk of new tokens over the cache
+// (kvf_b200_chunk_attention): checks, the choice of kernel and splits, launches
+// and the merge of splits. The kernels are in chunk_mma.cuh.
+#include "chunk_mma.cuh"
+
+#include <algorithm>
+
+namespace kvfb {
+
+cudaError_t ensure_kernel_smem(void *fn, uint32_t smem);  // decode.cu
+int device_sm_count();                                    // decode.cu
+
+namespace {
+
+// One warp per (token, query head): out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M).
+// Splits that saw nothing have m = -inf and no output.
+template <int DT, int D>
+__global__ void __launch_bounds__(128) chunk_merge(const ChunkArgs a) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int lane = threadIdx.x & 31;
+  const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (at >= (long long)a.B * a.T * a.H) return;
+  const int h = (int)(at % a.H);
+  const long long bt = at / a.H;
+  const int j = (int)(bt % a.T), b = (int)(bt / a.T);
+  if (a.q_lens && j >= a.q_lens[b]) return;
+  const float2 *ml = reinterpret_cast<const float2 *>(a.part_ml) + at * a.splits;
+  const float *po = a.part_o + at * a.splits * D;
+  float m = -INFINITY;
+  for (int s = lane; s < a.splits; s += 32) m = fmaxf(m, ml[s].x);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+  float acc[D / 32], l = 0.f;
+#pragma unroll
+  for (int k = 0; k < D / 32; ++k) acc[k] = 0.f;
+  for (int s = 0; s < a.splits; ++s) {
+    const float2 x = ml[s];
+    if (x.x == -INFINITY && !(x.y != x.y)) continue;
+    const float f = exp2f(x.x - (m == -INFINITY ? 0.f : m));
+    l = fmaf(x.y, f, l);
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) acc[k] = fmaf(po[s * D + lane + 32 * k], f, acc[k]);
+  }
+  const bool none = m == -INFINITY && l == 0.f;
+  const float inv = none ? 0.f : 1.f / l;
+  if (a.lse && lane == 0) a.lse[at] = none ? -INFINITY : m + log2f(l);
+  using E = Elem<DT>;
+  typename E::T *out = reinterpret_cast<typename E::T *>(a.out.p + b * a.out.sb + j * a.out.st + h * a.out.sh);
+#pragma unroll
+  for (int k = 0; k < D / 32; ++k) out[lane + 32 * k] = E::from(acc[k] * inv);
+}
+
+template <int DT, int D> void *merge_fn() { return reinterpret_cast<void *>(&chunk_merge<DT, D>); }
+
+template <int FMT, int DT> void *mma_fn(int d) {
+  return d == 128 ? reinterpret_cast<void *>(&chunk_mma_kernel<FMT, DT, 128>)
+                  : reinterpret_cast<void *>(&chunk_mma_kernel<FMT, DT, 64>);
+}
+template <int FMT> void *mma_fn(int dtype, int d) {
+  return dtype == KVF_DT_F32   ? mma_fn<FMT, KVF_DT_F32>(d)
+         : dtype == KVF_DT_F16 ? mma_fn<FMT, KVF_DT_F16>(d)
+                               : mma_fn<FMT, KVF_DT_BF16>(d);
+}
+
+cudaError_t launch(void *fn, long long blocks, int threads, uint32_t smem, const ChunkArgs &a, bool dependent,
+                   cudaStream_t st) {
+  if (blocks <= 0) return cudaSuccess;
+  if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)blocks, 1, 1);
+  cfg.blockDim = dim3((unsigned)threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = dependent ? 1 : 0;
+  void *params[] = {const_cast<ChunkArgs *>(&a)};
+  return cudaLaunchKernelExC(&cfg, fn, params);
+}
+
+ChunkRows chunk_rows(const kvf_heads &r) {
+  const long long e = dtype_bytes(r.dtype);
+  return ChunkRows{reinterpret_cast<uint8_t *>(r.p), r.stride_b * e, r.stride_t * e, r.stride_h * e,
+                   rows_aligned(r) ? 1 : 0};
+}
+
+// Splits of each tile's tokens: enough blocks for two waves, at least four
+// steps of tokens in each.
+int pick_splits(int B, int T, int H, int Hkv, int n) {
+  const long long tiles = ((long long)T * (H / Hkv) + kChunkRows - 1) / kChunkRows;
+  const long long blocks = tiles * B * Hkv;
+  const long long want = (4LL * device_sm_count() + blocks - 1) / std::max(1LL, blocks);
+  const long long most = std::max(1, n / (4 * kChunkTokens));
+  return (int)std::max(1LL, std::min({want, most, 64LL}));
+}
+
+} // namespace
+} // namespace kvfb
+
+using namespace kvfb;
+
+extern "C" int kvf_b200_chunk_splits(int B, int T, int H, int Hkv, int n, int fmt, int d, int dtype) {
+  if (B <= 0 || T <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || n <= 0 || fmt < 0 || fmt > 2 || (d != 64 && d != 128) ||
+      dtype < KVF_DT_F32 || dtype > KVF_DT_BF16)
+    return 1;
+  return pick_splits(B, T, H, Hkv, n);
+}
+
+extern "C" cudaError_t kvf_b200_chunk_attention(const kvf_args *args, int fmt, int d, int ord, int paged,
+                                                const kvf_heads *q, const kvf_heads *out, int T, const int *q_lens,
+                                                int causal, cudaStream_t stream) {
+  ChunkArgs a{};
+  cudaError_t e;
+  int group = 0;
+  if (T < 0 || (causal != 0 && causal != 1)) return cudaErrorInvalidValue;
+  if ((e = check_cache(args, fmt, d, ord, paged, a.cache, group)) != cudaSuccess) return e;
+  if (args->H <= 0 || args->H % args->Hkv || args->splits < 1) return cudaErrorInvalidValue;
+  if (args->B == 0 || T == 0) return cudaSuccess;
+  if ((e = check_heads(q)) != cudaSuccess || (e = check_heads(out)) != cudaSuccess) return e;
+  if (q->heads != args->H || out->heads != args->H || q->dtype != out->dtype) return cudaErrorInvalidValue;
+  if (paged && (long long)args->max_blocks << args->block_shift < args->n) return cudaErrorInvalidValue;
+  if (args->splits > 1 && (!args->part_o || !args->part_ml)) return cudaErrorInvalidValue;
+  if (args->splits > 1 && ((reinterpret_cast<uintptr_t>(args->part_o) & 15u) ||
+                           (reinterpret_cast<uintptr_t>(args->part_ml) & 7u)))
+    return cudaErrorMisalignedAddress;
+  a.q = chunk_rows(*q);
+  a.out = chunk_rows(*out);
+  a.B = args->B;
+  a.T = T;
+  a.H = args->H;
+  a.g = args->H / args->Hkv;
+  a.k = args->k;
+  a.v = args->v;
+  a.km = reinterpret_cast<const uint32_t *>(args->k_meta);
+  a.vm = reinterpret_cast<const uint32_t *>(args->v_meta);
+  a.gpr = group ? d / group : 0;
+  a.group_shift = group ? args->group_shift : 0;
+  a.seq_lens = args->seq_lens;
+  a.q_lens = q_lens;
+  a.causal = causal;
+  a.scale_log2 = args->scale_log2;
+  a.lse = args->lse;
+  a.splits = args->splits;
+  a.part_o = args->part_o;
+  a.part_ml = args->part_ml;
+  if ((long long)T * a.g > (1LL << 30)) return cudaErrorInvalidValue;
+  a.tiles = (T * a.g + kChunkRows - 1) / kChunkRows;
+  void *fn = fmt == KVF_FMT_F16    ? mma_fn<KVF_FMT_F16>(q->dtype, d)
+             : fmt == KVF_FMT_INT8 ? mma_fn<KVF_FMT_INT8>(q->dtype, d)
+                                   : mma_fn<KVF_FMT_INT4>(q->dtype, d);
+  const uint32_t smem = (uint32_t)chunk_mma_smem(d);
+  if ((e = ensure_kernel_smem(fn, smem)) != cudaSuccess) return e;
+  e = launch(fn, (long long)a.tiles * a.B * a.cache.Hkv * a.splits, kChunkThreads, smem, a, false, stream);
+  if (e != cudaSuccess || a.splits == 1) return e;
+  void *mf = d == 128 ? (q->dtype == KVF_DT_F32   ? merge_fn<KVF_DT_F32, 128>()
+                         : q->dtype == KVF_DT_F16 ? merge_fn<KVF_DT_F16, 128>()
+                                                  : merge_fn<KVF_DT_BF16, 128>())
+                      : (q->dtype == KVF_DT_F32   ? merge_fn<KVF_DT_F32, 64>()
+                         : q->dtype == KVF_DT_F16 ? merge_fn<KVF_DT_F16, 64>()
+                                                  : merge_fn<KVF_DT_BF16, 64>());
+  return launch(mf, ((long long)a.B * T * a.H + 3) / 4, 128, 0, a, true, stream);
+}

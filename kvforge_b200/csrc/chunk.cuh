@@ -1,0 +1,98 @@
+// chunk.cuh - attention of a chunk of new tokens over the cache: arguments,
+// lengths, masks and cache rows shared by its kernels.
+//
+//   s[r][t] = scale * q_r . k_t                 t < seen(r)
+//   out[r]  = sum_t softmax(s[r])_t v_t         0 where seen(r) = 0
+//   lse[r]  = log2 sum_t 2^(s[r][t] log2 e)
+//
+// A block takes a tile of rows of one (sequence, KV head): row r is query head
+// r mod g of new token r / g (g query heads share the KV head, so a tile's K
+// and V rows are read once for all of them). With kv tokens stored and ql new
+// ones, token j is token kv - ql + j of its sequence: seen = kv - ql + j + 1
+// (causal) or kv. Few tiles over a long cache are split along the tokens; the
+// splits' unnormalised outputs, maxima and sums are combined by chunk_merge.
+#pragma once
+
+#include "heads.cuh"
+#include "ptx.cuh"
+#include "quantize.cuh"
+
+namespace kvfb {
+namespace {
+
+struct ChunkRows {
+  uint8_t *p;
+  long long sb, st, sh;  // strides in bytes
+  int vec;               // rows start on 16-byte boundaries
+};
+
+struct ChunkArgs {
+  ChunkRows q, out;
+  int B, T, H, g;
+  CacheRows cache;       // Hkv, n
+  const uint8_t *k, *v;
+  const uint32_t *km, *vm;
+  int gpr, group_shift;
+  const int *seq_lens, *q_lens;
+  int causal;
+  float scale_log2;
+  float *lse;            // [B][T][H] or null
+  int splits, tiles;     // tiles: row tiles of a sequence's T tokens
+  float *part_o;         // [B][T][H][splits][D]
+  float *part_ml;        // [B][T][H][splits][2]
+};
+
+// What a block works on: sequence, KV head, first row, lengths, and its range
+// of tokens [t0, t1).
+struct ChunkWork {
+  int b, h, row0, rows;  // rows: valid rows from row0 on (<= tile height)
+  int ql, kv, split;
+  int t0, t1;
+  int seen0;             // tokens that row0 sees
+};
+
+__device__ __forceinline__ int chunk_seen(const ChunkArgs &a, const ChunkWork &w, int row) {
+  if (!a.causal) return w.kv;
+  const int s = w.kv - w.ql + row / a.g + 1;
+  return s < 0 ? 0 : s;
+}
+
+// False if the block has no rows. Longest rows first: the tiles of a sequence
+// are taken from its end, where a causal tile sees most. A tile's tokens are
+// shared evenly among its splits in whole steps of `step` tokens.
+__device__ __forceinline__ bool chunk_work(const ChunkArgs &a, int height, int step, ChunkWork &w) {
+  long long i = blockIdx.x;
+  w.split = (int)(i % a.splits);
+  i /= a.splits;
+  w.h = (int)(i % a.cache.Hkv);
+  i /= a.cache.Hkv;
+  w.b = (int)(i % a.B);
+  const int tile = a.tiles - 1 - (int)(i / a.B);
+  w.ql = a.q_lens ? min(max(a.q_lens[w.b], 0), a.T) : a.T;
+  w.kv = a.seq_lens ? min(max(a.seq_lens[w.b], 0), a.cache.n) : a.cache.n;
+  w.row0 = tile * height;
+  w.rows = min(height, w.ql * a.g - w.row0);
+  if (w.rows <= 0) return false;
+  const int seen = chunk_seen(a, w, w.row0 + w.rows - 1);
+  const int steps = (seen + step - 1) / step;
+  const int each = (steps + a.splits - 1) / a.splits;
+  w.t0 = (int)min((long long)w.split * each * step, (long long)seen);
+  w.t1 = (int)min((long long)w.t0 + (long long)each * step, (long long)seen);
+  w.seen0 = chunk_seen(a, w, w.row0);
+  return true;
+}
+
+// Byte offset of row r of the tile in q or out.
+__device__ __forceinline__ long long chunk_row(const ChunkRows &x, const ChunkArgs &a, const ChunkWork &w, int r) {
+  const int row = w.row0 + r, j = row / a.g;
+  return w.b * x.sb + j * x.st + (long long)(w.h * a.g + row - j * a.g) * x.sh;
+}
+
+// Index of row r in lse and in the split partials.
+__device__ __forceinline__ long long chunk_index(const ChunkArgs &a, const ChunkWork &w, int r) {
+  const int row = w.row0 + r, j = row / a.g;
+  return ((long long)w.b * a.T + j) * a.H + w.h * a.g + (row - j * a.g);
+}
+
+} // namespace
+} // namespace kvfb

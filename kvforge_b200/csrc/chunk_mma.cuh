@@ -1,0 +1,282 @@
+// chunk_mma.cuh - attention of a chunk on mma.sync in fp32 accuracy: every type
+// of query, every cache format, both head widths.
+//
+// Each operand x is split into two tf32 numbers, hi = tf32(x) and lo = x - hi
+// (11 significant bits each, the exponent range of fp32, so nothing has to be
+// scaled), and a product is hi*hi + lo*hi + hi*lo accumulated in fp32: relative
+// error about 2^-21 per product. f16 caches need no lo for K and V, whose 11
+// bits tf32 holds.
+//
+// Four warps of 16 rows share tiles of 64 tokens, dequantised to fp32 in shared
+// memory. Scores stay in registers: the fragment that the score product leaves
+// (rows x two adjacent tokens) is taken as it is for the operand of the value
+// product, whose k index then runs over tokens 2t and 2t + 1 instead of t and
+// t + 4, and V's rows are fetched in the same order.
+#pragma once
+
+#include "chunk.cuh"
+
+namespace kvfb {
+namespace {
+
+constexpr int kChunkRows = 64;    // rows of a tile
+constexpr int kChunkTokens = 64;  // tokens per step
+constexpr int kChunkThreads = 128;
+
+__host__ __device__ constexpr int chunk_mma_smem(int d) {
+  // q and k rows of d + 8 floats (conflict-free 8-byte reads), v rows of d + 4
+  return (kChunkRows * (d + 8) + kChunkTokens * (d + 8) + kChunkTokens * (d + 4)) * 4 + 16;
+}
+
+__device__ __forceinline__ uint32_t tf32(float x) {
+  uint32_t r;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
+  return r;
+}
+
+// x = hi + lo; an infinity or NaN stays in hi alone.
+__device__ __forceinline__ void split(float x, uint32_t &hi, uint32_t &lo) {
+  hi = tf32(x);
+  const float r = __fsub_rn(x, __uint_as_float(hi));
+  lo = fabsf(r) < INFINITY ? tf32(r) : 0u;
+}
+
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+
+// Eight channels of cache row `row` (from channel 8 * li) as fp32.
+template <int FMT, int D>
+__device__ __forceinline__ void cache8(const uint8_t *data, const uint32_t *meta, const ChunkArgs &a, long long row,
+                                       int li, float (&x)[8]) {
+  if (FMT == KVF_FMT_F16) {
+    const uint4 r = __ldg(reinterpret_cast<const uint4 *>(data + row * (2 * D)) + li);
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 f = widen2<KVF_DT_F16>(w[k]);
+      x[2 * k] = f.x;
+      x[2 * k + 1] = f.y;
+    }
+    return;
+  }
+  uint2 r;
+  if (FMT == KVF_FMT_INT8) {
+    r = __ldg(reinterpret_cast<const uint2 *>(data + row * D) + li);
+  } else {
+    r.x = __ldg(reinterpret_cast<const uint32_t *>(data + row * (D / 2)) + li);
+    r.y = 0;
+  }
+  const uint32_t m = __ldg(meta + row * a.gpr + ((8 * li) >> a.group_shift));
+  const __half2 sz = *reinterpret_cast<const __half2 *>(&m);
+  const float sc = __low2float(sz), zero = __high2float(sz);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const uint32_t c = FMT == KVF_FMT_INT8 ? ((k < 4 ? r.x : r.y) >> (8 * (k & 3))) & 255u : (r.x >> (4 * k)) & 15u;
+    x[k] = __fmaf_rn((float)c, sc, zero);
+  }
+}
+
+template <int FMT, int DT, int D>
+__global__ void __launch_bounds__(kChunkThreads) chunk_mma_kernel(const ChunkArgs a) {
+  constexpr int QS = D + 8, KS = D + 8, VS = D + 4;
+  constexpr bool LO = FMT != KVF_FMT_F16;  // K and V need their lo halves
+  extern __shared__ __align__(16) float sm[];
+  float *sq = sm, *sk = sq + kChunkRows * QS, *sv = sk + kChunkTokens * KS;
+  int *odd = reinterpret_cast<int *>(sv + kChunkTokens * VS);  // V rows of the step hold an infinity or NaN
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g4 = lane >> 2, t4 = lane & 3;
+
+  ChunkWork w;
+  if (!chunk_work(a, kChunkRows, kChunkTokens, w)) return;
+
+  for (int i = tid; i < kChunkRows * (D / 8); i += kChunkThreads) {
+    const int r = i / (D / 8), li = i % (D / 8);
+    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (r < w.rows) load8<DT>(a.q.p + chunk_row(a.q, a, w, r) + 8 * li * dtype_bytes(DT), a.q.vec, x);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sq[r * QS + 8 * li + k] = x[k];
+  }
+
+  const int r_lo = warp * 16 + g4, r_hi = r_lo + 8;
+  const int seen_lo = r_lo < w.rows ? chunk_seen(a, w, w.row0 + r_lo) : 0;
+  const int seen_hi = r_hi < w.rows ? chunk_seen(a, w, w.row0 + r_hi) : 0;
+  float m_lo = -INFINITY, m_hi = -INFINITY, l_lo = 0.f, l_hi = 0.f;
+  float o[D / 8][4];
+#pragma unroll
+  for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[n][k] = 0.f;
+
+  for (int t = w.t0; t < w.t1; t += kChunkTokens) {
+    __syncthreads();
+    if (tid == 0) *odd = 0;
+    __syncthreads();
+    const bool masked = t + kChunkTokens > w.seen0;  // some row of the tile does not see all of the step
+    for (int i = tid; i < kChunkTokens * (D / 8); i += kChunkThreads) {
+      const int r = i / (D / 8), li = i % (D / 8);
+      float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      // rows past the last that anyone sees are zero, whatever the cache holds there
+      const long long row = t + r < w.t1 ? a.cache.row(w.b, w.h, t + r) : -1;
+      if (row >= 0) {
+        cache8<FMT, D>(a.k, a.km, a, row, li, x);
+        cache8<FMT, D>(a.v, a.vm, a, row, li, y);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        sk[r * KS + 8 * li + k] = x[k];
+        sv[r * VS + 8 * li + k] = y[k];
+        if (masked && !(fabsf(y[k]) < INFINITY)) *odd = 1;
+      }
+    }
+    __syncthreads();
+
+    float s[kChunkTokens / 8][4];
+#pragma unroll
+    for (int n = 0; n < kChunkTokens / 8; ++n)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s[n][k] = 0.f;
+#pragma unroll 2
+    for (int c = 0; c < D; c += 8) {
+      const float2 q0 = *reinterpret_cast<const float2 *>(sq + r_lo * QS + c + 2 * t4);
+      const float2 q1 = *reinterpret_cast<const float2 *>(sq + r_hi * QS + c + 2 * t4);
+      uint32_t qh[4], ql[4];
+      split(q0.x, qh[0], ql[0]);
+      split(q1.x, qh[1], ql[1]);
+      split(q0.y, qh[2], ql[2]);
+      split(q1.y, qh[3], ql[3]);
+#pragma unroll
+      for (int n = 0; n < kChunkTokens / 8; ++n) {
+        const float2 k2 = *reinterpret_cast<const float2 *>(sk + (8 * n + g4) * KS + c + 2 * t4);
+        uint32_t kh[2], kl[2];
+        split(k2.x, kh[0], kl[0]);
+        split(k2.y, kh[1], kl[1]);
+        if (DT != KVF_DT_BF16 && DT != KVF_DT_F16) mma_tf32(s[n], ql, kh);  // 16-bit queries are tf32 numbers
+        if (LO) mma_tf32(s[n], qh, kl);
+        mma_tf32(s[n], qh, kh);
+      }
+    }
+
+    float mx_lo = -INFINITY, mx_hi = -INFINITY;
+#pragma unroll
+    for (int n = 0; n < kChunkTokens / 8; ++n)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int tok = t + 8 * n + 2 * t4 + k;
+        s[n][k] = tok < seen_lo ? s[n][k] * a.scale_log2 : -INFINITY;
+        s[n][2 + k] = tok < seen_hi ? s[n][2 + k] * a.scale_log2 : -INFINITY;
+        mx_lo = fmaxf(mx_lo, s[n][k]);
+        mx_hi = fmaxf(mx_hi, s[n][2 + k]);
+      }
+#pragma unroll
+    for (int off = 1; off < 4; off <<= 1) {
+      mx_lo = fmaxf(mx_lo, __shfl_xor_sync(0xffffffffu, mx_lo, off));
+      mx_hi = fmaxf(mx_hi, __shfl_xor_sync(0xffffffffu, mx_hi, off));
+    }
+    // a row that has seen nothing keeps -inf; 0 stands in for it in the exponents
+    const float n_lo = fmaxf(m_lo, mx_lo), n_hi = fmaxf(m_hi, mx_hi);
+    const float b_lo = n_lo == -INFINITY ? 0.f : n_lo, b_hi = n_hi == -INFINITY ? 0.f : n_hi;
+    const float f_lo = exp2f(m_lo - b_lo), f_hi = exp2f(m_hi - b_hi);
+    m_lo = n_lo;
+    m_hi = n_hi;
+    l_lo *= f_lo;
+    l_hi *= f_hi;
+#pragma unroll
+    for (int n = 0; n < kChunkTokens / 8; ++n)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        s[n][k] = exp2f(s[n][k] - b_lo);
+        s[n][2 + k] = exp2f(s[n][2 + k] - b_hi);
+        l_lo += s[n][k];
+        l_hi += s[n][2 + k];
+      }
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n) {
+      o[n][0] *= f_lo;
+      o[n][1] *= f_lo;
+      o[n][2] *= f_hi;
+      o[n][3] *= f_hi;
+    }
+    if (*reinterpret_cast<volatile int *>(odd)) {
+      // 0 * inf would carry an infinity or NaN into rows that do not see its
+      // token: such a step is added token by token, each row what it sees.
+      for (int u = 0; u < kChunkTokens; ++u) {
+        const int src = (lane & ~3) + ((u & 7) >> 1);
+        float p_lo = 0.f, p_hi = 0.f;
+#pragma unroll
+        for (int n = 0; n < kChunkTokens / 8; ++n) {
+          const float x0 = __shfl_sync(0xffffffffu, (u & 1) ? s[n][1] : s[n][0], src);
+          const float x1 = __shfl_sync(0xffffffffu, (u & 1) ? s[n][3] : s[n][2], src);
+          if (n == (u >> 3)) {
+            p_lo = x0;
+            p_hi = x1;
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float v = sv[u * VS + 8 * n + 2 * t4 + k];
+            if (t + u < seen_lo) o[n][k] = fmaf(p_lo, v, o[n][k]);
+            if (t + u < seen_hi) o[n][2 + k] = fmaf(p_hi, v, o[n][2 + k]);
+          }
+      }
+      continue;
+    }
+#pragma unroll
+    for (int u = 0; u < kChunkTokens / 8; ++u) {
+      uint32_t ph[4], pl[4];
+      split(s[u][0], ph[0], pl[0]);
+      split(s[u][2], ph[1], pl[1]);
+      split(s[u][1], ph[2], pl[2]);
+      split(s[u][3], ph[3], pl[3]);
+      const float *v0 = sv + (8 * u + 2 * t4) * VS + g4;
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n) {
+        uint32_t vh[2], vl[2];
+        split(v0[8 * n], vh[0], vl[0]);
+        split(v0[VS + 8 * n], vh[1], vl[1]);
+        mma_tf32(o[n], pl, vh);
+        if (LO) mma_tf32(o[n], ph, vl);
+        mma_tf32(o[n], ph, vh);
+      }
+    }
+  }
+
+#pragma unroll
+  for (int off = 1; off < 4; off <<= 1) {
+    l_lo += __shfl_xor_sync(0xffffffffu, l_lo, off);
+    l_hi += __shfl_xor_sync(0xffffffffu, l_hi, off);
+  }
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int r = half ? r_hi : r_lo;
+    if (r >= w.rows) continue;
+    const float m = half ? m_hi : m_lo, l = half ? l_hi : l_lo;
+    const long long at = chunk_index(a, w, r);
+    if (a.splits > 1) {
+      const long long part = at * a.splits + w.split;
+      float *po = a.part_o + part * D;
+      if (t4 == 0) *reinterpret_cast<float2 *>(a.part_ml + 2 * part) = make_float2(m, l);
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n)
+        *reinterpret_cast<float2 *>(po + 8 * n + 2 * t4) = make_float2(o[n][2 * half], o[n][2 * half + 1]);
+      continue;
+    }
+    // a row that sees nothing: zeros and -inf
+    const float inv = m == -INFINITY ? 0.f : 1.f / l;
+    if (a.lse && t4 == 0) a.lse[at] = m == -INFINITY ? -INFINITY : m + log2f(l);
+    using E = Elem<DT>;
+    typename E::T *out = reinterpret_cast<typename E::T *>(a.out.p + chunk_row(a.out, a, w, r));
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n) {
+      out[8 * n + 2 * t4] = E::from(o[n][2 * half] * inv);
+      out[8 * n + 2 * t4 + 1] = E::from(o[n][2 * half + 1] * inv);
+    }
+  }
+}
+
+} // namespace
+} // namespace kvfb

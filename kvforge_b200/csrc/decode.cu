@@ -1154,6 +1154,10 @@ extern "C" int kvf_b200_suggest_splits_ragged(int B, int H, int Hkv, int n, int 
 }
 
 namespace kvfb {
+// For the other translation units: this file's caches of driver facts.
+cudaError_t ensure_kernel_smem(void *fn, uint32_t smem) { return ensure_smem(fn, smem); }
+int device_sm_count() { return sm_count(); }
+
 unsigned take_append_errors();  // quantize.cu
 unsigned take_heads_errors();   // heads.cu
 }

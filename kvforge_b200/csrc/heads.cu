@@ -260,30 +260,6 @@ cudaError_t check_rope(const kvf_rope *r, int d, HeadsArgs &a) {
   return cudaSuccess;
 }
 
-// The cache half of a call's arguments: placement, payload and metadata, in
-// the formats that kvf_b200_decode reads.
-cudaError_t check_cache(const kvf_args *a, int fmt, int d, int ord, int paged, CacheRows &rows, int &group) {
-  if (!a || (d != 64 && d != 128) || fmt < 0 || fmt > 2 || (ord != KVF_ORD_HEAD && ord != KVF_ORD_TOKEN) ||
-      (paged != 0 && paged != 1) || a->B < 0 || a->Hkv <= 0 || a->n <= 0)
-    return cudaErrorInvalidValue;
-  group = 0;
-  if (fmt != KVF_FMT_F16) {
-    if (a->group_shift < 5 || a->group_shift > 7) return cudaErrorInvalidValue;
-    group = 1 << a->group_shift;
-    if (group > d || (fmt == KVF_FMT_INT8 && group < 64)) return cudaErrorInvalidValue;
-  }
-  if (paged && (a->block_shift < 0 || a->block_shift > 20 || a->max_blocks <= 0)) return cudaErrorInvalidValue;
-  if (a->B == 0) return cudaSuccess;
-  if (!a->k || !a->v || (group && (!a->k_meta || !a->v_meta)) || (paged && !a->block_table))
-    return cudaErrorInvalidValue;
-  if ((reinterpret_cast<uintptr_t>(a->k) | reinterpret_cast<uintptr_t>(a->v)) & 15u) return cudaErrorMisalignedAddress;
-  if (group && ((reinterpret_cast<uintptr_t>(a->k_meta) | reinterpret_cast<uintptr_t>(a->v_meta)) & 3u))
-    return cudaErrorMisalignedAddress;
-  rows = CacheRows{a->block_table, a->Hkv, a->n, ord == KVF_ORD_HEAD ? 1 : 0, paged, paged ? a->block_shift : 0,
-                   paged ? a->max_blocks : 0};
-  return cudaSuccess;
-}
-
 // ------------------------------------------------------------------ read back
 struct GatherArgs {
   Rows k, v;

@@ -81,3 +81,31 @@ def test_append_query_checks():
     for kw in (dict(pos=None), dict(q=q), dict(qo=q), dict(q=q, qo=heads(heads=16)), dict(q=heads(dtype=0), qo=heads(dtype=0)),
                dict(q=q, qo=heads(heads=32, dtype=0)), dict(qn=KvfNorm(FAKE, 0, 1e-6))):
         assert append(**kw) == INVALID, kw
+
+
+def chunk(a=None, fmt=1, d=128, ord=1, paged=1, q=None, out=None, T=3, causal=1):
+    a = cache(H=32, splits=1) if a is None else a
+    q = q or heads(heads=32)
+    return lib().kvf_b200_chunk_attention(ref(a), fmt, d, ord, paged, ref(q), ref(out or heads(heads=32)), T, None, causal,
+                                          None)
+
+
+def test_chunk_attention_checks():
+    good = dict(H=32, splits=1)
+    assert chunk(T=0) == 0 and chunk(a=cache(B=0, **good)) == 0
+    for kw in (dict(T=-1), dict(causal=2), dict(causal=-1), dict(fmt=3), dict(d=96), dict(ord=2), dict(paged=2),
+               dict(a=cache(H=30, splits=1)), dict(a=cache(H=32, splits=0)), dict(a=cache(H=0, splits=1)),
+               dict(a=cache(H=32, splits=2)), dict(a=cache(max_blocks=3, **good)), dict(a=cache(k=None, **good)),
+               dict(a=cache(group_shift=5, **good)), dict(q=heads(heads=16)), dict(out=heads(heads=32, dtype=1)),
+               dict(out=heads(heads=16)), dict(q=heads(heads=32, p=None)), dict(T=1 << 30)):
+        assert chunk(**kw) == INVALID, kw
+    for kw in (dict(a=cache(v=FAKE + 4, **good)), dict(out=heads(heads=32, p=FAKE + 1)),
+               dict(a=cache(H=32, splits=2, part_o=FAKE + 4, part_ml=FAKE))):
+        assert chunk(**kw) == MISALIGNED, kw
+
+
+def test_chunk_splits_needs_no_gpu():
+    f = lib().kvf_b200_chunk_splits
+    assert f(0, 1, 8, 8, 100, 0, 128, 0) == 1 and f(1, 1, 8, 3, 100, 0, 128, 0) == 1
+    assert f(1, 1, 8, 8, 100, 0, 128, 2) >= 1 and f(1, 4, 32, 8, 65536, 1, 128, 2) > 8
+    assert f(64, 4096, 32, 8, 65536, 1, 128, 2) == 1
