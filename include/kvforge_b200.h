@@ -300,7 +300,7 @@ cudaError_t kvf_b200_describe_path(const kvf_args *a, int fmt, int d, int ord, i
                                    int buf_len);
 
 /* Device-side error word of the current device, then cleared. Bit 0: a
- * shared-memory barrier wait in a decode kernel ran out of time (the kernel
+ * shared-memory barrier wait in a decode or chunk attention kernel ran out of time (the kernel
  * abandoned the step and its output is not valid). Bit 1: a cross-GPU wait
  * of kvf_b200_decode_exchange ran out of time (the affected output slices are
  * zero). Bit 2: kvf_b200_append, kvf_b200_append_rope, kvf_b200_norm_rope or
@@ -436,7 +436,9 @@ cudaError_t kvf_b200_gather(const kvf_args *a, int fmt, int d, int ord, int page
  * q, out, split_sem and max-splits rules of kvf_b200_decode do not apply. Blocks
  * that hold seen tokens must be mapped (a negative page's tokens count as
  * zero keys and values). Products of fp32 queries have fp32 accuracy (about
- * 2^-21 relative). */
+ * 2^-21 relative). For fp16 and bf16 queries keys, values and softmax weights
+ * are rounded to fp16 and the products accumulated in fp32: stored values past
+ * 65504 (which a quantized group can hold) count as infinities there. */
 cudaError_t kvf_b200_chunk_attention(const kvf_args *a, int fmt, int d, int ord, int paged, const kvf_heads *q,
                                      const kvf_heads *out, int T, const int *q_lens, int causal, cudaStream_t stream);
 

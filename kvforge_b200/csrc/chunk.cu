@@ -1,7 +1,9 @@
 // chunk.cu - attention of a chunk of new tokens over the cache
 // (kvf_b200_chunk_attention): checks, the choice of kernel and splits, launches
-// and the merge of splits. The kernels are in chunk_mma.cuh.
+// and the merge of splits. The kernels are in chunk_tc.cuh (fp16 and bf16
+// queries) and chunk_mma.cuh (fp32 queries).
 #include "chunk_mma.cuh"
+#include "chunk_tc.cuh"
 
 #include <algorithm>
 
@@ -52,15 +54,23 @@ __global__ void __launch_bounds__(128) chunk_merge(const ChunkArgs a) {
 
 template <int DT, int D> void *merge_fn() { return reinterpret_cast<void *>(&chunk_merge<DT, D>); }
 
-template <int FMT, int DT> void *mma_fn(int d) {
-  return d == 128 ? reinterpret_cast<void *>(&chunk_mma_kernel<FMT, DT, 128>)
-                  : reinterpret_cast<void *>(&chunk_mma_kernel<FMT, DT, 64>);
+template <int FMT> void *mma_fn(int d) {
+  return d == 128 ? reinterpret_cast<void *>(&chunk_mma_kernel<FMT, KVF_DT_F32, 128>)
+                  : reinterpret_cast<void *>(&chunk_mma_kernel<FMT, KVF_DT_F32, 64>);
 }
-template <int FMT> void *mma_fn(int dtype, int d) {
-  return dtype == KVF_DT_F32   ? mma_fn<FMT, KVF_DT_F32>(d)
-         : dtype == KVF_DT_F16 ? mma_fn<FMT, KVF_DT_F16>(d)
-                               : mma_fn<FMT, KVF_DT_BF16>(d);
+template <int FMT, int DT, int D> void *tc_fn(bool two) {
+  return two ? reinterpret_cast<void *>(&chunk_tc_kernel<FMT, DT, D, true>)
+             : reinterpret_cast<void *>(&chunk_tc_kernel<FMT, DT, D, false>);
 }
+template <int FMT> void *tc_fn(int dtype, int d, bool two) {
+  if (dtype == KVF_DT_F16) return d == 128 ? tc_fn<FMT, KVF_DT_F16, 128>(two) : tc_fn<FMT, KVF_DT_F16, 64>(two);
+  return d == 128 ? tc_fn<FMT, KVF_DT_BF16, 128>(two) : tc_fn<FMT, KVF_DT_BF16, 64>(two);
+}
+
+// Whether the two softmax groups of a tensor-core block take the steps of one
+// row tile in turn (as two splits) or a tile each. One tile has no second one
+// to hide its softmax behind.
+bool one_tile(long long rows, int splits) { return rows <= kTcRows && splits % 2 == 0; }
 
 cudaError_t launch(void *fn, long long blocks, int threads, uint32_t smem, const ChunkArgs &a, bool dependent,
                    cudaStream_t st) {
@@ -86,17 +96,46 @@ ChunkRows chunk_rows(const kvf_heads &r) {
                    rows_aligned(r) ? 1 : 0};
 }
 
-// Splits of each tile's tokens: enough blocks for two waves, at least four
-// steps of tokens in each.
-int pick_splits(int B, int T, int H, int Hkv, int n) {
-  const long long tiles = ((long long)T * (H / Hkv) + kChunkRows - 1) / kChunkRows;
-  const long long blocks = tiles * B * Hkv;
-  const long long want = (4LL * device_sm_count() + blocks - 1) / std::max(1LL, blocks);
-  const long long most = std::max(1, n / (4 * kChunkTokens));
-  return (int)std::max(1LL, std::min({want, most, 64LL}));
+// Splits of each tile's tokens. Tensor-core kernel: the blocks run one per SM,
+// a block costs its steps and about three more to start and end; the count
+// that makes the waves shortest.
+int pick_splits(int B, int T, int H, int Hkv, int n, int dtype) {
+  const long long rows = (long long)T * (H / Hkv);
+  const int sms = device_sm_count();
+  if (dtype == KVF_DT_F32) {
+    // two waves of blocks (two per SM), at least four steps of tokens in each
+    const long long blocks = (rows + kChunkRows - 1) / kChunkRows * B * Hkv;
+    const long long want = (4LL * sms + blocks - 1) / blocks;
+    return (int)std::max(1LL, std::min({want, (long long)n / (4 * kChunkTokens), 64LL}));
+  }
+  const bool one = rows <= kTcRows;
+  const long long blocks = (rows + 2 * kTcRows - 1) / (2 * kTcRows) * B * Hkv;
+  const int steps = (n + kTcStep - 1) / kTcStep;
+  long long best = -1;
+  int s = 1;
+  for (int k = 1; k <= std::min(64, std::max(1, steps / 2)); ++k) {
+    const long long cost = (blocks * k + sms - 1) / sms * ((steps + k - 1) / k + 3 + (k > 1 ? 2 : 0));
+    if (best < 0 || cost < best) {
+      best = cost;
+      s = k;
+    }
+  }
+  return one ? 2 * s : s;
 }
 
 } // namespace
+
+// Nonzero if a bounded wait ran out since the last call (then cleared).
+unsigned take_chunk_errors() {
+  unsigned v = 0, zero = 0;
+  if (cudaMemcpyFromSymbol(&v, g_kvfb_chunk_error, sizeof(v)) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  if (v) cudaMemcpyToSymbol(g_kvfb_chunk_error, &zero, sizeof(zero));
+  return v;
+}
+
 } // namespace kvfb
 
 using namespace kvfb;
@@ -105,7 +144,7 @@ extern "C" int kvf_b200_chunk_splits(int B, int T, int H, int Hkv, int n, int fm
   if (B <= 0 || T <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || n <= 0 || fmt < 0 || fmt > 2 || (d != 64 && d != 128) ||
       dtype < KVF_DT_F32 || dtype > KVF_DT_BF16)
     return 1;
-  return pick_splits(B, T, H, Hkv, n);
+  return pick_splits(B, T, H, Hkv, n, dtype);
 }
 
 extern "C" cudaError_t kvf_b200_chunk_attention(const kvf_args *args, int fmt, int d, int ord, int paged,
@@ -120,6 +159,9 @@ extern "C" cudaError_t kvf_b200_chunk_attention(const kvf_args *args, int fmt, i
   if (args->B == 0 || T == 0) return cudaSuccess;
   if ((e = check_heads(q)) != cudaSuccess || (e = check_heads(out)) != cudaSuccess) return e;
   if (q->heads != args->H || out->heads != args->H || q->dtype != out->dtype) return cudaErrorInvalidValue;
+  if (group && ((reinterpret_cast<uintptr_t>(args->k_meta) | reinterpret_cast<uintptr_t>(args->v_meta)) &
+                (uintptr_t)(4 * (d / group) - 1)))
+    return cudaErrorMisalignedAddress;
   if (paged && (long long)args->max_blocks << args->block_shift < args->n) return cudaErrorInvalidValue;
   if (args->splits > 1 && (!args->part_o || !args->part_ml)) return cudaErrorInvalidValue;
   if (args->splits > 1 && ((reinterpret_cast<uintptr_t>(args->part_o) & 15u) ||
@@ -146,13 +188,28 @@ extern "C" cudaError_t kvf_b200_chunk_attention(const kvf_args *args, int fmt, i
   a.part_o = args->part_o;
   a.part_ml = args->part_ml;
   if ((long long)T * a.g > (1LL << 30)) return cudaErrorInvalidValue;
-  a.tiles = (T * a.g + kChunkRows - 1) / kChunkRows;
-  void *fn = fmt == KVF_FMT_F16    ? mma_fn<KVF_FMT_F16>(q->dtype, d)
-             : fmt == KVF_FMT_INT8 ? mma_fn<KVF_FMT_INT8>(q->dtype, d)
-                                   : mma_fn<KVF_FMT_INT4>(q->dtype, d);
-  const uint32_t smem = (uint32_t)chunk_mma_smem(d);
+  void *fn;
+  uint32_t smem;
+  int threads;
+  long long blocks;
+  if (q->dtype == KVF_DT_F32) {
+    fn = fmt == KVF_FMT_F16 ? mma_fn<KVF_FMT_F16>(d) : fmt == KVF_FMT_INT8 ? mma_fn<KVF_FMT_INT8>(d) : mma_fn<KVF_FMT_INT4>(d);
+    smem = (uint32_t)chunk_mma_smem(d);
+    threads = kChunkThreads;
+    a.tiles = (T * a.g + kChunkRows - 1) / kChunkRows;
+    blocks = (long long)a.tiles * a.B * a.cache.Hkv * a.splits;
+  } else {
+    const bool two = !one_tile((long long)T * a.g, a.splits);
+    fn = fmt == KVF_FMT_F16    ? tc_fn<KVF_FMT_F16>(q->dtype, d, two)
+         : fmt == KVF_FMT_INT8 ? tc_fn<KVF_FMT_INT8>(q->dtype, d, two)
+                               : tc_fn<KVF_FMT_INT4>(q->dtype, d, two);
+    smem = tc_smem_bytes(fmt, d, two);
+    threads = kTcThreads;
+    a.tiles = (T * a.g + 2 * kTcRows - 1) / (2 * kTcRows);
+    blocks = (long long)a.tiles * a.B * a.cache.Hkv * (two ? a.splits : a.splits / 2);
+  }
   if ((e = ensure_kernel_smem(fn, smem)) != cudaSuccess) return e;
-  e = launch(fn, (long long)a.tiles * a.B * a.cache.Hkv * a.splits, kChunkThreads, smem, a, false, stream);
+  e = launch(fn, blocks, threads, smem, a, false, stream);
   if (e != cudaSuccess || a.splits == 1) return e;
   void *mf = d == 128 ? (q->dtype == KVF_DT_F32   ? merge_fn<KVF_DT_F32, 128>()
                          : q->dtype == KVF_DT_F16 ? merge_fn<KVF_DT_F16, 128>()

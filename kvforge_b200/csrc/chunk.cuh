@@ -59,11 +59,11 @@ __device__ __forceinline__ int chunk_seen(const ChunkArgs &a, const ChunkWork &w
 
 // False if the block has no rows. Longest rows first: the tiles of a sequence
 // are taken from its end, where a causal tile sees most. A tile's tokens are
-// shared evenly among its splits in whole steps of `step` tokens.
-__device__ __forceinline__ bool chunk_work(const ChunkArgs &a, int height, int step, ChunkWork &w) {
+// shared evenly among `splits` blocks in whole steps of `step` tokens.
+__device__ __forceinline__ bool chunk_work(const ChunkArgs &a, int splits, int height, int step, ChunkWork &w) {
   long long i = blockIdx.x;
-  w.split = (int)(i % a.splits);
-  i /= a.splits;
+  w.split = (int)(i % splits);
+  i /= splits;
   w.h = (int)(i % a.cache.Hkv);
   i /= a.cache.Hkv;
   w.b = (int)(i % a.B);
@@ -75,7 +75,7 @@ __device__ __forceinline__ bool chunk_work(const ChunkArgs &a, int height, int s
   if (w.rows <= 0) return false;
   const int seen = chunk_seen(a, w, w.row0 + w.rows - 1);
   const int steps = (seen + step - 1) / step;
-  const int each = (steps + a.splits - 1) / a.splits;
+  const int each = (steps + splits - 1) / splits;
   w.t0 = (int)min((long long)w.split * each * step, (long long)seen);
   w.t1 = (int)min((long long)w.t0 + (long long)each * step, (long long)seen);
   w.seen0 = chunk_seen(a, w, w.row0);
@@ -92,6 +92,38 @@ __device__ __forceinline__ long long chunk_row(const ChunkRows &x, const ChunkAr
 __device__ __forceinline__ long long chunk_index(const ChunkArgs &a, const ChunkWork &w, int r) {
   const int row = w.row0 + r, j = row / a.g;
   return ((long long)w.b * a.T + j) * a.H + w.h * a.g + (row - j * a.g);
+}
+
+// Eight channels of cache row `row` (from channel 8 * li) as fp32.
+template <int FMT, int D>
+__device__ __forceinline__ void cache8(const uint8_t *data, const uint32_t *meta, const ChunkArgs &a, long long row,
+                                       int li, float (&x)[8]) {
+  if (FMT == KVF_FMT_F16) {
+    const uint4 r = __ldg(reinterpret_cast<const uint4 *>(data + row * (2 * D)) + li);
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 f = widen2<KVF_DT_F16>(w[k]);
+      x[2 * k] = f.x;
+      x[2 * k + 1] = f.y;
+    }
+    return;
+  }
+  uint2 r;
+  if (FMT == KVF_FMT_INT8) {
+    r = __ldg(reinterpret_cast<const uint2 *>(data + row * D) + li);
+  } else {
+    r.x = __ldg(reinterpret_cast<const uint32_t *>(data + row * (D / 2)) + li);
+    r.y = 0;
+  }
+  const uint32_t m = __ldg(meta + row * a.gpr + ((8 * li) >> a.group_shift));
+  const __half2 sz = *reinterpret_cast<const __half2 *>(&m);
+  const float sc = __low2float(sz), zero = __high2float(sz);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const uint32_t c = FMT == KVF_FMT_INT8 ? ((k < 4 ? r.x : r.y) >> (8 * (k & 3))) & 255u : (r.x >> (4 * k)) & 15u;
+    x[k] = __fmaf_rn((float)c, sc, zero);
+  }
 }
 
 } // namespace

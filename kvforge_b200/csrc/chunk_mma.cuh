@@ -48,38 +48,6 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], 
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
 
-// Eight channels of cache row `row` (from channel 8 * li) as fp32.
-template <int FMT, int D>
-__device__ __forceinline__ void cache8(const uint8_t *data, const uint32_t *meta, const ChunkArgs &a, long long row,
-                                       int li, float (&x)[8]) {
-  if (FMT == KVF_FMT_F16) {
-    const uint4 r = __ldg(reinterpret_cast<const uint4 *>(data + row * (2 * D)) + li);
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float2 f = widen2<KVF_DT_F16>(w[k]);
-      x[2 * k] = f.x;
-      x[2 * k + 1] = f.y;
-    }
-    return;
-  }
-  uint2 r;
-  if (FMT == KVF_FMT_INT8) {
-    r = __ldg(reinterpret_cast<const uint2 *>(data + row * D) + li);
-  } else {
-    r.x = __ldg(reinterpret_cast<const uint32_t *>(data + row * (D / 2)) + li);
-    r.y = 0;
-  }
-  const uint32_t m = __ldg(meta + row * a.gpr + ((8 * li) >> a.group_shift));
-  const __half2 sz = *reinterpret_cast<const __half2 *>(&m);
-  const float sc = __low2float(sz), zero = __high2float(sz);
-#pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const uint32_t c = FMT == KVF_FMT_INT8 ? ((k < 4 ? r.x : r.y) >> (8 * (k & 3))) & 255u : (r.x >> (4 * k)) & 15u;
-    x[k] = __fmaf_rn((float)c, sc, zero);
-  }
-}
-
 template <int FMT, int DT, int D>
 __global__ void __launch_bounds__(kChunkThreads) chunk_mma_kernel(const ChunkArgs a) {
   constexpr int QS = D + 8, KS = D + 8, VS = D + 4;
@@ -90,7 +58,7 @@ __global__ void __launch_bounds__(kChunkThreads) chunk_mma_kernel(const ChunkArg
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g4 = lane >> 2, t4 = lane & 3;
 
   ChunkWork w;
-  if (!chunk_work(a, kChunkRows, kChunkTokens, w)) return;
+  if (!chunk_work(a, a.splits, kChunkRows, kChunkTokens, w)) return;
 
   for (int i = tid; i < kChunkRows * (D / 8); i += kChunkThreads) {
     const int r = i / (D / 8), li = i % (D / 8);

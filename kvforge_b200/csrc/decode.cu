@@ -1160,6 +1160,7 @@ int device_sm_count() { return sm_count(); }
 
 unsigned take_append_errors();  // quantize.cu
 unsigned take_heads_errors();   // heads.cu
+unsigned take_chunk_errors();   // chunk.cu
 }
 
 extern "C" unsigned kvf_b200_device_errors(void) {
@@ -1170,6 +1171,7 @@ extern "C" unsigned kvf_b200_device_errors(void) {
   }
   if (v) cudaMemcpyToSymbol(g_kvfb_error, &zero, sizeof(zero));
   if (kvfb::take_append_errors()) v |= 4u;  // an appended row fell outside the cache
+  if (kvfb::take_chunk_errors()) v |= 1u;   // a bounded wait ran out
   if (kvfb::take_heads_errors()) v |= 4u;   // a token outside the cache or the rotation table
   return v;
 }

@@ -195,6 +195,15 @@ __device__ __forceinline__ void cp_async_8_zfill(uint32_t dst, const void *src, 
 __device__ __forceinline__ void cp_async_4_zfill(uint32_t dst, const void *src, uint32_t bytes) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
+// 16-byte form; also the commit of the copies issued so far into a group and
+// the wait until at most N groups are in flight.
+__device__ __forceinline__ void cp_async_16_zfill(uint32_t dst, const void *src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
 // mbar_arrive_expect_tx by the threads for which `pred` holds.
 __device__ __forceinline__ void mbar_arrive_expect_tx_if(uint32_t bar, uint32_t bytes, bool pred) {
   asm volatile(
