@@ -11,6 +11,8 @@ namespace kvfb {
 
 cudaError_t ensure_kernel_smem(void *fn, uint32_t smem);  // decode.cu
 int device_sm_count();                                    // decode.cu
+cudaError_t encode_cache_maps(const kvf_args *a, int fmt, int d, int ord, int paged, int tbox, CUtensorMap &k,
+                              CUtensorMap &v);            // decode.cu
 
 namespace {
 
@@ -58,13 +60,21 @@ template <int FMT> void *mma_fn(int d) {
   return d == 128 ? reinterpret_cast<void *>(&chunk_mma_kernel<FMT, KVF_DT_F32, 128>)
                   : reinterpret_cast<void *>(&chunk_mma_kernel<FMT, KVF_DT_F32, 64>);
 }
-template <int FMT, int DT, int D> void *tc_fn(bool two) {
-  return two ? reinterpret_cast<void *>(&chunk_tc_kernel<FMT, DT, D, true>)
-             : reinterpret_cast<void *>(&chunk_tc_kernel<FMT, DT, D, false>);
+struct TcVariant {
+  void *fn;
+  int threads;
+  uint32_t smem;
+};
+template <int FMT, int DT, int D, bool TWO> TcVariant tc_variant() {
+  using L = TcLayout<FMT, D, TWO>;
+  return {reinterpret_cast<void *>(&chunk_tc_kernel<FMT, DT, D, TWO>), L::THREADS, L::BYTES};
 }
-template <int FMT> void *tc_fn(int dtype, int d, bool two) {
-  if (dtype == KVF_DT_F16) return d == 128 ? tc_fn<FMT, KVF_DT_F16, 128>(two) : tc_fn<FMT, KVF_DT_F16, 64>(two);
-  return d == 128 ? tc_fn<FMT, KVF_DT_BF16, 128>(two) : tc_fn<FMT, KVF_DT_BF16, 64>(two);
+template <int FMT, int DT> TcVariant tc_variant(int d, bool two) {
+  if (d == 128) return two ? tc_variant<FMT, DT, 128, true>() : tc_variant<FMT, DT, 128, false>();
+  return two ? tc_variant<FMT, DT, 64, true>() : tc_variant<FMT, DT, 64, false>();
+}
+template <int FMT> TcVariant tc_variant(int dtype, int d, bool two) {
+  return dtype == KVF_DT_F16 ? tc_variant<FMT, KVF_DT_F16>(d, two) : tc_variant<FMT, KVF_DT_BF16>(d, two);
 }
 
 // Whether the two softmax groups of a tensor-core block take the steps of one
@@ -72,8 +82,9 @@ template <int FMT> void *tc_fn(int dtype, int d, bool two) {
 // to hide its softmax behind.
 bool one_tile(long long rows, int splits) { return rows <= kTcRows && splits % 2 == 0; }
 
-cudaError_t launch(void *fn, long long blocks, int threads, uint32_t smem, const ChunkArgs &a, bool dependent,
-                   cudaStream_t st) {
+// Launches fn(a) or fn(a, maps[0], maps[1]).
+cudaError_t launch(void *fn, long long blocks, int threads, uint32_t smem, const ChunkArgs &a, CUtensorMap *maps,
+                   bool dependent, cudaStream_t st) {
   if (blocks <= 0) return cudaSuccess;
   if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
   cudaLaunchConfig_t cfg{};
@@ -86,7 +97,7 @@ cudaError_t launch(void *fn, long long blocks, int threads, uint32_t smem, const
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = dependent ? 1 : 0;
-  void *params[] = {const_cast<ChunkArgs *>(&a)};
+  void *params[] = {const_cast<ChunkArgs *>(&a), maps, maps ? maps + 1 : nullptr};
   return cudaLaunchKernelExC(&cfg, fn, params);
 }
 
@@ -162,7 +173,9 @@ extern "C" cudaError_t kvf_b200_chunk_attention(const kvf_args *args, int fmt, i
   if (group && ((reinterpret_cast<uintptr_t>(args->k_meta) | reinterpret_cast<uintptr_t>(args->v_meta)) &
                 (uintptr_t)(4 * (d / group) - 1)))
     return cudaErrorMisalignedAddress;
-  if (paged && (long long)args->max_blocks << args->block_shift < args->n) return cudaErrorInvalidValue;
+  if (paged && (args->block_shift < 4 || args->block_shift > 7 ||
+                (long long)args->max_blocks << args->block_shift < args->n))
+    return cudaErrorInvalidValue;
   if (args->splits > 1 && (!args->part_o || !args->part_ml)) return cudaErrorInvalidValue;
   if (args->splits > 1 && ((reinterpret_cast<uintptr_t>(args->part_o) & 15u) ||
                            (reinterpret_cast<uintptr_t>(args->part_ml) & 7u)))
@@ -188,28 +201,27 @@ extern "C" cudaError_t kvf_b200_chunk_attention(const kvf_args *args, int fmt, i
   a.part_o = args->part_o;
   a.part_ml = args->part_ml;
   if ((long long)T * a.g > (1LL << 30)) return cudaErrorInvalidValue;
-  void *fn;
-  uint32_t smem;
-  int threads;
-  long long blocks;
   if (q->dtype == KVF_DT_F32) {
-    fn = fmt == KVF_FMT_F16 ? mma_fn<KVF_FMT_F16>(d) : fmt == KVF_FMT_INT8 ? mma_fn<KVF_FMT_INT8>(d) : mma_fn<KVF_FMT_INT4>(d);
-    smem = (uint32_t)chunk_mma_smem(d);
-    threads = kChunkThreads;
+    void *fn = fmt == KVF_FMT_F16    ? mma_fn<KVF_FMT_F16>(d)
+               : fmt == KVF_FMT_INT8 ? mma_fn<KVF_FMT_INT8>(d)
+                                     : mma_fn<KVF_FMT_INT4>(d);
+    const uint32_t smem = (uint32_t)chunk_mma_smem(d);
     a.tiles = (T * a.g + kChunkRows - 1) / kChunkRows;
-    blocks = (long long)a.tiles * a.B * a.cache.Hkv * a.splits;
+    if ((e = ensure_kernel_smem(fn, smem)) != cudaSuccess) return e;
+    e = launch(fn, (long long)a.tiles * a.B * a.cache.Hkv * a.splits, kChunkThreads, smem, a, nullptr, false, stream);
   } else {
     const bool two = !one_tile((long long)T * a.g, a.splits);
-    fn = fmt == KVF_FMT_F16    ? tc_fn<KVF_FMT_F16>(q->dtype, d, two)
-         : fmt == KVF_FMT_INT8 ? tc_fn<KVF_FMT_INT8>(q->dtype, d, two)
-                               : tc_fn<KVF_FMT_INT4>(q->dtype, d, two);
-    smem = tc_smem_bytes(fmt, d, two);
-    threads = kTcThreads;
+    const TcVariant x = fmt == KVF_FMT_F16    ? tc_variant<KVF_FMT_F16>(q->dtype, d, two)
+                        : fmt == KVF_FMT_INT8 ? tc_variant<KVF_FMT_INT8>(q->dtype, d, two)
+                                              : tc_variant<KVF_FMT_INT4>(q->dtype, d, two);
     a.tiles = (T * a.g + 2 * kTcRows - 1) / (2 * kTcRows);
-    blocks = (long long)a.tiles * a.B * a.cache.Hkv * (two ? a.splits : a.splits / 2);
+    CUtensorMap maps[2];
+    const int tbox = paged ? std::min(kTcHalf, 1 << args->block_shift) : kTcHalf;
+    if ((e = encode_cache_maps(args, fmt, d, ord, paged, tbox, maps[0], maps[1])) != cudaSuccess) return e;
+    if ((e = ensure_kernel_smem(x.fn, x.smem)) != cudaSuccess) return e;
+    e = launch(x.fn, (long long)a.tiles * a.B * a.cache.Hkv * (two ? a.splits : a.splits / 2), x.threads, x.smem, a, maps,
+               false, stream);
   }
-  if ((e = ensure_kernel_smem(fn, smem)) != cudaSuccess) return e;
-  e = launch(fn, blocks, threads, smem, a, false, stream);
   if (e != cudaSuccess || a.splits == 1) return e;
   void *mf = d == 128 ? (q->dtype == KVF_DT_F32   ? merge_fn<KVF_DT_F32, 128>()
                          : q->dtype == KVF_DT_F16 ? merge_fn<KVF_DT_F16, 128>()
@@ -217,5 +229,5 @@ extern "C" cudaError_t kvf_b200_chunk_attention(const kvf_args *args, int fmt, i
                       : (q->dtype == KVF_DT_F32   ? merge_fn<KVF_DT_F32, 64>()
                          : q->dtype == KVF_DT_F16 ? merge_fn<KVF_DT_F16, 64>()
                                                   : merge_fn<KVF_DT_BF16, 64>());
-  return launch(mf, ((long long)a.B * T * a.H + 3) / 4, 128, 0, a, true, stream);
+  return launch(mf, ((long long)a.B * T * a.H + 3) / 4, 128, 0, a, nullptr, true, stream);
 }

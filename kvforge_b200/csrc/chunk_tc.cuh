@@ -9,19 +9,22 @@
 // rounding. Softmax weights are rounded to fp16, their sum is kept in fp32 of
 // the unrounded ones. Both products accumulate in fp32.
 //
-// Warp roles (416 threads, one block per SM):
-//   warps 0-3, 4-7  two softmax groups, thread = row of a 128-row tile. TWO: each
-//                   has its own row tile and both take every step of 128 tokens;
-//                   else both have the same rows and take steps in turn, each
-//                   with its own output, as two splits. Either way one group's
-//                   softmax runs while the tensor cores work for the other;
-//   warps 8-11      loaders: rows come by cp.async from wherever their pages lie,
-//                   quantized ones into a staging area of the thread that also
-//                   converts them, into tiles of 128 tokens x 64 channels with the
-//                   128-byte swizzle; K and V tiles share a ring of four slots;
-//   warp 12         one thread issues the MMAs: S = Q K^T into tensor memory,
-//                   O += P V with P read from tensor memory, where the softmax
-//                   group writes it over its scores, and V read MN-major.
+// Warp groups (of 128 threads; one block per SM):
+//   0, 1   softmax, thread = row of a 128-row tile. TWO: each group has its own
+//          row tile and both take every step of 128 tokens; else both have the
+//          same rows and take steps in turn, each with its own output, as two
+//          splits. Either way one group's softmax runs while the tensor cores
+//          work for the other;
+//   2, 3   quantized caches: converters, one for K and one for V. Raw half steps
+//          (64 tokens) land in a ring of their own and become fp16 tiles of 128
+//          tokens x 64 channels with the 128-byte swizzle. f16 caches: TMA writes
+//          those tiles itself, and group 2 only clears what must not be seen;
+//   last   one warp issues the MMAs (one thread): S = Q K^T into tensor memory,
+//          O += P V with P read from tensor memory, where the softmax group writes
+//          it over its scores, and V read MN-major. Two warps are the producers of K
+//          and of V: TMA boxes per page, metadata rows by cp.async. A box of tokens
+//          that nobody sees, or of a block mapped to a negative page, is asked for
+//          at page -1, which TMA fills with zeros.
 // The running maximum a row's weights are taken against is raised only when a
 // step exceeds it by more than 2^8 (weights up to 256 fit fp16, and their sum
 // fp32), so the output in tensor memory is rescaled rarely and a step's scores
@@ -31,6 +34,8 @@
 
 #include "chunk.cuh"
 #include "tc.cuh"
+
+#include <cuda.h>
 
 namespace kvfb {
 
@@ -42,31 +47,56 @@ namespace {
 
 constexpr int kTcRows = 128;    // rows of a tile
 constexpr int kTcStep = 128;    // tokens of a step
-constexpr int kTcThreads = 416;
-constexpr int kTcLoadWarp = 8;  // to 11
-constexpr int kTcMmaWarp = 12;
-constexpr int kTcSlots = 4;
-constexpr int kTcStages = 2;    // staged items of a quantized cache
+constexpr int kTcHalf = 64;     // tokens of a raw half step
 constexpr float kTcLazy = 8.f;  // log2 of the most a weight may exceed 1 by
-
-struct TcShared {
-  uint64_t bars[16];  // full[4], empty[4], sfull[2], pready[2], ofull[2], done
-  uint32_t tmem;
-  int abort_flag;
-  int odd;            // a masked V tile held an infinity or NaN, taken as 0
-};
 
 __host__ __device__ constexpr int cache_row_bytes(int fmt, int d) {
   return fmt == KVF_FMT_F16 ? 2 * d : fmt == KVF_FMT_INT8 ? d : d / 2;
 }
-__host__ __device__ constexpr uint32_t tc_tile_bytes(int d) { return (uint32_t)(kTcStep * d * 2); }
-// One staged item: raw rows, then their metadata words.
-__host__ __device__ constexpr uint32_t tc_stage_bytes(int fmt, int d) {
-  return fmt == KVF_FMT_F16 ? 0u : (uint32_t)(kTcStep * cache_row_bytes(fmt, d) + kTcStep * (fmt == KVF_FMT_INT8 ? 8 : 16));
+
+// Shared memory of a variant: query tiles, then rings of fp16 tiles for K and
+// for V, then rings of raw half steps with their metadata, as deep as fits.
+template <int FMT, int D, bool TWO> struct TcLayout {
+  static constexpr bool RAW = FMT != KVF_FMT_F16;
+  static constexpr int GROUPS = RAW ? 5 : 4;                 // warp groups
+  static constexpr int THREADS = 128 * GROUPS;
+  // Registers per thread after the start: the block is launched with 96 (five
+  // groups) or 128 (four), and the groups' shares add up to no more than that.
+  static constexpr int SOFT_REGS = RAW ? 136 : 168, CONV_REGS = 72, LAST_REGS = RAW ? 64 : 96;
+  static_assert(2 * SOFT_REGS + (RAW ? 2 : 1) * CONV_REGS + LAST_REGS <= (RAW ? 96 * 5 : 128 * 4), "registers");
+  static constexpr uint32_t TILE = kTcStep * D * 2;
+  static constexpr uint32_t QB = (TWO ? 2u : 1u) * TILE;
+  static constexpr int SLOTS = RAW || TWO ? 2 : 3;           // fp16 tiles per operand
+  static constexpr uint32_t RAWB = RAW ? kTcHalf * (uint32_t)cache_row_bytes(FMT, D) : 0u;
+  static constexpr uint32_t METAB = RAW ? kTcHalf * (FMT == KVF_FMT_INT8 ? 8u : 16u) : 0u;
+  static constexpr uint32_t FREE = 232448u - 1024u - QB - 2u * SLOTS * TILE;
+  static constexpr int FIT = RAW ? (int)(FREE / (2u * (RAWB + METAB))) : 0;
+  static constexpr int RSLOTS = FIT > 8 ? 8 : FIT;           // raw half steps per operand
+  static constexpr uint32_t OFF_RING = QB;
+  static constexpr uint32_t OFF_RAW = OFF_RING + 2u * SLOTS * TILE;
+  static constexpr uint32_t OFF_META = OFF_RAW + 2u * RSLOTS * RAWB;
+  static constexpr uint32_t OFF_MISC = OFF_META + 2u * RSLOTS * METAB;
+  static constexpr uint32_t BYTES = OFF_MISC + 512u;
+  static_assert(!RAW || RSLOTS >= 2, "two raw half steps per operand");
+  static_assert(BYTES <= 232448u, "shared memory");
+};
+
+struct TcShared {
+  uint64_t kfull[3], kempty[3], vfull[3], vempty[3];
+  uint64_t sfull[2], pready[2], ofull[2];
+  uint64_t vraw[3], vfixed[3], done;  // vraw, vfixed: f16 V tiles on their way through group 2
+  uint64_t rfull[2][8], rempty[2][8];
+  uint32_t tmem;
+  int abort_flag;
+  int odd;            // a masked V tile held an infinity or NaN, taken as 0
+};
+static_assert(sizeof(TcShared) <= 512, "misc area");
+
+template <int N> __device__ __forceinline__ void regs_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
 }
-__host__ __device__ constexpr uint32_t tc_smem_bytes(int fmt, int d, bool two) {
-  return (two ? 2u : 1u) * tc_tile_bytes(d) + kTcSlots * tc_tile_bytes(d) + kTcStages * tc_stage_bytes(fmt, d) +
-         (uint32_t)sizeof(TcShared);
+template <int N> __device__ __forceinline__ void regs_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 // Waits (bounded) for a phase of a barrier; every lane of a warp may call it.
@@ -118,39 +148,24 @@ __device__ __forceinline__ uint32_t even_f16x2(uint32_t w) {
   return w;
 }
 
-// Order in which K and V tiles are loaded and consumed: `lead` K tiles, then
-// V0, K(lead), V1, ...
-struct TcItems {
-  int kn = 0, vn = 0;
-  __device__ __forceinline__ bool next(int n, int lead, int &i) {  // true: a V tile
-    if (kn < n && kn < vn + lead) {
-      i = kn++;
-      return false;
-    }
-    i = vn++;
-    return true;
-  }
-};
-
 template <int FMT, int DT, int D, bool TWO>
-__global__ void __launch_bounds__(kTcThreads, 1) chunk_tc_kernel(const ChunkArgs a) {
+__global__ void __launch_bounds__(TcLayout<FMT, D, TWO>::THREADS, 1)
+chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv) {
+  using L = TcLayout<FMT, D, TWO>;
   constexpr int KB = D / 64;                       // 64-channel blocks of a tile
-  constexpr uint32_t TILE = tc_tile_bytes(D);
+  constexpr uint32_t TILE = L::TILE;
   constexpr uint32_t BLK = TILE / KB;              // 128 rows x 128 bytes
   constexpr int RB = cache_row_bytes(FMT, D);
-  constexpr int CPR = RB / 16;                     // 16-byte pieces of a cache row
-  constexpr int RPP = 128 / CPR;                   // rows that the 128 loader threads take at a time
-  constexpr int LEAD = TWO ? 1 : 2;
+  constexpr int SLOTS = L::SLOTS, RSLOTS = L::RSLOTS;
   constexpr uint32_t S_COL = 0, O_COL = 256;       // tensor-memory columns: scores (2 x 128), outputs (2 x D)
+  constexpr int LAST = 4 * (L::GROUPS - 1);        // first warp of the last group: MMA issue, then the producers
 
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sbase = ptx::smem_u32(smem);
-  const uint32_t sq = sbase, sring = sq + (TWO ? 2u : 1u) * TILE, sstage = sring + kTcSlots * TILE;
-  TcShared &sh = *reinterpret_cast<TcShared *>(smem + (sstage - sbase) + kTcStages * tc_stage_bytes(FMT, D));
+  const uint32_t sq = sbase, skr = sbase + L::OFF_RING, svr = skr + SLOTS * TILE;
+  TcShared &sh = *reinterpret_cast<TcShared *>(smem + L::OFF_MISC);
   volatile int *abort_flag = &sh.abort_flag;
-  const uint32_t bars = ptx::smem_u32(&sh.bars[0]);
-  const uint32_t bar_full = bars, bar_empty = bars + 32, bar_sfull = bars + 64, bar_pready = bars + 80,
-                 bar_ofull = bars + 96, bar_done = bars + 112;
+  auto bar = [&](const uint64_t *b) -> uint32_t { return ptx::smem_u32(b); };
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   ChunkWork w;
@@ -171,22 +186,36 @@ __global__ void __launch_bounds__(kTcThreads, 1) chunk_tc_kernel(const ChunkArgs
     }
   }
 
+  // First step that some row of the block does not see whole. From there on V
+  // tiles must not carry infinities or NaN into such rows (0 * inf): zeros stand
+  // in, and the rows that do see them get them at the end.
+  const int first_masked = w.seen0 > w.t0 ? (w.seen0 - w.t0) / kTcStep : 0;
+
   if (tid == 0) {
     sh.abort_flag = 0;
     sh.odd = 0;
-    for (int s = 0; s < kTcSlots; ++s) {
-      ptx::mbar_init(bar_full + 8u * s, 4u);
-      ptx::mbar_init(bar_empty + 8u * s, 1u);
+    for (int s = 0; s < SLOTS; ++s) {
+      // filled by four converter warps, or by TMA
+      ptx::mbar_init(bar(&sh.kfull[s]), L::RAW ? 4u : 1u);
+      ptx::mbar_init(bar(&sh.vfull[s]), L::RAW ? 4u : 1u);
+      ptx::mbar_init(bar(&sh.kempty[s]), 1u);
+      ptx::mbar_init(bar(&sh.vempty[s]), 1u);
+      ptx::mbar_init(bar(&sh.vraw[s]), 1u);
+      ptx::mbar_init(bar(&sh.vfixed[s]), 4u);
     }
     for (int g = 0; g < 2; ++g) {
-      ptx::mbar_init(bar_sfull + 8u * g, 1u);
-      ptx::mbar_init(bar_pready + 8u * g, 4u);
-      ptx::mbar_init(bar_ofull + 8u * g, 1u);
+      ptx::mbar_init(bar(&sh.sfull[g]), 1u);
+      ptx::mbar_init(bar(&sh.pready[g]), 4u);
+      ptx::mbar_init(bar(&sh.ofull[g]), 1u);
+      for (int s = 0; s < RSLOTS; ++s) {
+        ptx::mbar_init(bar(&sh.rfull[g][s]), 33u);  // the boxes' bytes, and 32 lanes of cp.async
+        ptx::mbar_init(bar(&sh.rempty[g][s]), 4u);
+      }
     }
-    ptx::mbar_init(bar_done, 1u);
+    ptx::mbar_init(bar(&sh.done), 1u);
     ptx::fence_barrier_init();
   }
-  if (warp == kTcMmaWarp) {
+  if (warp == LAST) {
     tc::alloc(ptx::smem_u32(&sh.tmem), 512u);
     tc::relinquish();
   }
@@ -234,269 +263,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) chunk_tc_kernel(const ChunkArgs
   __syncthreads();
   tc::fence_after();
   const uint32_t tbase = sh.tmem;
-
-  if (warp >= kTcLoadWarp && warp < kTcMmaWarp) {
-    // ------------------------------------------------------------- loaders
-    const int lt = tid - kTcLoadWarp * 32;
-    const int ch = lt % CPR, r0 = lt / CPR;
-    const int items = 2 * n;
-    bool ok = true;
-    TcItems gi, gc;
-    const int gword = FMT == KVF_FMT_F16 ? 0 : (ch * (16 * D / RB)) >> a.group_shift;  // metadata word of the piece
-    // Starts the copies of item `it` and closes their group.
-    auto issue = [&](int it) {
-      if (it < items && ok) {
-        int i;
-        const bool isv = gi.next(n, LEAD, i);
-        const uint8_t *src = isv ? a.v : a.k;
-        const uint32_t *meta = isv ? a.vm : a.km;
-        const int t = w.t0 + i * kTcStep;
-        uint32_t dst = sstage + (it % kTcStages) * tc_stage_bytes(FMT, D);
-        const uint32_t mdst = dst + kTcStep * RB;
-        if (FMT == KVF_FMT_F16) {
-          const int s = it % kTcSlots;
-          if (it >= kTcSlots && !tc_wait_warp(bar_empty + 8u * s, (uint32_t)((it / kTcSlots - 1) & 1), abort_flag)) ok = false;
-          dst = sring + s * TILE;
-        }
-        if (ok) {
-#pragma unroll
-          for (int k = 0; k < CPR; ++k) {
-            const int rr = r0 + k * RPP;
-            const long long rw = t + rr < w.t1 ? a.cache.row(w.b, w.h, t + rr) : -1;
-            const bool there = rw >= 0;
-            const uint8_t *p = there ? src + rw * RB + ch * 16 : src;
-            if (FMT == KVF_FMT_F16) {
-              ptx::cp_async_16_zfill(dst + (ch >> 3) * BLK + rr * 128u + ((uint32_t)((ch ^ rr) & 7) << 4), p, there ? 16u : 0u);
-            } else {
-              ptx::cp_async_16_zfill(dst + (uint32_t)(k * 128 + lt) * 16u, p, there ? 16u : 0u);
-              if (ch == 0) {
-                const uint32_t *mp = there ? meta + rw * a.gpr : meta;
-                const uint32_t md = mdst + (uint32_t)(rr * a.gpr * 4);
-                if (a.gpr == 1)
-                  ptx::cp_async_4_zfill(md, mp, there ? 4u : 0u);
-                else if (a.gpr == 2)
-                  ptx::cp_async_8_zfill(md, mp, there ? 8u : 0u);
-                else
-                  ptx::cp_async_16_zfill(md, mp, there ? 16u : 0u);
-              }
-            }
-          }
-        }
-      }
-      ptx::cp_async_commit();
-    };
-    constexpr int AHEAD = FMT == KVF_FMT_F16 ? kTcSlots - 1 : kTcStages;  // items in flight
-    for (int it = 0; it < AHEAD; ++it) issue(it);
-    for (int it = 0; it < items && ok; ++it) {
-      int i;
-      const bool isv = gc.next(n, LEAD, i);
-      const int s = it % kTcSlots;
-      const int t = w.t0 + i * kTcStep;
-      // V tiles that some row of the block does not see whole must not carry
-      // infinities or NaN into it (0 * inf): zeros stand in, and the rows that
-      // do see them get them at the end.
-      const bool masked = isv && t + kTcStep > w.seen0;
-      bool odd = false;
-      ptx::cp_async_wait<AHEAD - 1>();
-      const uint32_t tile = sring + s * TILE;
-      if (FMT == KVF_FMT_F16) {
-        if (masked) {
-#pragma unroll 4
-          for (int k = 0; k < CPR; ++k) {
-            const int rr = r0 + k * RPP;
-            const uint32_t ad = tile + (ch >> 3) * BLK + rr * 128u + ((uint32_t)((ch ^ rr) & 7) << 4);
-            uint32_t p[4];
-            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(p[0]), "=r"(p[1]), "=r"(p[2]), "=r"(p[3]) : "r"(ad));
-            if (odd_f16x2(p[0]) || odd_f16x2(p[1]) || odd_f16x2(p[2]) || odd_f16x2(p[3])) {
-              odd = true;
-              asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(ad), "r"(even_f16x2(p[0])),
-                           "r"(even_f16x2(p[1])), "r"(even_f16x2(p[2])), "r"(even_f16x2(p[3]))
-                           : "memory");
-            }
-          }
-        }
-      } else {
-        __syncwarp();  // the row's metadata words came by its first lane
-        if (it >= kTcSlots && !tc_wait_warp(bar_empty + 8u * s, (uint32_t)((it / kTcSlots - 1) & 1), abort_flag)) {
-          ok = false;
-          break;
-        }
-        const uint32_t stage = sstage + (it % kTcStages) * tc_stage_bytes(FMT, D);
-        const uint32_t mstage = stage + kTcStep * RB;
-#pragma unroll 4
-        for (int k = 0; k < CPR; ++k) {
-          const int rr = r0 + k * RPP;
-          uint32_t raw[4], sz;
-          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                       : "=r"(raw[0]), "=r"(raw[1]), "=r"(raw[2]), "=r"(raw[3])
-                       : "r"(stage + (uint32_t)(k * 128 + lt) * 16u));
-          asm volatile("ld.shared.u32 %0, [%1];" : "=r"(sz) : "r"(mstage + (uint32_t)((rr * a.gpr + gword) * 4)));
-          const uint32_t s2 = ptx::prmt(sz, sz, 0x1010), z2 = ptx::prmt(sz, sz, 0x3232);
-          uint32_t o[16];
-          if (FMT == KVF_FMT_INT8) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              // bytes under the exponent of 1024: half2 of 1024 + code, exact; less 1024, exact
-              const uint32_t lo = ptx::prmt(raw[q], 0x64646464u, 0x4140), hi = ptx::prmt(raw[q], 0x64646464u, 0x4342);
-              o[2 * q] = ptx::hfma2_u32(ptx::hsub2_u32(lo, 0x64006400u), s2, z2);
-              o[2 * q + 1] = ptx::hfma2_u32(ptx::hsub2_u32(hi, 0x64006400u), s2, z2);
-            }
-          } else {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              uint32_t v[4];  // columns (0,4), (1,5), (2,6), (3,7) of the word's eight
-#pragma unroll
-              for (int u = 0; u < 4; ++u)
-                v[u] = ptx::hfma2_u32(ptx::hsub2_u32(ptx::lop3_and_or(raw[q] >> (4 * u), 0x000F000Fu, 0x64006400u), 0x64006400u), s2, z2);
-              o[4 * q] = ptx::prmt(v[0], v[1], 0x5410);
-              o[4 * q + 1] = ptx::prmt(v[2], v[3], 0x5410);
-              o[4 * q + 2] = ptx::prmt(v[0], v[1], 0x7632);
-              o[4 * q + 3] = ptx::prmt(v[2], v[3], 0x7632);
-            }
-          }
-          constexpr int P16 = 32 / (RB * 16 / D);  // 16-byte pieces out per piece in: 2 (int8), 4 (int4)
-          static_assert(FMT == KVF_FMT_F16 || P16 == (FMT == KVF_FMT_INT8 ? 2 : 4), "pieces");
-          if (masked) {
-#pragma unroll
-            for (int q = 0; q < 4 * P16; ++q)
-              if (odd_f16x2(o[q])) {
-                odd = true;
-                o[q] = even_f16x2(o[q]);
-              }
-          }
-          // lanes that share a row start at different pieces, so that a
-          // quarter of a warp stores to all banks
-          const int turn = FMT == KVF_FMT_INT8 ? ch >> 2 : (ch >> 1) << 1;
-#pragma unroll
-          for (int q = 0; q < P16; ++q) {
-            const int at = q ^ (D == 128 ? turn & (P16 - 1) : 0);
-            const int ci = ch * P16 + at;  // 16-byte piece of the tile row
-            uint32_t x0 = o[0], x1 = o[1], x2 = o[2], x3 = o[3];
-#pragma unroll
-            for (int u = 1; u < P16; ++u)
-              if (at == u) {
-                x0 = o[4 * u];
-                x1 = o[4 * u + 1];
-                x2 = o[4 * u + 2];
-                x3 = o[4 * u + 3];
-              }
-            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(tile + (ci >> 3) * BLK + rr * 128u +
-                                                                     ((uint32_t)((ci ^ rr) & 7) << 4)),
-                         "r"(x0), "r"(x1), "r"(x2), "r"(x3)
-                         : "memory");
-          }
-        }
-      }
-      if (odd) *reinterpret_cast<volatile int *>(&sh.odd) = 1;
-      ptx::fence_proxy_async_smem();
-      __syncwarp();
-      ptx::mbar_arrive_if(bar_full + 8u * s, lane == 0);
-      issue(it + AHEAD);
-    }
-    if (!ok && lane == 0) {
-      atomicOr(&g_kvfb_chunk_error, 1u);
-      *abort_flag = 1;
-    }
-    ptx::cp_async_wait<0>();
-  } else if (warp == kTcMmaWarp) {
-    // ----------------------------------------------------------- MMA issue
-    if (lane == 0) {
-      constexpr uint32_t ID_S = tc::idesc_f16(false, false, 128, 128), ID_O = tc::idesc_f16(false, true, 128, D);
-      bool ok = true;
-      int it = 0;  // items consumed
-      uint32_t kslot = 0;
-      // Waits for the next item of the ring and returns its tile.
-      auto take = [&](uint32_t &slot) -> bool {
-        slot = (uint32_t)(it % kTcSlots);
-        if (!tc_wait(bar_full + 8u * slot, (uint32_t)((it / kTcSlots) & 1), abort_flag)) return ok = false;
-        ++it;
-        tc::fence_after();
-        return true;
-      };
-      auto scores = [&](int g, uint32_t slot) {
-        const uint32_t q = sq + (TWO ? (uint32_t)g * TILE : 0u), k = sring + slot * TILE;
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-          const uint32_t off = (ks >> 2) * BLK + (ks & 3) * 32u;
-          tc::mma_f16_ss(tbase + S_COL + 128u * g, tc::smem_desc(q + off, 16u, 1024u, tc::kSwizzle128),
-                         tc::smem_desc(k + off, 16u, 1024u, tc::kSwizzle128), ID_S, ks > 0);
-        }
-        tc::commit(bar_sfull + 8u * g);
-      };
-      auto values = [&](int g, uint32_t slot, bool acc) {
-        const uint32_t v = sring + slot * TILE;
-#pragma unroll
-        for (int ks = 0; ks < kTcStep / 16; ++ks)
-          tc::mma_f16_ta(tbase + O_COL + (uint32_t)(D * g), tbase + S_COL + 128u * g + 8u * ks,
-                         tc::smem_desc(v + ks * 2048u, BLK, 1024u, tc::kSwizzle128), ID_O, acc || ks > 0);
-        tc::commit(bar_ofull + 8u * g);
-      };
-      if (TWO) {
-        if (n > 0 && take(kslot)) {
-          for (int g = 0; g < 2; ++g)
-            if (nw[g] > 0) scores(g, kslot);
-          tc::commit(bar_empty + 8u * kslot);
-        }
-        for (int i = 0; i < n && ok; ++i) {
-          uint32_t vslot;
-          if (!take(vslot)) break;
-          bool have = false;
-          const int last = i < nw[1] ? 1 : 0;
-          for (int g = 0; g < 2 && ok; ++g) {
-            if (i < nw[g]) {
-              if (!tc_wait(bar_pready + 8u * g, (uint32_t)(i & 1), abort_flag)) {
-                ok = false;
-                break;
-              }
-              tc::fence_after();
-              values(g, vslot, i > 0);
-            }
-            if (g == last) tc::commit(bar_empty + 8u * vslot);
-            if (i + 1 < nw[g]) {
-              if (!have && !take(kslot)) break;
-              have = true;
-              scores(g, kslot);
-            }
-          }
-          if (ok && i + 1 < n) {
-            if (!have && !take(kslot)) break;
-            tc::commit(bar_empty + 8u * kslot);
-          }
-        }
-      } else {
-        for (int g = 0; g < 2 && g < n && ok; ++g)
-          if (take(kslot)) {
-            scores(g, kslot);
-            tc::commit(bar_empty + 8u * kslot);
-          }
-        for (int i = 0; i < n && ok; ++i) {
-          const int g = i & 1, j = i >> 1;
-          uint32_t vslot;
-          if (!take(vslot)) break;
-          if (!tc_wait(bar_pready + 8u * g, (uint32_t)(j & 1), abort_flag)) {
-            ok = false;
-            break;
-          }
-          tc::fence_after();
-          values(g, vslot, j > 0);
-          tc::commit(bar_empty + 8u * vslot);
-          if (i + 2 < n && take(kslot)) {
-            scores(g, kslot);
-            tc::commit(bar_empty + 8u * kslot);
-          }
-        }
-      }
-      if (!ok) {
-        atomicOr(&g_kvfb_chunk_error, 1u);
-        *abort_flag = 1;
-      }
-      // tensor memory is freed below only after every MMA issued here completed
-      tc::commit(bar_done);
-      if (!ptx::mbar_wait(bar_done, 0u, 1000000000ull)) atomicOr(&g_kvfb_chunk_error, 1u);
-    }
-    __syncwarp();
-  } else {
+  // Each group executes one setmaxnreg, all four warps the same one.
+  if (warp < 8) {
     // ------------------------------------------------------------- softmax
+    regs_up<L::SOFT_REGS>();
     const bool live = row < w.rows;
     const int seen = live ? chunk_seen(a, w, w.row0 + row) : 0;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
@@ -506,7 +276,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) chunk_tc_kernel(const ChunkArgs
     bool ok = true;
     for (int j = 0; j < steps; ++j) {
       const int t = w.t0 + (TWO ? j : 2 * j + grp) * kTcStep;
-      if (!tc_wait_warp(bar_sfull + 8u * grp, (uint32_t)(j & 1), abort_flag)) {
+      if (!tc_wait_warp(bar(&sh.sfull[grp]), (uint32_t)(j & 1), abort_flag)) {
         ok = false;
         break;
       }
@@ -554,7 +324,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) chunk_tc_kernel(const ChunkArgs
         m = mn;
         l *= f;
         if (j > 0 && __any_sync(0xffffffffu, f != 1.f)) {
-          if (!tc_wait_warp(bar_ofull + 8u * grp, (uint32_t)((j - 1) & 1), abort_flag)) {
+          if (!tc_wait_warp(bar(&sh.ofull[grp]), (uint32_t)((j - 1) & 1), abort_flag)) {
             ok = false;
             break;
           }
@@ -598,9 +368,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) chunk_tc_kernel(const ChunkArgs
       tc::wait_st();
       tc::fence_before();
       __syncwarp();
-      ptx::mbar_arrive_if(bar_pready + 8u * grp, lane == 0);
+      ptx::mbar_arrive_if(bar(&sh.pready[grp]), lane == 0);
     }
-    if (ok && steps > 0 && !tc_wait_warp(bar_ofull + 8u * grp, (uint32_t)((steps - 1) & 1), abort_flag)) ok = false;
+    if (ok && steps > 0 && !tc_wait_warp(bar(&sh.ofull[grp]), (uint32_t)((steps - 1) & 1), abort_flag)) ok = false;
     tc::fence_after();
     if (!ok && lane == 0) {
       atomicOr(&g_kvfb_chunk_error, 1u);
@@ -632,8 +402,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) chunk_tc_kernel(const ChunkArgs
       }
       if (odd && live && !none) {
         // what the masked tiles left out, for a row that sees it
-        const int first = w.seen0 >= w.t0 + kTcStep ? (w.seen0 - w.t0) / kTcStep : 0;
-        for (int t = w.t0 + first * kTcStep; t < min(seen, w.t1); ++t) {
+        for (int t = w.t0 + first_masked * kTcStep; t < min(seen, w.t1); ++t) {
           if (!TWO && (((t - w.t0) / kTcStep) & 1) != grp) continue;
           const long long rw = a.cache.row(w.b, w.h, t);
           if (rw < 0) continue;
@@ -670,9 +439,324 @@ __global__ void __launch_bounds__(kTcThreads, 1) chunk_tc_kernel(const ChunkArgs
       }
     }
     tc::fence_before();
+  } else if (warp < LAST) {
+    // ---------------------------------------------------------- converters
+    regs_down<L::CONV_REGS>();
+    const int lt = tid & 127;
+    bool ok = true, odd = false;
+    if constexpr (L::RAW) {
+      constexpr int CPR = RB / 16;                 // 16-byte pieces of a raw row
+      constexpr int RPP = 128 / CPR;               // rows that the group takes at a time
+      constexpr int P16 = 2 * D / RB;              // 16-byte pieces of the tile per raw piece: 2 (int8), 4 (int4)
+      const int op = (warp >> 2) - 2;              // 0: K, 1: V
+      const int ch = lt % CPR, r0 = lt / CPR;
+      const int gword = (ch * (16 * D / RB)) >> a.group_shift;  // metadata word of the piece
+      const uint32_t ring = op ? svr : skr;
+      for (int i = 0; i < 2 * n; ++i) {
+        const int rs = i % RSLOTS, s = (i >> 1) % SLOTS, use = (i >> 1) / SLOTS;
+        const bool masked = op && (i >> 1) >= first_masked;
+        if (!tc_wait_warp(bar(&sh.rfull[op][rs]), (uint32_t)((i / RSLOTS) & 1), abort_flag) ||
+            (!(i & 1) && use > 0 &&
+             !tc_wait_warp(bar(op ? &sh.vempty[s] : &sh.kempty[s]), (uint32_t)((use - 1) & 1), abort_flag))) {
+          ok = false;
+          break;
+        }
+        const uint32_t raw = sbase + L::OFF_RAW + (uint32_t)(op * RSLOTS + rs) * L::RAWB;
+        const uint32_t meta = sbase + L::OFF_META + (uint32_t)(op * RSLOTS + rs) * L::METAB;
+        const int tok = w.t0 + i * kTcHalf;
+#pragma unroll
+        for (int k = 0; k < CPR / 2; ++k) {
+          const int rr = r0 + k * RPP;             // row of the half step
+          // the raw tile has TMA's swizzle of its row width
+          const int pc = RB == 128 ? ch ^ (rr & 7) : RB == 64 ? ch ^ ((rr >> 1) & 3) : ch ^ ((rr >> 2) & 1);
+          uint32_t in[4], sz;
+          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                       : "=r"(in[0]), "=r"(in[1]), "=r"(in[2]), "=r"(in[3])
+                       : "r"(raw + (uint32_t)(rr * RB + pc * 16)));
+          asm volatile("ld.shared.u32 %0, [%1];" : "=r"(sz) : "r"(meta + (uint32_t)((rr * a.gpr + gword) * 4)));
+          if (tok + rr >= w.t1) sz = 0u;           // a row that nobody sees: zeros, whatever its page holds
+          const uint32_t s2 = ptx::prmt(sz, sz, 0x1010), z2 = ptx::prmt(sz, sz, 0x3232);
+          uint32_t o[4 * P16];
+          if (FMT == KVF_FMT_INT8) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              // bytes under the exponent of 1024: half2 of 1024 + code, exact; less 1024, exact
+              const uint32_t lo = ptx::prmt(in[q], 0x64646464u, 0x4140), hi = ptx::prmt(in[q], 0x64646464u, 0x4342);
+              o[2 * q] = ptx::hfma2_u32(ptx::hsub2_u32(lo, 0x64006400u), s2, z2);
+              o[2 * q + 1] = ptx::hfma2_u32(ptx::hsub2_u32(hi, 0x64006400u), s2, z2);
+            }
+          } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              uint32_t v[4];  // columns (0,4), (1,5), (2,6), (3,7) of the word's eight
+#pragma unroll
+              for (int u = 0; u < 4; ++u)
+                v[u] = ptx::hfma2_u32(
+                    ptx::hsub2_u32(ptx::lop3_and_or(in[q] >> (4 * u), 0x000F000Fu, 0x64006400u), 0x64006400u), s2, z2);
+              o[4 * q] = ptx::prmt(v[0], v[1], 0x5410);
+              o[4 * q + 1] = ptx::prmt(v[2], v[3], 0x5410);
+              o[4 * q + 2] = ptx::prmt(v[0], v[1], 0x7632);
+              o[4 * q + 3] = ptx::prmt(v[2], v[3], 0x7632);
+            }
+          }
+          if (masked) {
+#pragma unroll
+            for (int q = 0; q < 4 * P16; ++q)
+              if (odd_f16x2(o[q])) {
+                odd = true;
+                o[q] = even_f16x2(o[q]);
+              }
+          }
+          // lanes that share a row start at different pieces, so that a
+          // quarter of a warp stores to all banks
+          const int turn = D == 64 ? 0 : FMT == KVF_FMT_INT8 ? ch >> 2 : (ch >> 1) << 1;
+          const int tr = rr + (i & 1) * kTcHalf;   // row of the tile
+          const uint32_t base = ring + s * TILE + tr * 128u;
+#pragma unroll
+          for (int q = 0; q < P16; ++q) {
+            const int at = q ^ turn;
+            const int ci = ch * P16 + at;          // 16-byte piece of the tile row
+            uint32_t x0 = o[0], x1 = o[1], x2 = o[2], x3 = o[3];
+#pragma unroll
+            for (int u = 1; u < P16; ++u)
+              if (at == u) {
+                x0 = o[4 * u];
+                x1 = o[4 * u + 1];
+                x2 = o[4 * u + 2];
+                x3 = o[4 * u + 3];
+              }
+            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(base + (ci >> 3) * BLK +
+                                                                     ((uint32_t)((ci ^ tr) & 7) << 4)),
+                         "r"(x0), "r"(x1), "r"(x2), "r"(x3)
+                         : "memory");
+          }
+        }
+        if (i & 1) {
+          if (odd) *reinterpret_cast<volatile int *>(&sh.odd) = 1;
+          ptx::fence_proxy_async_smem();
+        }
+        __syncwarp();
+        ptx::mbar_arrive_if(bar(&sh.rempty[op][rs]), lane == 0);
+        if (i & 1) ptx::mbar_arrive_if(bar(op ? &sh.vfull[s] : &sh.kfull[s]), lane == 0);
+      }
+    } else {
+      for (int i = first_masked; i < n; ++i) {
+        const int s = i % SLOTS;
+        if (!tc_wait_warp(bar(&sh.vraw[s]), (uint32_t)(((i - first_masked) / SLOTS) & 1), abort_flag)) {
+          ok = false;
+          break;
+        }
+        const int ch = lt % (D / 8);
+        for (int rr = lt / (D / 8); rr < kTcStep; rr += 128 / (D / 8)) {
+          const uint32_t ad = svr + s * TILE + (ch >> 3) * BLK + rr * 128u + ((uint32_t)((ch ^ rr) & 7) << 4);
+          const bool seen = w.t0 + i * kTcStep + rr < w.t1;
+          uint32_t x[4];
+          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(ad));
+          const bool bad = odd_f16x2(x[0]) || odd_f16x2(x[1]) || odd_f16x2(x[2]) || odd_f16x2(x[3]);
+          if (seen && !bad) continue;
+          if (seen) odd = true;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) x[q] = seen ? even_f16x2(x[q]) : 0u;
+          asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(ad), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3])
+                       : "memory");
+        }
+        if (odd) *reinterpret_cast<volatile int *>(&sh.odd) = 1;
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+        ptx::mbar_arrive_if(bar(&sh.vfixed[s]), lane == 0);
+      }
+    }
+    if (!ok && lane == 0) {
+      atomicOr(&g_kvfb_chunk_error, 1u);
+      *abort_flag = 1;
+    }
+  } else {
+    regs_down<L::LAST_REGS>();
+    if (warp == LAST + 1 || warp == LAST + 2) {
+    // ----------------------------------------------------------- producers
+    const int op = warp - LAST - 1;  // 0: K, 1: V
+    const CUtensorMap *map = op ? &tmv : &tmk;
+    if (lane == 0) ptx::prefetch_tmap(map);
+    const uint64_t pol = ptx::policy_evict_last();
+    const bool paged = a.cache.paged != 0;
+    const int bts = paged ? a.cache.bt_shift : 30;
+    const int tbs = min(bts, 6);             // log2 of the tokens of a box
+    const int span = L::RAW ? kTcHalf : kTcStep, boxes = span >> tbs;
+    const int count = L::RAW ? 2 * n : n;
+    const int *table = paged ? a.cache.table + (long long)w.b * a.cache.max_blocks : nullptr;
+    // Page (or sequence) of box `lane` of item i; -1 where there is nothing to read.
+    auto page_of = [&](int i) -> int {
+      const int t = w.t0 + i * span + ((lane % boxes) << tbs);
+      if (i >= count || t >= w.t1) return -1;
+      return paged ? max(__ldg(table + (t >> bts)), -1) : w.b;
+    };
+    bool ok = true;
+    int page = page_of(0), i = 0;
+    for (; i < count; ++i) {
+      const int next = page_of(i + 1);
+      const int t = w.t0 + i * span;
+      const int c1 = paged ? (t + ((lane % boxes) << tbs)) & ((1 << bts) - 1) : t + ((lane % boxes) << tbs);
+      if (L::RAW) {
+        constexpr int R = RSLOTS > 0 ? RSLOTS : 1;
+        const int s = i % R;
+        if (i >= R && !tc_wait_warp(bar(&sh.rempty[op][s]), (uint32_t)((i / R - 1) & 1), abort_flag)) {
+          ok = false;
+          break;
+        }
+        const uint32_t full = bar(&sh.rfull[op][s]);
+        const uint32_t dst = sbase + L::OFF_RAW + (uint32_t)(op * RSLOTS + s) * L::RAWB;
+        ptx::mbar_arrive_expect_tx_if(full, L::RAWB, lane == 0);
+        __syncwarp();
+        ptx::tma_g2s_4d_if(dst + ((uint32_t)lane << tbs) * RB, map, 0, c1, w.h, page, full, pol, lane < boxes);
+        const uint32_t *meta = op ? a.vm : a.km;
+        const uint32_t md = sbase + L::OFF_META + (uint32_t)(op * RSLOTS + s) * L::METAB;
+#pragma unroll
+        for (int k = 0; k < kTcHalf / 32; ++k) {
+          const int rr = lane + 32 * k, tok = t + rr;
+          const int pg = __shfl_sync(0xffffffffu, page, rr >> tbs);
+          long long row;
+          if (paged) {
+            const long long tl = tok & ((1 << bts) - 1), base = ((long long)pg * a.cache.Hkv) << bts;
+            row = a.cache.head_major ? base + ((long long)w.h << bts) + tl : base + tl * a.cache.Hkv + w.h;
+          } else {
+            row = a.cache.head_major ? ((long long)w.b * a.cache.Hkv + w.h) * a.cache.n + tok
+                                     : ((long long)w.b * a.cache.n + tok) * a.cache.Hkv + w.h;
+          }
+          const bool there = tok < w.t1 && pg >= 0;
+          const uint32_t *src = there ? meta + row * a.gpr : meta;
+          const uint32_t d = md + (uint32_t)(rr * a.gpr * 4);
+          if (a.gpr == 1)
+            ptx::cp_async_4_zfill(d, src, there ? 4u : 0u);
+          else if (a.gpr == 2)
+            ptx::cp_async_8_zfill(d, src, there ? 8u : 0u);
+          else
+            ptx::cp_async_16_zfill(d, src, there ? 16u : 0u);
+        }
+        ptx::cp_async_arrive(full);
+      } else {
+        const int s = i % SLOTS;
+        if (i >= SLOTS && !tc_wait_warp(bar(op ? &sh.vempty[s] : &sh.kempty[s]), (uint32_t)((i / SLOTS - 1) & 1), abort_flag)) {
+          ok = false;
+          break;
+        }
+        const uint32_t full = bar(!op ? &sh.kfull[s] : i < first_masked ? &sh.vfull[s] : &sh.vraw[s]);
+        const int blk = lane / boxes;  // 64-channel block of this lane's box
+        ptx::mbar_arrive_expect_tx_if(full, TILE, lane == 0);
+        __syncwarp();
+        ptx::tma_g2s_4d_if((op ? svr : skr) + s * TILE + blk * BLK + ((uint32_t)(lane % boxes) << tbs) * 128u, map,
+                           128 * blk, c1, w.h, page, full, pol, lane < boxes * KB);
+      }
+      page = next;
+    }
+    if (!ok && lane == 0) {
+      atomicOr(&g_kvfb_chunk_error, 1u);
+      *abort_flag = 1;
+    }
+    // Never leave with copies in flight: the last item of each slot has landed.
+    constexpr int RING = L::RAW ? RSLOTS : SLOTS;
+    for (int k = max(0, i - RING); k < i; ++k) {
+      const int s = k % RING;
+      const bool fixed = !L::RAW && op && k >= first_masked;
+      const uint32_t full = L::RAW ? bar(&sh.rfull[op][s]) : bar(!op ? &sh.kfull[s] : fixed ? &sh.vraw[s] : &sh.vfull[s]);
+      if (!ptx::mbar_wait(full, (uint32_t)(((fixed ? k - first_masked : k) / RING) & 1)) && lane == 0) atomicOr(&g_kvfb_chunk_error, 1u);
+    }
+    // ----------------------------------------------------------- MMA issue
+    } else if (warp == LAST && lane == 0) {
+      constexpr uint32_t ID_S = tc::idesc_f16(false, false, 128, 128), ID_O = tc::idesc_f16(false, true, 128, D);
+      bool ok = true;
+      // Waits for K or V tile i.
+      auto take_k = [&](int i) -> bool {
+        if (!tc_wait(bar(&sh.kfull[i % SLOTS]), (uint32_t)((i / SLOTS) & 1), abort_flag)) return ok = false;
+        tc::fence_after();
+        return true;
+      };
+      auto take_v = [&](int i) -> bool {
+        const bool fixed = !L::RAW && i >= first_masked;
+        const int use = (fixed ? i - first_masked : i) / SLOTS;
+        if (!tc_wait(bar(fixed ? &sh.vfixed[i % SLOTS] : &sh.vfull[i % SLOTS]), (uint32_t)(use & 1), abort_flag))
+          return ok = false;
+        tc::fence_after();
+        return true;
+      };
+      auto scores = [&](int g, int i) {
+        const uint32_t q = sq + (TWO ? (uint32_t)g * TILE : 0u), k = skr + (uint32_t)(i % SLOTS) * TILE;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          const uint32_t off = (ks >> 2) * BLK + (ks & 3) * 32u;
+          tc::mma_f16_ss(tbase + S_COL + 128u * g, tc::smem_desc(q + off, 16u, 1024u, tc::kSwizzle128),
+                         tc::smem_desc(k + off, 16u, 1024u, tc::kSwizzle128), ID_S, ks > 0);
+        }
+        tc::commit(bar(&sh.sfull[g]));
+      };
+      auto values = [&](int g, int i, bool acc) {
+        const uint32_t v = svr + (uint32_t)(i % SLOTS) * TILE;
+#pragma unroll
+        for (int ks = 0; ks < kTcStep / 16; ++ks)
+          tc::mma_f16_ta(tbase + O_COL + (uint32_t)(D * g), tbase + S_COL + 128u * g + 8u * ks,
+                         tc::smem_desc(v + ks * 2048u, BLK, 1024u, tc::kSwizzle128), ID_O, acc || ks > 0);
+        tc::commit(bar(&sh.ofull[g]));
+      };
+      auto weights = [&](int g, int j) -> bool {
+        if (!tc_wait(bar(&sh.pready[g]), (uint32_t)(j & 1), abort_flag)) return ok = false;
+        tc::fence_after();
+        return true;
+      };
+      if (TWO) {
+        if (n > 0 && take_k(0)) {
+          for (int g = 0; g < 2; ++g)
+            if (nw[g] > 0) scores(g, 0);
+          tc::commit(bar(&sh.kempty[0]));
+        }
+        for (int i = 0; i < n && ok; ++i) {
+          if (!take_v(i)) break;
+          bool have = false;
+          const int last = i < nw[1] ? 1 : 0;
+          for (int g = 0; g < 2 && ok; ++g) {
+            if (i < nw[g]) {
+              if (!weights(g, i)) break;
+              values(g, i, i > 0);
+            }
+            if (g == last) tc::commit(bar(&sh.vempty[i % SLOTS]));
+            if (i + 1 < nw[g]) {
+              if (!have && !take_k(i + 1)) break;
+              have = true;
+              scores(g, i + 1);
+            }
+          }
+          if (ok && i + 1 < n) {
+            if (!have && !take_k(i + 1)) break;
+            tc::commit(bar(&sh.kempty[(i + 1) % SLOTS]));
+          }
+        }
+      } else {
+        for (int g = 0; g < 2 && g < n && ok; ++g)
+          if (take_k(g)) {
+            scores(g, g);
+            tc::commit(bar(&sh.kempty[g % SLOTS]));
+          }
+        for (int i = 0; i < n && ok; ++i) {
+          const int g = i & 1, j = i >> 1;
+          if (!take_v(i) || !weights(g, j)) break;
+          values(g, i, j > 0);
+          tc::commit(bar(&sh.vempty[i % SLOTS]));
+          if (i + 2 < n && take_k(i + 2)) {
+            scores(g, i + 2);
+            tc::commit(bar(&sh.kempty[(i + 2) % SLOTS]));
+          }
+        }
+      }
+      if (!ok) {
+        atomicOr(&g_kvfb_chunk_error, 1u);
+        *abort_flag = 1;
+      }
+      // tensor memory is freed below only after every MMA issued here completed
+      tc::commit(bar(&sh.done));
+      if (!ptx::mbar_wait(bar(&sh.done), 0u, 1000000000ull)) atomicOr(&g_kvfb_chunk_error, 1u);
+    }
+    __syncwarp();
   }
   __syncthreads();
-  if (warp == kTcMmaWarp) tc::dealloc(tbase, 512u);
+  if (warp == LAST) tc::dealloc(tbase, 512u);
 }
 
 } // namespace

@@ -1157,6 +1157,14 @@ namespace kvfb {
 // For the other translation units: this file's caches of driver facts.
 cudaError_t ensure_kernel_smem(void *fn, uint32_t smem) { return ensure_smem(fn, smem); }
 int device_sm_count() { return sm_count(); }
+// Tensor maps over the K and V payload with boxes of tbox tokens of one head,
+// at most 128 bytes wide and swizzled by their width.
+cudaError_t encode_cache_maps(const kvf_args *a, int fmt, int d, int ord, int paged, int tbox, CUtensorMap &k,
+                              CUtensorMap &v) {
+  Shape sh{fmt, d, ord, paged, paged ? 1 << a->block_shift : 0, 0};
+  const int rb = fmt == KVF_FMT_F16 ? 2 * d : fmt == KVF_FMT_INT8 ? d : d / 2;
+  return encode_maps_box(a, sh, rb, std::min(rb, 128), tbox, 1, k, v);
+}
 
 unsigned take_append_errors();  // quantize.cu
 unsigned take_heads_errors();   // heads.cu
