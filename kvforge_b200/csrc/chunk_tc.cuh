@@ -166,7 +166,8 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
   TcShared &sh = *reinterpret_cast<TcShared *>(smem + L::OFF_MISC);
   volatile int *abort_flag = &sh.abort_flag;
   auto bar = [&](const uint64_t *b) -> uint32_t { return ptx::smem_u32(b); };
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // known to be the same in all lanes
 
   ChunkWork w;
   const int nsplit = TWO ? a.splits : a.splits / 2;
@@ -661,43 +662,53 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
       if (!ptx::mbar_wait(full, (uint32_t)(((fixed ? k - first_masked : k) / RING) & 1)) && lane == 0) atomicOr(&g_kvfb_chunk_error, 1u);
     }
     // ----------------------------------------------------------- MMA issue
-    } else if (warp == LAST && lane == 0) {
+    } else if (warp == LAST) {
       constexpr uint32_t ID_S = tc::idesc_f16(false, false, 128, 128), ID_O = tc::idesc_f16(false, true, 128, D);
       bool ok = true;
       // Waits for K or V tile i.
       auto take_k = [&](int i) -> bool {
-        if (!tc_wait(bar(&sh.kfull[i % SLOTS]), (uint32_t)((i / SLOTS) & 1), abort_flag)) return ok = false;
+        if (!tc_wait_warp(bar(&sh.kfull[i % SLOTS]), (uint32_t)((i / SLOTS) & 1), abort_flag)) return ok = false;
         tc::fence_after();
         return true;
       };
       auto take_v = [&](int i) -> bool {
         const bool fixed = !L::RAW && i >= first_masked;
         const int use = (fixed ? i - first_masked : i) / SLOTS;
-        if (!tc_wait(bar(fixed ? &sh.vfixed[i % SLOTS] : &sh.vfull[i % SLOTS]), (uint32_t)(use & 1), abort_flag))
+        if (!tc_wait_warp(bar(fixed ? &sh.vfixed[i % SLOTS] : &sh.vfull[i % SLOTS]), (uint32_t)(use & 1), abort_flag))
           return ok = false;
         tc::fence_after();
         return true;
       };
       auto scores = [&](int g, int i) {
         const uint32_t q = sq + (TWO ? (uint32_t)g * TILE : 0u), k = skr + (uint32_t)(i % SLOTS) * TILE;
+        const uint64_t dq = tc::smem_desc(q, 16u, 1024u, tc::kSwizzle128), dk = tc::smem_desc(k, 16u, 1024u, tc::kSwizzle128);
+        if (tc::elect_one()) {
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-          const uint32_t off = (ks >> 2) * BLK + (ks & 3) * 32u;
-          tc::mma_f16_ss(tbase + S_COL + 128u * g, tc::smem_desc(q + off, 16u, 1024u, tc::kSwizzle128),
-                         tc::smem_desc(k + off, 16u, 1024u, tc::kSwizzle128), ID_S, ks > 0);
+          for (int ks = 0; ks < D / 16; ++ks) {
+            const uint32_t off = ((ks >> 2) * BLK + (ks & 3) * 32u) >> 4;  // descriptors count 16-byte units
+            tc::mma_f16_ss(tbase + S_COL + 128u * g, dq + off, dk + off, ID_S, ks > 0);
+          }
+          tc::commit(bar(&sh.sfull[g]));
         }
-        tc::commit(bar(&sh.sfull[g]));
+        __syncwarp();
       };
       auto values = [&](int g, int i, bool acc) {
-        const uint32_t v = svr + (uint32_t)(i % SLOTS) * TILE;
+        const uint64_t dv = tc::smem_desc(svr + (uint32_t)(i % SLOTS) * TILE, BLK, 1024u, tc::kSwizzle128);
+        if (tc::elect_one()) {
 #pragma unroll
-        for (int ks = 0; ks < kTcStep / 16; ++ks)
-          tc::mma_f16_ta(tbase + O_COL + (uint32_t)(D * g), tbase + S_COL + 128u * g + 8u * ks,
-                         tc::smem_desc(v + ks * 2048u, BLK, 1024u, tc::kSwizzle128), ID_O, acc || ks > 0);
-        tc::commit(bar(&sh.ofull[g]));
+          for (int ks = 0; ks < kTcStep / 16; ++ks)
+            tc::mma_f16_ta(tbase + O_COL + (uint32_t)(D * g), tbase + S_COL + 128u * g + 8u * ks, dv + ks * (2048u >> 4), ID_O,
+                           acc || ks > 0);
+          tc::commit(bar(&sh.ofull[g]));
+        }
+        __syncwarp();
+      };
+      auto release = [&](const uint64_t *b) {
+        if (tc::elect_one()) tc::commit(bar(b));
+        __syncwarp();
       };
       auto weights = [&](int g, int j) -> bool {
-        if (!tc_wait(bar(&sh.pready[g]), (uint32_t)(j & 1), abort_flag)) return ok = false;
+        if (!tc_wait_warp(bar(&sh.pready[g]), (uint32_t)(j & 1), abort_flag)) return ok = false;
         tc::fence_after();
         return true;
       };
@@ -705,7 +716,7 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
         if (n > 0 && take_k(0)) {
           for (int g = 0; g < 2; ++g)
             if (nw[g] > 0) scores(g, 0);
-          tc::commit(bar(&sh.kempty[0]));
+          release(&sh.kempty[0]);
         }
         for (int i = 0; i < n && ok; ++i) {
           if (!take_v(i)) break;
@@ -716,7 +727,7 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
               if (!weights(g, i)) break;
               values(g, i, i > 0);
             }
-            if (g == last) tc::commit(bar(&sh.vempty[i % SLOTS]));
+            if (g == last) release(&sh.vempty[i % SLOTS]);
             if (i + 1 < nw[g]) {
               if (!have && !take_k(i + 1)) break;
               have = true;
@@ -725,33 +736,33 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
           }
           if (ok && i + 1 < n) {
             if (!have && !take_k(i + 1)) break;
-            tc::commit(bar(&sh.kempty[(i + 1) % SLOTS]));
+            release(&sh.kempty[(i + 1) % SLOTS]);
           }
         }
       } else {
         for (int g = 0; g < 2 && g < n && ok; ++g)
           if (take_k(g)) {
             scores(g, g);
-            tc::commit(bar(&sh.kempty[g % SLOTS]));
+            release(&sh.kempty[g % SLOTS]);
           }
         for (int i = 0; i < n && ok; ++i) {
           const int g = i & 1, j = i >> 1;
           if (!take_v(i) || !weights(g, j)) break;
           values(g, i, j > 0);
-          tc::commit(bar(&sh.vempty[i % SLOTS]));
+          release(&sh.vempty[i % SLOTS]);
           if (i + 2 < n && take_k(i + 2)) {
             scores(g, i + 2);
-            tc::commit(bar(&sh.kempty[(i + 2) % SLOTS]));
+            release(&sh.kempty[(i + 2) % SLOTS]);
           }
         }
       }
-      if (!ok) {
+      if (!ok && lane == 0) {
         atomicOr(&g_kvfb_chunk_error, 1u);
         *abort_flag = 1;
       }
       // tensor memory is freed below only after every MMA issued here completed
-      tc::commit(bar(&sh.done));
-      if (!ptx::mbar_wait(bar(&sh.done), 0u, 1000000000ull)) atomicOr(&g_kvfb_chunk_error, 1u);
+      release(&sh.done);
+      if (!ptx::mbar_wait(bar(&sh.done), 0u, 1000000000ull) && lane == 0) atomicOr(&g_kvfb_chunk_error, 1u);
     }
     __syncwarp();
   }

@@ -55,6 +55,15 @@ __device__ __forceinline__ void mma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_
       : "memory");
 }
 
+// One lane of the (whole) warp, the same one every time. Code under it keeps
+// warp-uniform operands in uniform registers, which tcgen05 instructions take;
+// under a test of the lane index each operand is moved there first.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
 // Instruction descriptor of a kind::f16 MMA on fp16 operands with an fp32
 // accumulator; a_mn / b_mn: operand is MN-major (else K-major); m = 128.
 __host__ __device__ constexpr uint32_t idesc_f16(bool a_mn, bool b_mn, int m, int n) {
