@@ -25,10 +25,10 @@
 //          and of V: TMA boxes per page, metadata rows by cp.async. A box of tokens
 //          that nobody sees, or of a block mapped to a negative page, is asked for
 //          at page -1, which TMA fills with zeros.
-// The running maximum a row's weights are taken against is raised only when a
-// step exceeds it by more than 2^8 (weights up to 256 fit fp16, and their sum
-// fp32), so the output in tensor memory is rescaled rarely and a step's scores
-// are read once.
+// The running maximum a row's weights are taken against is raised only when 64
+// of them add up to more than 256 (weights up to that fit fp16, and their sum
+// fp32), so the output in tensor memory is rescaled rarely, a step's scores are
+// read once, and their maximum is not needed before.
 // Waits are bounded in time; tensor memory is released before exit.
 #pragma once
 
@@ -36,6 +36,8 @@
 #include "tc.cuh"
 
 #include <cuda.h>
+
+#include <type_traits>
 
 namespace kvfb {
 
@@ -48,7 +50,8 @@ namespace {
 constexpr int kTcRows = 128;    // rows of a tile
 constexpr int kTcStep = 128;    // tokens of a step
 constexpr int kTcHalf = 64;     // tokens of a raw half step
-constexpr float kTcLazy = 8.f;  // log2 of the most a weight may exceed 1 by
+constexpr int kTcPoly = 4;           // one pair of weights in this many is computed without the special function unit
+constexpr float kTcLazySum = 256.f;  // most that 64 weights may add up to before the maximum is raised
 
 __host__ __device__ constexpr int cache_row_bytes(int fmt, int d) {
   return fmt == KVF_FMT_F16 ? 2 * d : fmt == KVF_FMT_INT8 ? d : d / 2;
@@ -137,6 +140,48 @@ __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
+}
+// 2^x for a pair in fp32 arithmetic, for x in [-126, 127]: the integer nearest
+// x is added to the exponent of a polynomial in the rest, |rest| <= 1/2, whose
+// coefficients minimise the largest relative error (7.5e-5, a third of fp16's
+// rounding). Weights below 2^-126 become 2^-126 (fp16: 0).
+__device__ __forceinline__ float2 ex2_poly(float2 x) {
+  x.x = fmaxf(x.x, -126.f);
+  x.y = fmaxf(x.y, -126.f);
+  const float big = 12582912.f;  // 1.5 * 2^23: the sum's low bits are the nearest integer
+  const float2 y = add2f(x, make_float2(big, big));
+  const float2 r = add2f(y, make_float2(-big, -big));
+  const float2 f = fma2f(r, make_float2(-1.f, -1.f), x);
+  float2 p = fma2f(make_float2(0.05517167f, 0.05517167f), f, make_float2(0.24261113f, 0.24261113f));
+  p = fma2f(p, f, make_float2(0.69326097f, 0.69326097f));
+  p = fma2f(p, f, make_float2(0.99992806f, 0.99992806f));
+  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(y.x) << 23)),
+                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(y.y) << 23)));
+}
+
+// Weights 2^(s c - m) of 32 scores as fp16 pairs, and their sum; 0 for tokens
+// from `seen` on. One pair in kTcPoly goes by ex2_poly, since the special
+// function unit alone would take as long as the tensor cores.
+template <bool MASKED>
+__device__ __forceinline__ float weigh(const uint32_t (&s)[32], float m, float c, int at, int seen, uint32_t *p) {
+  const float ref = m == -INFINITY ? 0.f : m;
+  const float2 c2 = make_float2(c, c), m2 = make_float2(-ref, -ref);
+  float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const float2 x = fma2f(make_float2(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1])), c2, m2);
+    float2 e = kTcPoly > 0 && k % (kTcPoly > 0 ? kTcPoly : 1) == 1 ? ex2_poly(x) : make_float2(ex2(x.x), ex2(x.y));
+    if (MASKED) {
+      e.x = at + 2 * k < seen ? e.x : 0.f;
+      e.y = at + 2 * k + 1 < seen ? e.y : 0.f;
+    }
+    if (k & 1)
+      sum1 = add2f(sum1, e);
+    else
+      sum0 = add2f(sum0, e);
+    p[k] = narrow2<KVF_DT_F16>(e.x, e.y);
+  }
+  return (sum0.x + sum0.y) + (sum1.x + sum1.y);
 }
 __device__ __forceinline__ bool odd_f16x2(uint32_t w) {
   return (w & 0x7C00u) == 0x7C00u || (w & 0x7C000000u) == 0x7C000000u;
@@ -269,7 +314,9 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
     // ------------------------------------------------------------- softmax
     regs_up<L::SOFT_REGS>();
     const bool live = row < w.rows;
-    const int seen = live ? chunk_seen(a, w, w.row0 + row) : 0;
+    // a lane without a row goes along (its query is zero); a warp without one only signs off
+    const int seen = live ? chunk_seen(a, w, w.row0 + row) : 0x7fffffff;
+    const bool idle = __all_sync(0xffffffffu, !live);
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
     const uint32_t ts = tbase + lanes + S_COL + 128u * grp, to = tbase + lanes + O_COL + (uint32_t)(D * grp);
     const int steps = nw[grp];
@@ -281,97 +328,98 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
         ok = false;
         break;
       }
-      tc::fence_after();
-      uint32_t p[64];
-      bool done = false;
-      // Every row sees the whole step and has a maximum: scores are read once.
-      if (__all_sync(0xffffffffu, !live || (t + kTcStep <= seen && m > -INFINITY))) {
-        const float ref = live ? m : 0.f;
-        const float2 c2 = make_float2(c, c), m2 = make_float2(-ref, -ref);
-        float2 sum = make_float2(0.f, 0.f);
-        float over = -INFINITY;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint32_t s[32];
-          tc::ld32(ts + 32u * q, s);
-          tc::wait_ld32(s);
-#pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            const float2 x = fma2f(make_float2(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1])), c2, m2);
-            over = max3f(over, x.x, x.y);
-            const float2 e = make_float2(ex2(x.x), ex2(x.y));
-            sum = add2f(sum, e);
-            p[16 * q + k] = narrow2<KVF_DT_F16>(e.x, e.y);
-          }
+      if (idle) {
+        ptx::mbar_arrive_if(bar(&sh.pready[grp]), lane == 0);
+        if (!tc_wait_warp(bar(&sh.ofull[grp]), 0u, abort_flag)) {  // the first half's product
+          ok = false;
+          break;
         }
-        if (__all_sync(0xffffffffu, !live || over <= kTcLazy)) {
-          l += sum.x + sum.y;
-          done = true;
-        }
+        ptx::mbar_arrive_if(bar(&sh.pready[grp]), lane == 0);
+        continue;
       }
-      if (!done) {
-        float mx = -INFINITY;
-#pragma unroll 1
-        for (int q = 0; q < 4; ++q) {
-          uint32_t s[32];
-          tc::ld32(ts + 32u * q, s);
-          tc::wait_ld32(s);
-#pragma unroll
-          for (int k = 0; k < 32; ++k)
-            if (t + 32 * q + k < seen) mx = fmaxf(mx, __uint_as_float(s[k]) * c);
-        }
-        const float mn = fmaxf(m, mx), ref = mn == -INFINITY ? 0.f : mn;
-        const float f = exp2f(m - ref);
-        m = mn;
-        l *= f;
-        if (j > 0 && __any_sync(0xffffffffu, f != 1.f)) {
-          if (!tc_wait_warp(bar(&sh.ofull[grp]), (uint32_t)((j - 1) & 1), abort_flag)) {
+      tc::fence_after();
+      // Whole steps and steps that some row does not see to the end are code of
+      // their own: the comparisons would cost the first a third of its instructions.
+      auto step = [&](auto is_masked) {
+        constexpr bool masked = decltype(is_masked)::value;
+        uint32_t sa[32], sb[32];
+        tc::ld32(ts, sa);
+        tc::ld32(ts + 32u, sb);
+        // Half the step at a time (64 tokens): its weights go over scores already
+        // read, and the value product of the half can start.
+  #pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          const int at = t + 64 * h;
+          uint32_t p[32];
+          tc::wait_ld32(sa);
+          tc::wait_ld32(sb);
+          float sum = weigh<masked>(sa, m, c, at, seen, p);
+          if (h == 0) tc::ld32(ts + 64u, sa);
+          sum += weigh<masked>(sb, m, c, at + 32, seen, p + 16);
+          if (h == 0) tc::ld32(ts + 96u, sb);
+          // Weights are taken against the maximum as it stands; only where their
+          // sum is past kTcLazySum is it raised, the output so far rescaled, and
+          // the scores of the half read and weighed again.
+          if (__any_sync(0xffffffffu, !(sum <= kTcLazySum) || (m == -INFINITY && at < seen))) {
+            float mx = -INFINITY;
+  #pragma unroll 1
+            for (int u = 0; u < 4; ++u) {
+              uint32_t s[16];
+              tc::ld16(ts + 64u * h + 16u * u, s);
+              tc::wait_ld16(s);
+  #pragma unroll
+              for (int k = 0; k < 16; ++k)
+                if (at + 16 * u + k < seen) mx = fmaxf(mx, __uint_as_float(s[k]) * c);
+            }
+            const float mn = fmaxf(m, mx);
+            const float f = m == mn ? 1.f : exp2f(m - mn);
+            m = mn;
+            l *= f;
+            if (2 * j + h > 0 && __any_sync(0xffffffffu, f != 1.f)) {
+              if (!tc_wait_warp(bar(&sh.ofull[grp]), (uint32_t)((h + 1) & 1), abort_flag)) {
+                ok = false;
+                break;
+              }
+              tc::fence_after();
+  #pragma unroll 1
+              for (int u = 0; u < D / 16; ++u) {
+                uint32_t o[16];
+                tc::ld16(to + 16u * u, o);
+                tc::wait_ld16(o);
+  #pragma unroll
+                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                tc::st16(to + 16u * u, o);
+              }
+            }
+            sum = 0.f;
+  #pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              uint32_t s[32];
+              tc::ld32(ts + 64u * h + 32u * u, s);
+              tc::wait_ld32(s);
+              sum += weigh<true>(s, m, c, at + 32 * u, seen, p + 16 * u);
+            }
+          }
+          l += sum;
+          tc::st32(ts + 32u * h, p);
+          tc::wait_st();
+          // every phase of ofull is waited for, or a later wait could take it for another
+          if (h == 1 && !tc_wait_warp(bar(&sh.ofull[grp]), 0u, abort_flag)) {
             ok = false;
             break;
           }
-          tc::fence_after();
-#pragma unroll 1
-          for (int q = 0; q < D / 32; ++q) {
-            uint32_t o[32];
-            tc::ld32(to + 32u * q, o);
-            tc::wait_ld32(o);
-#pragma unroll
-            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-            tc::st32(to + 32u * q, o);
-          }
+          tc::fence_before();
+          __syncwarp();
+          ptx::mbar_arrive_if(bar(&sh.pready[grp]), lane == 0);
         }
-        float sum = 0.f;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint32_t s[32];
-          tc::ld32(ts + 32u * q, s);
-          tc::wait_ld32(s);
-#pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            const int at = t + 32 * q + 2 * k;
-            const float e0 = at < seen ? ex2(fmaf(__uint_as_float(s[2 * k]), c, -ref)) : 0.f;
-            const float e1 = at + 1 < seen ? ex2(fmaf(__uint_as_float(s[2 * k + 1]), c, -ref)) : 0.f;
-            sum += e0 + e1;
-            p[16 * q + k] = narrow2<KVF_DT_F16>(e0, e1);
-          }
-        }
-        l += sum;
-      }
-      {
-        uint32_t x[32];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-          for (int k = 0; k < 32; ++k) x[k] = p[32 * h + k];
-          tc::st32(ts + 32u * h, x);
-        }
-      }
-      tc::wait_st();
-      tc::fence_before();
-      __syncwarp();
-      ptx::mbar_arrive_if(bar(&sh.pready[grp]), lane == 0);
+      };
+      if (__any_sync(0xffffffffu, t + kTcStep > seen))
+        step(std::true_type{});
+      else
+        step(std::false_type{});
+      if (!ok) break;
     }
-    if (ok && steps > 0 && !tc_wait_warp(bar(&sh.ofull[grp]), (uint32_t)((steps - 1) & 1), abort_flag)) ok = false;
+    if (ok && steps > 0 && !tc_wait_warp(bar(&sh.ofull[grp]), 1u, abort_flag)) ok = false;  // second half of the last step
     tc::fence_after();
     if (!ok && lane == 0) {
       atomicOr(&g_kvfb_chunk_error, 1u);
@@ -692,25 +740,27 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
         }
         __syncwarp();
       };
-      auto values = [&](int g, int i, bool acc) {
+      // O += P V for group g's step j on V tile i, each half once its weights are there.
+      auto values = [&](int g, int i, int j) -> bool {
         const uint64_t dv = tc::smem_desc(svr + (uint32_t)(i % SLOTS) * TILE, BLK, 1024u, tc::kSwizzle128);
-        if (tc::elect_one()) {
 #pragma unroll
-          for (int ks = 0; ks < kTcStep / 16; ++ks)
-            tc::mma_f16_ta(tbase + O_COL + (uint32_t)(D * g), tbase + S_COL + 128u * g + 8u * ks, dv + ks * (2048u >> 4), ID_O,
-                           acc || ks > 0);
-          tc::commit(bar(&sh.ofull[g]));
+        for (int h = 0; h < 2; ++h) {
+          if (!tc_wait_warp(bar(&sh.pready[g]), (uint32_t)h, abort_flag)) return ok = false;
+          tc::fence_after();
+          if (tc::elect_one()) {
+#pragma unroll
+            for (int ks = 4 * h; ks < 4 * h + 4; ++ks)
+              tc::mma_f16_ta(tbase + O_COL + (uint32_t)(D * g), tbase + S_COL + 128u * g + 8u * ks, dv + ks * (2048u >> 4),
+                             ID_O, j > 0 || ks > 0);
+            tc::commit(bar(&sh.ofull[g]));
+          }
+          __syncwarp();
         }
-        __syncwarp();
+        return true;
       };
       auto release = [&](const uint64_t *b) {
         if (tc::elect_one()) tc::commit(bar(b));
         __syncwarp();
-      };
-      auto weights = [&](int g, int j) -> bool {
-        if (!tc_wait_warp(bar(&sh.pready[g]), (uint32_t)(j & 1), abort_flag)) return ok = false;
-        tc::fence_after();
-        return true;
       };
       if (TWO) {
         if (n > 0 && take_k(0)) {
@@ -723,10 +773,7 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
           bool have = false;
           const int last = i < nw[1] ? 1 : 0;
           for (int g = 0; g < 2 && ok; ++g) {
-            if (i < nw[g]) {
-              if (!weights(g, i)) break;
-              values(g, i, i > 0);
-            }
+            if (i < nw[g] && !values(g, i, i)) break;
             if (g == last) release(&sh.vempty[i % SLOTS]);
             if (i + 1 < nw[g]) {
               if (!have && !take_k(i + 1)) break;
@@ -747,8 +794,7 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
           }
         for (int i = 0; i < n && ok; ++i) {
           const int g = i & 1, j = i >> 1;
-          if (!take_v(i) || !weights(g, j)) break;
-          values(g, i, j > 0);
+          if (!take_v(i) || !values(g, i, j)) break;
           release(&sh.vempty[i % SLOTS]);
           if (i + 2 < n && take_k(i + 2)) {
             scores(g, i + 2);
