@@ -19,12 +19,13 @@
 //          (64 tokens) land in a ring of their own and become fp16 tiles of 128
 //          tokens x 64 channels with the 128-byte swizzle. f16 caches: TMA writes
 //          those tiles itself, and group 2 only clears what must not be seen;
-//   last   one warp issues the MMAs (one thread): S = Q K^T into tensor memory,
-//          O += P V with P read from tensor memory, where the softmax group writes
-//          it over its scores, and V read MN-major. Two warps are the producers of K
-//          and of V: TMA boxes per page, metadata rows by cp.async. A box of tokens
-//          that nobody sees, or of a block mapped to a negative page, is asked for
-//          at page -1, which TMA fills with zeros.
+//   last   two warps issue the MMAs (one lane each), one per softmax group, so that
+//          neither waits on the other's weights: S = Q K^T into tensor memory, O += P V
+//          with P read from tensor memory, where the softmax group writes it over its
+//          scores, and V read MN-major. The other two are the producers of K and of V:
+//          TMA boxes per page, metadata rows by cp.async. A box of tokens that nobody
+//          sees, or of a block mapped to a negative page, is asked for at page -1,
+//          which TMA fills with zeros.
 // The running maximum a row's weights are taken against is raised only when 64
 // of them add up to more than 256 (weights up to that fit fp16, and their sum
 // fp32), so the output in tensor memory is rescaled rarely, a step's scores are
@@ -50,7 +51,7 @@ namespace {
 constexpr int kTcRows = 128;    // rows of a tile
 constexpr int kTcStep = 128;    // tokens of a step
 constexpr int kTcHalf = 64;     // tokens of a raw half step
-constexpr int kTcPoly = 4;           // one pair of weights in this many is computed without the special function unit
+constexpr int kTcPoly = 0;           // one pair of weights in this many is computed without the special function unit
 constexpr float kTcLazySum = 256.f;  // most that 64 weights may add up to before the maximum is raised
 
 __host__ __device__ constexpr int cache_row_bytes(int fmt, int d) {
@@ -69,7 +70,9 @@ template <int FMT, int D, bool TWO> struct TcLayout {
   static_assert(2 * SOFT_REGS + (RAW ? 2 : 1) * CONV_REGS + LAST_REGS <= (RAW ? 96 * 5 : 128 * 4), "registers");
   static constexpr uint32_t TILE = kTcStep * D * 2;
   static constexpr uint32_t QB = (TWO ? 2u : 1u) * TILE;
-  static constexpr int SLOTS = RAW || TWO ? 2 : 3;           // fp16 tiles per operand
+  // fp16 tiles per operand. Without TWO a tile belongs to one issuer, which must
+  // meet every phase of its slots' barriers: an even number.
+  static constexpr int SLOTS = RAW || TWO || D == 128 ? 2 : 4;
   static constexpr uint32_t RAWB = RAW ? kTcHalf * (uint32_t)cache_row_bytes(FMT, D) : 0u;
   static constexpr uint32_t METAB = RAW ? kTcHalf * (FMT == KVF_FMT_INT8 ? 8u : 16u) : 0u;
   static constexpr uint32_t FREE = 232448u - 1024u - QB - 2u * SLOTS * TILE;
@@ -79,21 +82,21 @@ template <int FMT, int D, bool TWO> struct TcLayout {
   static constexpr uint32_t OFF_RAW = OFF_RING + 2u * SLOTS * TILE;
   static constexpr uint32_t OFF_META = OFF_RAW + 2u * RSLOTS * RAWB;
   static constexpr uint32_t OFF_MISC = OFF_META + 2u * RSLOTS * METAB;
-  static constexpr uint32_t BYTES = OFF_MISC + 512u;
+  static constexpr uint32_t BYTES = OFF_MISC + 1024u;
   static_assert(!RAW || RSLOTS >= 2, "two raw half steps per operand");
   static_assert(BYTES <= 232448u, "shared memory");
 };
 
 struct TcShared {
-  uint64_t kfull[3], kempty[3], vfull[3], vempty[3];
-  uint64_t sfull[2], pready[2], ofull[2];
-  uint64_t vraw[3], vfixed[3], done;  // vraw, vfixed: f16 V tiles on their way through group 2
+  uint64_t kfull[4], kempty[4], vfull[4], vempty[4];
+  uint64_t sfull[2], pready[2][2], ofull[2][2];  // pready, ofull: per half step
+  uint64_t vraw[4], vfixed[4], done;  // vraw, vfixed: f16 V tiles on their way through group 2
   uint64_t rfull[2][8], rempty[2][8];
   uint32_t tmem;
   int abort_flag;
   int odd;            // a masked V tile held an infinity or NaN, taken as 0
 };
-static_assert(sizeof(TcShared) <= 512, "misc area");
+static_assert(sizeof(TcShared) <= 1024, "misc area");
 
 template <int N> __device__ __forceinline__ void regs_up() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -244,21 +247,23 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
       // filled by four converter warps, or by TMA
       ptx::mbar_init(bar(&sh.kfull[s]), L::RAW ? 4u : 1u);
       ptx::mbar_init(bar(&sh.vfull[s]), L::RAW ? 4u : 1u);
-      ptx::mbar_init(bar(&sh.kempty[s]), 1u);
-      ptx::mbar_init(bar(&sh.vempty[s]), 1u);
+      ptx::mbar_init(bar(&sh.kempty[s]), TWO ? 2u : 1u);  // by each issuer that uses the tile
+      ptx::mbar_init(bar(&sh.vempty[s]), TWO ? 2u : 1u);
       ptx::mbar_init(bar(&sh.vraw[s]), 1u);
       ptx::mbar_init(bar(&sh.vfixed[s]), 4u);
     }
     for (int g = 0; g < 2; ++g) {
       ptx::mbar_init(bar(&sh.sfull[g]), 1u);
-      ptx::mbar_init(bar(&sh.pready[g]), 4u);
-      ptx::mbar_init(bar(&sh.ofull[g]), 1u);
+      ptx::mbar_init(bar(&sh.pready[g][0]), 4u);
+      ptx::mbar_init(bar(&sh.pready[g][1]), 4u);
+      ptx::mbar_init(bar(&sh.ofull[g][0]), 1u);
+      ptx::mbar_init(bar(&sh.ofull[g][1]), 1u);
       for (int s = 0; s < RSLOTS; ++s) {
         ptx::mbar_init(bar(&sh.rfull[g][s]), 33u);  // the boxes' bytes, and 32 lanes of cp.async
         ptx::mbar_init(bar(&sh.rempty[g][s]), 4u);
       }
     }
-    ptx::mbar_init(bar(&sh.done), 1u);
+    ptx::mbar_init(bar(&sh.done), 2u);
     ptx::fence_barrier_init();
   }
   if (warp == LAST) {
@@ -329,12 +334,8 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
         break;
       }
       if (idle) {
-        ptx::mbar_arrive_if(bar(&sh.pready[grp]), lane == 0);
-        if (!tc_wait_warp(bar(&sh.ofull[grp]), 0u, abort_flag)) {  // the first half's product
-          ok = false;
-          break;
-        }
-        ptx::mbar_arrive_if(bar(&sh.pready[grp]), lane == 0);
+        ptx::mbar_arrive_if(bar(&sh.pready[grp][0]), lane == 0);
+        ptx::mbar_arrive_if(bar(&sh.pready[grp][1]), lane == 0);
         continue;
       }
       tc::fence_after();
@@ -347,7 +348,7 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
         tc::ld32(ts + 32u, sb);
         // Half the step at a time (64 tokens): its weights go over scores already
         // read, and the value product of the half can start.
-  #pragma unroll 1
+#pragma unroll 1
         for (int h = 0; h < 2; ++h) {
           const int at = t + 64 * h;
           uint32_t p[32];
@@ -362,12 +363,12 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
           // the scores of the half read and weighed again.
           if (__any_sync(0xffffffffu, !(sum <= kTcLazySum) || (m == -INFINITY && at < seen))) {
             float mx = -INFINITY;
-  #pragma unroll 1
+#pragma unroll 1
             for (int u = 0; u < 4; ++u) {
               uint32_t s[16];
               tc::ld16(ts + 64u * h + 16u * u, s);
               tc::wait_ld16(s);
-  #pragma unroll
+#pragma unroll
               for (int k = 0; k < 16; ++k)
                 if (at + 16 * u + k < seen) mx = fmaxf(mx, __uint_as_float(s[k]) * c);
             }
@@ -376,23 +377,24 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
             m = mn;
             l *= f;
             if (2 * j + h > 0 && __any_sync(0xffffffffu, f != 1.f)) {
-              if (!tc_wait_warp(bar(&sh.ofull[grp]), (uint32_t)((h + 1) & 1), abort_flag)) {
+              // the half before this one; those before it were done when the scores came
+              if (!tc_wait_warp(bar(&sh.ofull[grp][h ^ 1]), (uint32_t)((h ? j : j - 1) & 1), abort_flag)) {
                 ok = false;
                 break;
               }
               tc::fence_after();
-  #pragma unroll 1
+#pragma unroll 1
               for (int u = 0; u < D / 16; ++u) {
                 uint32_t o[16];
                 tc::ld16(to + 16u * u, o);
                 tc::wait_ld16(o);
-  #pragma unroll
+#pragma unroll
                 for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
                 tc::st16(to + 16u * u, o);
               }
             }
             sum = 0.f;
-  #pragma unroll
+#pragma unroll
             for (int u = 0; u < 2; ++u) {
               uint32_t s[32];
               tc::ld32(ts + 64u * h + 32u * u, s);
@@ -403,14 +405,9 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
           l += sum;
           tc::st32(ts + 32u * h, p);
           tc::wait_st();
-          // every phase of ofull is waited for, or a later wait could take it for another
-          if (h == 1 && !tc_wait_warp(bar(&sh.ofull[grp]), 0u, abort_flag)) {
-            ok = false;
-            break;
-          }
           tc::fence_before();
           __syncwarp();
-          ptx::mbar_arrive_if(bar(&sh.pready[grp]), lane == 0);
+          ptx::mbar_arrive_if(bar(&sh.pready[grp][h]), lane == 0);
         }
       };
       if (__any_sync(0xffffffffu, t + kTcStep > seen))
@@ -419,7 +416,7 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
         step(std::false_type{});
       if (!ok) break;
     }
-    if (ok && steps > 0 && !tc_wait_warp(bar(&sh.ofull[grp]), 1u, abort_flag)) ok = false;  // second half of the last step
+    if (ok && steps > 0 && !tc_wait_warp(bar(&sh.ofull[grp][1]), (uint32_t)((steps - 1) & 1), abort_flag)) ok = false;
     tc::fence_after();
     if (!ok && lane == 0) {
       atomicOr(&g_kvfb_chunk_error, 1u);
@@ -710,7 +707,8 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
       if (!ptx::mbar_wait(full, (uint32_t)(((fixed ? k - first_masked : k) / RING) & 1)) && lane == 0) atomicOr(&g_kvfb_chunk_error, 1u);
     }
     // ----------------------------------------------------------- MMA issue
-    } else if (warp == LAST) {
+    } else {
+      const int g = warp == LAST ? 0 : 1;  // the softmax group that this warp issues for
       constexpr uint32_t ID_S = tc::idesc_f16(false, false, 128, 128), ID_O = tc::idesc_f16(false, true, 128, D);
       bool ok = true;
       // Waits for K or V tile i.
@@ -727,7 +725,7 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
         tc::fence_after();
         return true;
       };
-      auto scores = [&](int g, int i) {
+      auto scores = [&](int i) {
         const uint32_t q = sq + (TWO ? (uint32_t)g * TILE : 0u), k = skr + (uint32_t)(i % SLOTS) * TILE;
         const uint64_t dq = tc::smem_desc(q, 16u, 1024u, tc::kSwizzle128), dk = tc::smem_desc(k, 16u, 1024u, tc::kSwizzle128);
         if (tc::elect_one()) {
@@ -740,19 +738,19 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
         }
         __syncwarp();
       };
-      // O += P V for group g's step j on V tile i, each half once its weights are there.
-      auto values = [&](int g, int i, int j) -> bool {
+      // O += P V for the group's step j on V tile i, each half once its weights are there.
+      auto values = [&](int i, int j) -> bool {
         const uint64_t dv = tc::smem_desc(svr + (uint32_t)(i % SLOTS) * TILE, BLK, 1024u, tc::kSwizzle128);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          if (!tc_wait_warp(bar(&sh.pready[g]), (uint32_t)h, abort_flag)) return ok = false;
+          if (!tc_wait_warp(bar(&sh.pready[g][h]), (uint32_t)(j & 1), abort_flag)) return ok = false;
           tc::fence_after();
           if (tc::elect_one()) {
 #pragma unroll
             for (int ks = 4 * h; ks < 4 * h + 4; ++ks)
               tc::mma_f16_ta(tbase + O_COL + (uint32_t)(D * g), tbase + S_COL + 128u * g + 8u * ks, dv + ks * (2048u >> 4),
                              ID_O, j > 0 || ks > 0);
-            tc::commit(bar(&sh.ofull[g]));
+            tc::commit(bar(&sh.ofull[g][h]));
           }
           __syncwarp();
         }
@@ -764,40 +762,27 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
       };
       if (TWO) {
         if (n > 0 && take_k(0)) {
-          for (int g = 0; g < 2; ++g)
-            if (nw[g] > 0) scores(g, 0);
+          if (nw[g] > 0) scores(0);
           release(&sh.kempty[0]);
         }
         for (int i = 0; i < n && ok; ++i) {
-          if (!take_v(i)) break;
-          bool have = false;
-          const int last = i < nw[1] ? 1 : 0;
-          for (int g = 0; g < 2 && ok; ++g) {
-            if (i < nw[g] && !values(g, i, i)) break;
-            if (g == last) release(&sh.vempty[i % SLOTS]);
-            if (i + 1 < nw[g]) {
-              if (!have && !take_k(i + 1)) break;
-              have = true;
-              scores(g, i + 1);
-            }
-          }
-          if (ok && i + 1 < n) {
-            if (!have && !take_k(i + 1)) break;
+          if (!take_v(i) || (i < nw[g] && !values(i, i))) break;
+          release(&sh.vempty[i % SLOTS]);
+          if (i + 1 < n && take_k(i + 1)) {
+            if (i + 1 < nw[g]) scores(i + 1);
             release(&sh.kempty[(i + 1) % SLOTS]);
           }
         }
       } else {
-        for (int g = 0; g < 2 && g < n && ok; ++g)
-          if (take_k(g)) {
-            scores(g, g);
-            release(&sh.kempty[g % SLOTS]);
-          }
-        for (int i = 0; i < n && ok; ++i) {
-          const int g = i & 1, j = i >> 1;
-          if (!take_v(i) || !values(g, i, j)) break;
+        if (g < n && take_k(g)) {
+          scores(g);
+          release(&sh.kempty[g % SLOTS]);
+        }
+        for (int i = g; i < n && ok; i += 2) {
+          if (!take_v(i) || !values(i, i >> 1)) break;
           release(&sh.vempty[i % SLOTS]);
           if (i + 2 < n && take_k(i + 2)) {
-            scores(g, i + 2);
+            scores(i + 2);
             release(&sh.kempty[(i + 2) % SLOTS]);
           }
         }
