@@ -89,7 +89,7 @@ template <int FMT, int D, bool TWO> struct TcLayout {
 
 struct TcShared {
   uint64_t kfull[4], kempty[4], vfull[4], vempty[4];
-  uint64_t sfull[2], pready[2][2], ofull[2][2];  // pready, ofull: per half step
+  uint64_t sfull[2][2], pready[2][2], ofull[2][2];  // per group and half step
   uint64_t vraw[4], vfixed[4], done;  // vraw, vfixed: f16 V tiles on their way through group 2
   uint64_t rfull[2][8], rempty[2][8];
   uint32_t tmem;
@@ -253,11 +253,11 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
       ptx::mbar_init(bar(&sh.vfixed[s]), 4u);
     }
     for (int g = 0; g < 2; ++g) {
-      ptx::mbar_init(bar(&sh.sfull[g]), 1u);
-      ptx::mbar_init(bar(&sh.pready[g][0]), 4u);
-      ptx::mbar_init(bar(&sh.pready[g][1]), 4u);
-      ptx::mbar_init(bar(&sh.ofull[g][0]), 1u);
-      ptx::mbar_init(bar(&sh.ofull[g][1]), 1u);
+      for (int h = 0; h < 2; ++h) {
+        ptx::mbar_init(bar(&sh.sfull[g][h]), 1u);
+        ptx::mbar_init(bar(&sh.pready[g][h]), 4u);
+        ptx::mbar_init(bar(&sh.ofull[g][h]), 1u);
+      }
       for (int s = 0; s < RSLOTS; ++s) {
         ptx::mbar_init(bar(&sh.rfull[g][s]), 33u);  // the boxes' bytes, and 32 lanes of cp.async
         ptx::mbar_init(bar(&sh.rempty[g][s]), 4u);
@@ -329,91 +329,93 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
     bool ok = true;
     for (int j = 0; j < steps; ++j) {
       const int t = w.t0 + (TWO ? j : 2 * j + grp) * kTcStep;
-      if (!tc_wait_warp(bar(&sh.sfull[grp]), (uint32_t)(j & 1), abort_flag)) {
-        ok = false;
-        break;
-      }
-      if (idle) {
-        ptx::mbar_arrive_if(bar(&sh.pready[grp][0]), lane == 0);
-        ptx::mbar_arrive_if(bar(&sh.pready[grp][1]), lane == 0);
-        continue;
-      }
-      tc::fence_after();
-      // Whole steps and steps that some row does not see to the end are code of
-      // their own: the comparisons would cost the first a third of its instructions.
-      auto step = [&](auto is_masked) {
+      // Half a step at a time (64 tokens), each half with scores, weights and
+      // barriers of its own: while one half is weighed, the tensor cores take the
+      // other's value product and its next scores. Whole steps and steps that some
+      // row does not see to the end are code of their own: the comparisons would
+      // cost the first a third of its instructions.
+      auto half = [&](int h, auto is_masked) {
         constexpr bool masked = decltype(is_masked)::value;
-        uint32_t sa[32], sb[32];
-        tc::ld32(ts, sa);
-        tc::ld32(ts + 32u, sb);
-        // Half the step at a time (64 tokens): its weights go over scores already
-        // read, and the value product of the half can start.
-#pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
-          const int at = t + 64 * h;
-          uint32_t p[32];
+        const int at = t + 64 * h;
+        const uint32_t tsh = ts + 64u * h;
+        uint32_t p[32];
+        float sum;
+        {
+          uint32_t sa[32], sb[32];
+          tc::ld32(tsh, sa);
+          tc::ld32(tsh + 32u, sb);
           tc::wait_ld32(sa);
           tc::wait_ld32(sb);
-          float sum = weigh<masked>(sa, m, c, at, seen, p);
-          if (h == 0) tc::ld32(ts + 64u, sa);
+          sum = weigh<masked>(sa, m, c, at, seen, p);
           sum += weigh<masked>(sb, m, c, at + 32, seen, p + 16);
-          if (h == 0) tc::ld32(ts + 96u, sb);
-          // Weights are taken against the maximum as it stands; only where their
-          // sum is past kTcLazySum is it raised, the output so far rescaled, and
-          // the scores of the half read and weighed again.
-          if (__any_sync(0xffffffffu, !(sum <= kTcLazySum) || (m == -INFINITY && at < seen))) {
-            float mx = -INFINITY;
+        }
+        // Weights are taken against the maximum as it stands; only where their
+        // sum is past kTcLazySum is it raised, the output so far rescaled, and
+        // the scores of the half read and weighed again.
+        if (__any_sync(0xffffffffu, !(sum <= kTcLazySum) || (m == -INFINITY && at < seen))) {
+          float mx = -INFINITY;
 #pragma unroll 1
-            for (int u = 0; u < 4; ++u) {
-              uint32_t s[16];
-              tc::ld16(ts + 64u * h + 16u * u, s);
-              tc::wait_ld16(s);
+          for (int u = 0; u < 4; ++u) {
+            uint32_t s[16];
+            tc::ld16(tsh + 16u * u, s);
+            tc::wait_ld16(s);
 #pragma unroll
-              for (int k = 0; k < 16; ++k)
-                if (at + 16 * u + k < seen) mx = fmaxf(mx, __uint_as_float(s[k]) * c);
+            for (int k = 0; k < 16; ++k)
+              if (at + 16 * u + k < seen) mx = fmaxf(mx, __uint_as_float(s[k]) * c);
+          }
+          const float mn = fmaxf(m, mx);
+          const float f = m == mn ? 1.f : exp2f(m - mn);
+          m = mn;
+          l *= f;
+          if (2 * j + h > 0 && __any_sync(0xffffffffu, f != 1.f)) {
+            // the half before this one; those before it were done when the scores came
+            if (!tc_wait_warp(bar(&sh.ofull[grp][h ^ 1]), (uint32_t)((h ? j : j - 1) & 1), abort_flag)) {
+              ok = false;
+              return;
             }
-            const float mn = fmaxf(m, mx);
-            const float f = m == mn ? 1.f : exp2f(m - mn);
-            m = mn;
-            l *= f;
-            if (2 * j + h > 0 && __any_sync(0xffffffffu, f != 1.f)) {
-              // the half before this one; those before it were done when the scores came
-              if (!tc_wait_warp(bar(&sh.ofull[grp][h ^ 1]), (uint32_t)((h ? j : j - 1) & 1), abort_flag)) {
-                ok = false;
-                break;
-              }
-              tc::fence_after();
+            tc::fence_after();
 #pragma unroll 1
-              for (int u = 0; u < D / 16; ++u) {
-                uint32_t o[16];
-                tc::ld16(to + 16u * u, o);
-                tc::wait_ld16(o);
+            for (int u = 0; u < D / 16; ++u) {
+              uint32_t o[16];
+              tc::ld16(to + 16u * u, o);
+              tc::wait_ld16(o);
 #pragma unroll
-                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-                tc::st16(to + 16u * u, o);
-              }
-            }
-            sum = 0.f;
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              uint32_t s[32];
-              tc::ld32(ts + 64u * h + 32u * u, s);
-              tc::wait_ld32(s);
-              sum += weigh<true>(s, m, c, at + 32 * u, seen, p + 16 * u);
+              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+              tc::st16(to + 16u * u, o);
             }
           }
-          l += sum;
-          tc::st32(ts + 32u * h, p);
-          tc::wait_st();
-          tc::fence_before();
-          __syncwarp();
-          ptx::mbar_arrive_if(bar(&sh.pready[grp][h]), lane == 0);
+          sum = 0.f;
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            uint32_t s[32];
+            tc::ld32(tsh + 32u * u, s);
+            tc::wait_ld32(s);
+            sum += weigh<true>(s, m, c, at + 32 * u, seen, p + 16 * u);
+          }
         }
+        l += sum;
+        tc::st32(tsh, p);
+        tc::wait_st();
+        tc::fence_before();
       };
-      if (__any_sync(0xffffffffu, t + kTcStep > seen))
-        step(std::true_type{});
-      else
-        step(std::false_type{});
+      const bool masked = __any_sync(0xffffffffu, t + kTcStep > seen);
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {
+        if (!tc_wait_warp(bar(&sh.sfull[grp][h]), (uint32_t)(j & 1), abort_flag)) {
+          ok = false;
+          break;
+        }
+        if (!idle) {
+          tc::fence_after();
+          if (masked)
+            half(h, std::true_type{});
+          else
+            half(h, std::false_type{});
+          if (!ok) break;
+          __syncwarp();
+        }
+        ptx::mbar_arrive_if(bar(&sh.pready[grp][h]), lane == 0);
+      }
       if (!ok) break;
     }
     if (ok && steps > 0 && !tc_wait_warp(bar(&sh.ofull[grp][1]), (uint32_t)((steps - 1) & 1), abort_flag)) ok = false;
@@ -709,7 +711,7 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
     // ----------------------------------------------------------- MMA issue
     } else {
       const int g = warp == LAST ? 0 : 1;  // the softmax group that this warp issues for
-      constexpr uint32_t ID_S = tc::idesc_f16(false, false, 128, 128), ID_O = tc::idesc_f16(false, true, 128, D);
+      constexpr uint32_t ID_S = tc::idesc_f16(false, false, 128, 64), ID_O = tc::idesc_f16(false, true, 128, D);
       bool ok = true;
       // Waits for K or V tile i.
       auto take_k = [&](int i) -> bool {
@@ -725,67 +727,58 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
         tc::fence_after();
         return true;
       };
-      auto scores = [&](int i) {
-        const uint32_t q = sq + (TWO ? (uint32_t)g * TILE : 0u), k = skr + (uint32_t)(i % SLOTS) * TILE;
+      // S = Q K^T for half h of K tile i, and O += P V for half h of V tile i (the
+      // group's step j) once the weights are there.
+      auto scores = [&](int i, int h) {
+        const uint32_t q = sq + (TWO ? (uint32_t)g * TILE : 0u), k = skr + (uint32_t)(i % SLOTS) * TILE + 8192u * h;
         const uint64_t dq = tc::smem_desc(q, 16u, 1024u, tc::kSwizzle128), dk = tc::smem_desc(k, 16u, 1024u, tc::kSwizzle128);
         if (tc::elect_one()) {
 #pragma unroll
           for (int ks = 0; ks < D / 16; ++ks) {
             const uint32_t off = ((ks >> 2) * BLK + (ks & 3) * 32u) >> 4;  // descriptors count 16-byte units
-            tc::mma_f16_ss(tbase + S_COL + 128u * g, dq + off, dk + off, ID_S, ks > 0);
+            tc::mma_f16_ss(tbase + S_COL + 128u * g + 64u * h, dq + off, dk + off, ID_S, ks > 0);
           }
-          tc::commit(bar(&sh.sfull[g]));
+          tc::commit(bar(&sh.sfull[g][h]));
         }
         __syncwarp();
       };
-      // O += P V for the group's step j on V tile i, each half once its weights are there.
-      auto values = [&](int i, int j) -> bool {
-        const uint64_t dv = tc::smem_desc(svr + (uint32_t)(i % SLOTS) * TILE, BLK, 1024u, tc::kSwizzle128);
+      auto values = [&](int i, int j, int h) -> bool {
+        const uint64_t dv = tc::smem_desc(svr + (uint32_t)(i % SLOTS) * TILE + 8192u * h, BLK, 1024u, tc::kSwizzle128);
+        if (!tc_wait_warp(bar(&sh.pready[g][h]), (uint32_t)(j & 1), abort_flag)) return ok = false;
+        tc::fence_after();
+        if (tc::elect_one()) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (!tc_wait_warp(bar(&sh.pready[g][h]), (uint32_t)(j & 1), abort_flag)) return ok = false;
-          tc::fence_after();
-          if (tc::elect_one()) {
-#pragma unroll
-            for (int ks = 4 * h; ks < 4 * h + 4; ++ks)
-              tc::mma_f16_ta(tbase + O_COL + (uint32_t)(D * g), tbase + S_COL + 128u * g + 8u * ks, dv + ks * (2048u >> 4),
-                             ID_O, j > 0 || ks > 0);
-            tc::commit(bar(&sh.ofull[g][h]));
-          }
-          __syncwarp();
+          for (int ks = 0; ks < 4; ++ks)
+            tc::mma_f16_ta(tbase + O_COL + (uint32_t)(D * g), tbase + S_COL + 128u * g + 64u * h + 8u * ks, dv + ks * (2048u >> 4),
+                           ID_O, j > 0 || h > 0 || ks > 0);
+          tc::commit(bar(&sh.ofull[g][h]));
         }
+        __syncwarp();
         return true;
       };
       auto release = [&](const uint64_t *b) {
         if (tc::elect_one()) tc::commit(bar(b));
         __syncwarp();
       };
-      if (TWO) {
-        if (n > 0 && take_k(0)) {
-          if (nw[g] > 0) scores(0);
-          release(&sh.kempty[0]);
+      // Tiles: every one (TWO; past the group's last step only to hand it back), or
+      // every second.
+      constexpr int STRIDE = TWO ? 1 : 2;
+      int i = TWO ? 0 : g;
+      if (i < n && take_k(i)) {
+        if (nw[g] > 0)
+          for (int h = 0; h < 2; ++h) scores(i, h);
+        release(&sh.kempty[i % SLOTS]);
+      }
+      for (int j = 0; i < n && ok; ++j, i += STRIDE) {
+        if (!take_v(i)) break;
+        const int next = i + STRIDE;
+        const bool more = next < n;
+        for (int h = 0; h < 2 && ok; ++h) {
+          if (j < nw[g] && !values(i, j, h)) break;
+          if (h == 1) release(&sh.vempty[i % SLOTS]);
+          if (more && (h == 1 || take_k(next)) && j + 1 < nw[g]) scores(next, h);
         }
-        for (int i = 0; i < n && ok; ++i) {
-          if (!take_v(i) || (i < nw[g] && !values(i, i))) break;
-          release(&sh.vempty[i % SLOTS]);
-          if (i + 1 < n && take_k(i + 1)) {
-            if (i + 1 < nw[g]) scores(i + 1);
-            release(&sh.kempty[(i + 1) % SLOTS]);
-          }
-        }
-      } else {
-        if (g < n && take_k(g)) {
-          scores(g);
-          release(&sh.kempty[g % SLOTS]);
-        }
-        for (int i = g; i < n && ok; i += 2) {
-          if (!take_v(i) || !values(i, i >> 1)) break;
-          release(&sh.vempty[i % SLOTS]);
-          if (i + 2 < n && take_k(i + 2)) {
-            scores(i + 2);
-            release(&sh.kempty[(i + 2) % SLOTS]);
-          }
-        }
+        if (more && ok) release(&sh.kempty[next % SLOTS]);
       }
       if (!ok && lane == 0) {
         atomicOr(&g_kvfb_chunk_error, 1u);
