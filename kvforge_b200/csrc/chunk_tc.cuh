@@ -326,7 +326,8 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
     const uint32_t ts = tbase + lanes + S_COL + 128u * grp, to = tbase + lanes + O_COL + (uint32_t)(D * grp);
     const int steps = nw[grp];
     float m = -INFINITY, l = 0.f;
-    bool ok = true;
+    bool ok = true, early = false;
+    uint32_t sa[32], sb[32];                // scores of the half at hand, or (early) of the next
     for (int j = 0; j < steps; ++j) {
       const int t = w.t0 + (TWO ? j : 2 * j + grp) * kTcStep;
       // Half a step at a time (64 tokens), each half with scores, weights and
@@ -339,16 +340,14 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
         const int at = t + 64 * h;
         const uint32_t tsh = ts + 64u * h;
         uint32_t p[32];
-        float sum;
-        {
-          uint32_t sa[32], sb[32];
+        if (!early) {
           tc::ld32(tsh, sa);
           tc::ld32(tsh + 32u, sb);
-          tc::wait_ld32(sa);
-          tc::wait_ld32(sb);
-          sum = weigh<masked>(sa, m, c, at, seen, p);
-          sum += weigh<masked>(sb, m, c, at + 32, seen, p + 16);
         }
+        tc::wait_ld32(sa);
+        tc::wait_ld32(sb);
+        float sum = weigh<masked>(sa, m, c, at, seen, p);
+        sum += weigh<masked>(sb, m, c, at + 32, seen, p + 16);
         // Weights are taken against the maximum as it stands; only where their
         // sum is past kTcLazySum is it raised, the output so far rescaled, and
         // the scores of the half read and weighed again.
@@ -394,6 +393,14 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
           }
         }
         l += sum;
+        // The next half's scores, if they are there: read while this half's weights are stored.
+        const int nj = j + h, nh = h ^ 1;
+        early = nj < steps && __all_sync(0xffffffffu, ptx::mbar_test_wait(bar(&sh.sfull[grp][nh]), (uint32_t)(nj & 1)));
+        if (early) {
+          tc::fence_after();
+          tc::ld32(ts + 64u * nh, sa);
+          tc::ld32(ts + 64u * nh + 32u, sb);
+        }
         tc::st32(tsh, p);
         tc::wait_st();
         tc::fence_before();
@@ -401,7 +408,7 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
       const bool masked = __any_sync(0xffffffffu, t + kTcStep > seen);
 #pragma unroll 1
       for (int h = 0; h < 2; ++h) {
-        if (!tc_wait_warp(bar(&sh.sfull[grp][h]), (uint32_t)(j & 1), abort_flag)) {
+        if (!early && !tc_wait_warp(bar(&sh.sfull[grp][h]), (uint32_t)(j & 1), abort_flag)) {
           ok = false;
           break;
         }
