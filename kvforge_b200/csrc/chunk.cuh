@@ -61,13 +61,13 @@ __device__ __forceinline__ int chunk_seen(const ChunkArgs &a, const ChunkWork &w
 // are taken from its end, where a causal tile sees most. A tile's tokens are
 // shared evenly among `splits` blocks in whole steps of `step` tokens.
 __device__ __forceinline__ bool chunk_work(const ChunkArgs &a, int splits, int height, int step, ChunkWork &w) {
-  long long i = blockIdx.x;
-  w.split = (int)(i % splits);
-  i /= splits;
-  w.h = (int)(i % a.cache.Hkv);
-  i /= a.cache.Hkv;
-  w.b = (int)(i % a.B);
-  const int tile = a.tiles - 1 - (int)(i / a.B);
+  unsigned i = blockIdx.x;
+  w.split = (int)(i % (unsigned)splits);
+  i /= (unsigned)splits;
+  w.h = (int)(i % (unsigned)a.cache.Hkv);
+  i /= (unsigned)a.cache.Hkv;
+  w.b = (int)(i % (unsigned)a.B);
+  const int tile = a.tiles - 1 - (int)(i / (unsigned)a.B);
   w.ql = a.q_lens ? min(max(a.q_lens[w.b], 0), a.T) : a.T;
   w.kv = a.seq_lens ? min(max(a.seq_lens[w.b], 0), a.cache.n) : a.cache.n;
   w.row0 = tile * height;

@@ -38,6 +38,7 @@
 
 #include <cuda.h>
 
+#include <cstddef>
 #include <type_traits>
 
 namespace kvfb {
@@ -88,14 +89,35 @@ template <int FMT, int D, bool TWO> struct TcLayout {
 };
 
 struct TcShared {
-  uint64_t kfull[4], kempty[4], vfull[4], vempty[4];
-  uint64_t sfull[2][2], pready[2][2], ofull[2][2];  // per group and half step
-  uint64_t vraw[4], vfixed[4], done;  // vraw, vfixed: f16 V tiles on their way through group 2
-  uint64_t rfull[2][8], rempty[2][8];
+  // Barriers, in the order of tc_bar_count.
+  uint64_t kfull[4], vfull[4];                        // a tile is there
+  uint64_t kempty[4], vempty[4];                      // its slot is free
+  uint64_t sfull[2][2], pready[2][2], ofull[2][2];    // per group and half step: scores, weights, output
+  uint64_t vraw[4], vfixed[4];                        // f16 V tiles on their way through group 2
+  uint64_t qready, done;
+  uint64_t rfull[2][8], rempty[2][8];                 // raw half steps of K, of V
+  uint8_t qexp[2 * kTcRows];                          // 14 + exponent (biased) of the power of two a row was divided by
   uint32_t tmem;
   int abort_flag;
   int odd;            // a masked V tile held an infinity or NaN, taken as 0
 };
+constexpr int kTcBars = 16 + 12 + 8 + 2 + 32;
+static_assert(offsetof(TcShared, qexp) == 8 * kTcBars, "barriers");
+
+// Arrivals that complete a phase of barrier i of TcShared.
+template <bool RAW, bool TWO> __device__ __forceinline__ uint32_t tc_bar_count(int i) {
+  return i < 8    ? (RAW ? 4u : 1u)   // kfull, vfull: four converter warps, or TMA
+         : i < 16 ? (TWO ? 2u : 1u)   // kempty, vempty: each issuer that uses the tile
+         : i < 20 ? 1u                // sfull
+         : i < 24 ? 4u                // pready: a group's warps
+         : i < 28 ? 1u                // ofull
+         : i < 32 ? 1u                // vraw
+         : i < 36 ? 4u                // vfixed
+         : i < 37 ? (TWO ? 8u : 4u)   // qready: the warps that load queries
+         : i < 38 ? 2u                // done: both issuers
+         : i < 54 ? 33u               // rfull: the boxes' bytes, and 32 lanes of cp.async
+                  : 4u;               // rempty: converter warps
+}
 static_assert(sizeof(TcShared) <= 1024, "misc area");
 
 template <int N> __device__ __forceinline__ void regs_up() {
@@ -240,85 +262,84 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
   // in, and the rows that do see them get them at the end.
   const int first_masked = w.seen0 > w.t0 ? (w.seen0 - w.t0) / kTcStep : 0;
 
+  if (tid < kTcBars) ptx::mbar_init(bar(&sh.kfull[0]) + 8u * tid, tc_bar_count<L::RAW, TWO>(tid));
   if (tid == 0) {
     sh.abort_flag = 0;
     sh.odd = 0;
-    for (int s = 0; s < SLOTS; ++s) {
-      // filled by four converter warps, or by TMA
-      ptx::mbar_init(bar(&sh.kfull[s]), L::RAW ? 4u : 1u);
-      ptx::mbar_init(bar(&sh.vfull[s]), L::RAW ? 4u : 1u);
-      ptx::mbar_init(bar(&sh.kempty[s]), TWO ? 2u : 1u);  // by each issuer that uses the tile
-      ptx::mbar_init(bar(&sh.vempty[s]), TWO ? 2u : 1u);
-      ptx::mbar_init(bar(&sh.vraw[s]), 1u);
-      ptx::mbar_init(bar(&sh.vfixed[s]), 4u);
-    }
-    for (int g = 0; g < 2; ++g) {
-      for (int h = 0; h < 2; ++h) {
-        ptx::mbar_init(bar(&sh.sfull[g][h]), 1u);
-        ptx::mbar_init(bar(&sh.pready[g][h]), 4u);
-        ptx::mbar_init(bar(&sh.ofull[g][h]), 1u);
-      }
-      for (int s = 0; s < RSLOTS; ++s) {
-        ptx::mbar_init(bar(&sh.rfull[g][s]), 33u);  // the boxes' bytes, and 32 lanes of cp.async
-        ptx::mbar_init(bar(&sh.rempty[g][s]), 4u);
-      }
-    }
-    ptx::mbar_init(bar(&sh.done), 2u);
-    ptx::fence_barrier_init();
   }
+  ptx::fence_barrier_init();
   if (warp == LAST) {
     tc::alloc(ptx::smem_u32(&sh.tmem), 512u);
     tc::relinquish();
-  }
-
-  // Query rows, scaled, into their tile: thread = row.
-  const int grp = warp >> 2;              // softmax group (warps 0-7)
-  const int r = tid & 127;                // row of the tile
-  float c = a.scale_log2;                 // softmax scale of the row, log2 units
-  const int row = (TWO ? grp * kTcRows : 0) + r;
-  if (warp < 8) {
-    float mx = 0.f;
-    uint32_t e = 127u << 23;
-    const bool live = row < w.rows;
-    const uint8_t *src = a.q.p + (live ? chunk_row(a.q, a, w, row) : 0);
-    if (DT == KVF_DT_BF16 && live) {
-      for (int i = 0; i < D / 8; ++i) {
-        float x[8];
-        load8<DT>(src + 16 * i, a.q.vec, x);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) mx = fmaxf(mx, fabsf(x[k]));
-      }
-      // 2^(14 - exponent of mx), within what fp32 holds; 1 for zero, infinities and NaN
-      if (mx > 0.f && mx < INFINITY) {
-        const int ex = min(max((int)(__float_as_uint(mx) >> 23), 27), 240);
-        e = (uint32_t)(127 + 14 + 127 - ex) << 23;
-        c *= __uint_as_float((uint32_t)(ex - 14) << 23);
-      }
-    }
-    if (TWO || grp == 0) {
-      const float f = __uint_as_float(e);
-      for (int i = 0; i < D / 8; ++i) {
-        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (live) load8<DT>(src + 16 * i, a.q.vec, x);
-        uint32_t p[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) p[k] = narrow2<KVF_DT_F16>(x[2 * k] * f, x[2 * k + 1] * f);
-        const uint32_t ad = sq + (TWO ? grp * TILE : 0u) + (i >> 3) * BLK + r * 128u + ((uint32_t)((i ^ r) & 7) << 4);
-        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(ad), "r"(p[0]), "r"(p[1]), "r"(p[2]), "r"(p[3])
-                     : "memory");
-      }
-    }
-    ptx::fence_proxy_async_smem();
   }
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
   const uint32_t tbase = sh.tmem;
+  const int grp = warp >> 2;              // softmax group (warps 0-7)
   // Each group executes one setmaxnreg, all four warps the same one.
   if (warp < 8) {
     // ------------------------------------------------------------- softmax
     regs_up<L::SOFT_REGS>();
+    const int row = (TWO ? grp * kTcRows : 0) + (tid & 127);
     const bool live = row < w.rows;
+
+    // Query rows, scaled, into their tile: a warp takes its own 32 rows, each by
+    // D / 8 lanes, all loads in flight at once. A bf16 row is scaled by 2^(14 -
+    // exponent of its largest magnitude), within what fp32 holds; by 1 if that
+    // is zero, infinite or NaN.
+    if (TWO || grp == 0) {
+      constexpr int LPR = D / 8, RPW = 32 / LPR, N = 32 / RPW;
+      const int li = lane % LPR, r0 = 32 * (warp & 3) + lane / LPR;
+      uint4 raw[N];
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const int rt = r0 + k * RPW, rr = (TWO ? grp * kTcRows : 0) + rt;
+        raw[k] = make_uint4(0u, 0u, 0u, 0u);
+        if (rr < w.rows) {
+          const uint8_t *src = a.q.p + chunk_row(a.q, a, w, rr) + 16 * li;
+          if (a.q.vec) {
+            raw[k] = __ldg(reinterpret_cast<const uint4 *>(src));
+          } else {
+            const uint16_t *e = reinterpret_cast<const uint16_t *>(src);
+            raw[k] = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16,
+                                e[6] | (uint32_t)e[7] << 16);
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const int rt = r0 + k * RPW;
+        uint32_t x[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+        int ex = 127 + 14;
+        if (DT == KVF_DT_BF16) {
+          // magnitudes order as integers; bf16 bits and fp32's upper half are the same
+          uint32_t mx = 0u;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) mx = max(mx, max(x[q] & 0x7fffu, (x[q] >> 16) & 0x7fffu));
+#pragma unroll
+          for (int off = 1; off < LPR; off <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+          float f = 1.f;
+          if (mx > 0u && mx < 0x7f80u) {
+            ex = min(max((int)(mx >> 7), 27), 240);
+            f = __uint_as_float((uint32_t)(127 + 14 + 127 - ex) << 23);
+          }
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float2 e = widen2<KVF_DT_BF16>(x[q]);
+            x[q] = narrow2<KVF_DT_F16>(e.x * f, e.y * f);
+          }
+        }
+        const uint32_t ad = sq + (TWO ? grp * TILE : 0u) + (li >> 3) * BLK + rt * 128u + ((uint32_t)((li ^ rt) & 7) << 4);
+        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(ad), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+        if (li == 0) sh.qexp[(TWO ? grp * kTcRows : 0) + rt] = (uint8_t)ex;
+      }
+      ptx::fence_proxy_async_smem();
+      __syncwarp();
+      ptx::mbar_arrive_if(bar(&sh.qready), lane == 0);
+    }
+    bool ok = tc_wait_warp(bar(&sh.qready), 0u, abort_flag);  // without TWO group 1 has group 0's rows
+    const float c = a.scale_log2 * __uint_as_float((uint32_t)(sh.qexp[row] - 14) << 23);  // softmax scale of the row
     // a lane without a row goes along (its query is zero); a warp without one only signs off
     const int seen = live ? chunk_seen(a, w, w.row0 + row) : 0x7fffffff;
     const bool idle = __all_sync(0xffffffffu, !live);
@@ -326,9 +347,9 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
     const uint32_t ts = tbase + lanes + S_COL + 128u * grp, to = tbase + lanes + O_COL + (uint32_t)(D * grp);
     const int steps = nw[grp];
     float m = -INFINITY, l = 0.f;
-    bool ok = true, early = false;
+    bool early = false;
     uint32_t sa[32], sb[32];                // scores of the half at hand, or (early) of the next
-    for (int j = 0; j < steps; ++j) {
+    for (int j = 0; j < steps && ok; ++j) {
       const int t = w.t0 + (TWO ? j : 2 * j + grp) * kTcStep;
       // Half a step at a time (64 tokens), each half with scores, weights and
       // barriers of its own: while one half is weighed, the tensor cores take the
@@ -443,7 +464,10 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
       else if (a.lse)
         a.lse[at] = none ? -INFINITY : m + log2f(l);
     }
-    uint8_t *out = a.out.p + (live ? chunk_row(a.out, a, w, row) : 0);
+    // 32 columns at a time through the warp's part of the query tile, which no MMA
+    // reads any more (without TWO group 1 uses its K tile): threads have rows, stores
+    // take whole rows.
+    const uint32_t stage = (TWO || grp == 0 ? sq + (TWO ? grp * TILE : 0u) : skr + TILE) + (uint32_t)(warp & 3) * 4096u;
 #pragma unroll 1
     for (int q = 0; q < D / 32; ++q) {
       uint32_t o[32];
@@ -476,20 +500,58 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
           }
         }
       }
-      if (!live) continue;
+      __syncwarp();
       if (a.splits > 1) {
-        float4 *po = reinterpret_cast<float4 *>(a.part_o + part * D + 32 * q);
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          po[k] = make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]), __uint_as_float(o[4 * k + 2]),
-                              __uint_as_float(o[4 * k + 3]));
+          asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(stage + lane * 128u + ((uint32_t)((k ^ lane) & 7) << 4)),
+                       "r"(o[4 * k]), "r"(o[4 * k + 1]), "r"(o[4 * k + 2]), "r"(o[4 * k + 3])
+                       : "memory");
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int rw = 4 * k + (lane >> 3), rr = row - lane + rw;  // eight lanes a row
+          uint32_t x[4];
+          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                       : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+                       : "r"(stage + rw * 128u + ((uint32_t)((lane ^ rw) & 7) << 4)));
+          if (rr < w.rows) {
+            const long long pr = chunk_index(a, w, rr) * a.splits + (TWO ? w.split : 2 * w.split + grp);
+            *reinterpret_cast<uint4 *>(a.part_o + pr * D + 32 * q + 4 * (lane & 7)) = make_uint4(x[0], x[1], x[2], x[3]);
+          }
+        }
       } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          float x[8];
+          uint32_t x[4];
 #pragma unroll
-          for (int u = 0; u < 8; ++u) x[u] = __uint_as_float(o[8 * k + u]) * inv;
-          store8<DT>(out + (32 * q + 8 * k) * 2, a.out.vec, x);
+          for (int u = 0; u < 4; ++u)
+            x[u] = narrow2<DT>(__uint_as_float(o[8 * k + 2 * u]) * inv, __uint_as_float(o[8 * k + 2 * u + 1]) * inv);
+          asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(stage + lane * 64u + ((uint32_t)((k ^ (lane >> 1)) & 3) << 4)),
+                       "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3])
+                       : "memory");
+        }
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int rw = 8 * k + (lane >> 2), rr = row - lane + rw;  // four lanes a row
+          uint32_t x[4];
+          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                       : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+                       : "r"(stage + rw * 64u + ((uint32_t)((lane ^ (rw >> 1)) & 3) << 4)));
+          if (rr < w.rows) {
+            uint8_t *out = a.out.p + chunk_row(a.out, a, w, rr) + 64 * q + 16 * (lane & 3);
+            if (a.out.vec) {
+              *reinterpret_cast<uint4 *>(out) = make_uint4(x[0], x[1], x[2], x[3]);
+            } else {
+              uint16_t *e = reinterpret_cast<uint16_t *>(out);
+#pragma unroll
+              for (int u = 0; u < 4; ++u) {
+                e[2 * u] = (uint16_t)x[u];
+                e[2 * u + 1] = (uint16_t)(x[u] >> 16);
+              }
+            }
+          }
         }
       }
     }
@@ -771,7 +833,8 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
       // every second.
       constexpr int STRIDE = TWO ? 1 : 2;
       int i = TWO ? 0 : g;
-      if (i < n && take_k(i)) {
+      ok = tc_wait_warp(bar(&sh.qready), 0u, abort_flag);
+      if (ok && i < n && take_k(i)) {
         if (nw[g] > 0)
           for (int h = 0; h < 2; ++h) scores(i, h);
         release(&sh.kempty[i % SLOTS]);
