@@ -428,8 +428,9 @@ cudaError_t kvf_b200_gather(const kvf_args *a, int fmt, int d, int ord, int page
  * (causal = 1), or all kv (causal = 0: cross attention, or a chunk that sees
  * itself whole). A row that sees nothing gets zeros. What lies in the cache
  * at tokens a row does not see has no effect on it, infinities and NaN included.
- * q and out have H heads and one type, any multiple of Hkv query heads, and
- * may not overlap. Read from `a`: the cache, H, seq_lens, scale_log2, lse
+ * q and out have H heads and one type, any multiple of Hkv query heads (at
+ * most 32768 times), and may not overlap; their strides between tokens and
+ * heads are at most 2^29 - 1 elements. Read from `a`: the cache, H, seq_lens, scale_log2, lse
  * ([B][T][H], optional: log2 of each row's softmax denominator, -inf where it
  * sees nothing), splits, and for splits > 1 the workspace part_o
  * [B][T][H][splits][d] (16-byte aligned) and part_ml [B][T][H][splits][2].

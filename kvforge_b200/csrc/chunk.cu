@@ -6,6 +6,7 @@
 #include "chunk_tc.cuh"
 
 #include <algorithm>
+#include <cstdlib>
 
 namespace kvfb {
 
@@ -49,7 +50,7 @@ __global__ void __launch_bounds__(128) chunk_merge(const ChunkArgs a) {
   const float inv = none ? 0.f : 1.f / l;
   if (a.lse && lane == 0) a.lse[at] = none ? -INFINITY : m + log2f(l);
   using E = Elem<DT>;
-  typename E::T *out = reinterpret_cast<typename E::T *>(a.out.p + b * a.out.sb + j * a.out.st + h * a.out.sh);
+  typename E::T *out = reinterpret_cast<typename E::T *>(a.out.p + b * a.out.sb + (long long)j * a.out.st + (long long)h * a.out.sh);
 #pragma unroll
   for (int k = 0; k < D / 32; ++k) out[lane + 32 * k] = E::from(acc[k] * inv);
 }
@@ -103,7 +104,7 @@ cudaError_t launch(void *fn, long long blocks, int threads, uint32_t smem, const
 
 ChunkRows chunk_rows(const kvf_heads &r) {
   const long long e = dtype_bytes(r.dtype);
-  return ChunkRows{reinterpret_cast<uint8_t *>(r.p), r.stride_b * e, r.stride_t * e, r.stride_h * e,
+  return ChunkRows{reinterpret_cast<uint8_t *>(r.p), r.stride_b * e, (int)(r.stride_t * e), (int)(r.stride_h * e),
                    rows_aligned(r) ? 1 : 0};
 }
 
@@ -180,12 +181,16 @@ extern "C" cudaError_t kvf_b200_chunk_attention(const kvf_args *args, int fmt, i
   if (args->splits > 1 && ((reinterpret_cast<uintptr_t>(args->part_o) & 15u) ||
                            (reinterpret_cast<uintptr_t>(args->part_ml) & 7u)))
     return cudaErrorMisalignedAddress;
+  for (const kvf_heads *x : {q, out})
+    if (std::llabs(x->stride_t) > 0x1fffffffLL || std::llabs(x->stride_h) > 0x1fffffffLL) return cudaErrorInvalidValue;
   a.q = chunk_rows(*q);
   a.out = chunk_rows(*out);
   a.B = args->B;
   a.T = T;
   a.H = args->H;
   a.g = args->H / args->Hkv;
+  if (a.g > 32768) return cudaErrorInvalidValue;
+  a.gmul = ((1ull << 32) + a.g - 1) / a.g;
   a.k = args->k;
   a.v = args->v;
   a.km = reinterpret_cast<const uint32_t *>(args->k_meta);

@@ -22,13 +22,15 @@ namespace {
 
 struct ChunkRows {
   uint8_t *p;
-  long long sb, st, sh;  // strides in bytes
+  long long sb;          // strides in bytes
+  int st, sh;
   int vec;               // rows start on 16-byte boundaries
 };
 
 struct ChunkArgs {
   ChunkRows q, out;
   int B, T, H, g;
+  unsigned long long gmul;  // ceil(2^32 / g): x / g = x * gmul >> 32 for x < 2^16, g < 2^16
   CacheRows cache;       // Hkv, n
   const uint8_t *k, *v;
   const uint32_t *km, *vm;
@@ -49,12 +51,22 @@ struct ChunkWork {
   int ql, kv, split;
   int t0, t1;
   int seen0;             // tokens that row0 sees
+  int j0, g0;            // token and query head (within the group) of row0
 };
 
-__device__ __forceinline__ int chunk_seen(const ChunkArgs &a, const ChunkWork &w, int row) {
+// Token (from w.j0 on) and query head of row r of the tile.
+__device__ __forceinline__ void chunk_at(const ChunkArgs &a, const ChunkWork &w, int r, int &j, int &head) {
+  const unsigned x = (unsigned)(w.g0 + r);
+  j = (int)(x * a.gmul >> 32);
+  head = (int)x - j * a.g;
+}
+
+// Tokens that row r of the tile sees.
+__device__ __forceinline__ int chunk_seen(const ChunkArgs &a, const ChunkWork &w, int r) {
   if (!a.causal) return w.kv;
-  const int s = w.kv - w.ql + row / a.g + 1;
-  return s < 0 ? 0 : s;
+  int j, head;
+  chunk_at(a, w, r, j, head);
+  return max(0, w.kv - w.ql + w.j0 + j + 1);
 }
 
 // False if the block has no rows. Longest rows first: the tiles of a sequence
@@ -73,25 +85,30 @@ __device__ __forceinline__ bool chunk_work(const ChunkArgs &a, int splits, int h
   w.row0 = tile * height;
   w.rows = min(height, w.ql * a.g - w.row0);
   if (w.rows <= 0) return false;
-  const int seen = chunk_seen(a, w, w.row0 + w.rows - 1);
+  w.j0 = w.row0 / a.g;
+  w.g0 = w.row0 - w.j0 * a.g;
+  const int seen = chunk_seen(a, w, w.rows - 1);
   const int steps = (seen + step - 1) / step;
   const int each = (steps + splits - 1) / splits;
   w.t0 = (int)min((long long)w.split * each * step, (long long)seen);
   w.t1 = (int)min((long long)w.t0 + (long long)each * step, (long long)seen);
-  w.seen0 = chunk_seen(a, w, w.row0);
+  w.seen0 = chunk_seen(a, w, 0);
   return true;
 }
 
-// Byte offset of row r of the tile in q or out.
-__device__ __forceinline__ long long chunk_row(const ChunkRows &x, const ChunkArgs &a, const ChunkWork &w, int r) {
-  const int row = w.row0 + r, j = row / a.g;
-  return w.b * x.sb + j * x.st + (long long)(w.h * a.g + row - j * a.g) * x.sh;
+// Row r of the tile in q or out. Strides between tokens and heads fit 32 bits.
+__device__ __forceinline__ uint8_t *chunk_row(const ChunkRows &x, const ChunkArgs &a, const ChunkWork &w, int r) {
+  int j, head;
+  chunk_at(a, w, r, j, head);
+  uint8_t *base = x.p + w.b * x.sb + (long long)w.j0 * x.st + (long long)(w.h * a.g) * x.sh;
+  return base + (long long)j * x.st + (long long)head * x.sh;
 }
 
 // Index of row r in lse and in the split partials.
 __device__ __forceinline__ long long chunk_index(const ChunkArgs &a, const ChunkWork &w, int r) {
-  const int row = w.row0 + r, j = row / a.g;
-  return ((long long)w.b * a.T + j) * a.H + w.h * a.g + (row - j * a.g);
+  int j, head;
+  chunk_at(a, w, r, j, head);
+  return ((long long)w.b * a.T + w.j0) * a.H + w.h * a.g + (long long)j * a.H + head;
 }
 
 // Eight channels of cache row `row` (from channel 8 * li) as fp32.

@@ -63,14 +63,14 @@ __global__ void __launch_bounds__(kChunkThreads) chunk_mma_kernel(const ChunkArg
   for (int i = tid; i < kChunkRows * (D / 8); i += kChunkThreads) {
     const int r = i / (D / 8), li = i % (D / 8);
     float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (r < w.rows) load8<DT>(a.q.p + chunk_row(a.q, a, w, r) + 8 * li * dtype_bytes(DT), a.q.vec, x);
+    if (r < w.rows) load8<DT>(chunk_row(a.q, a, w, r) + 8 * li * dtype_bytes(DT), a.q.vec, x);
 #pragma unroll
     for (int k = 0; k < 8; ++k) sq[r * QS + 8 * li + k] = x[k];
   }
 
   const int r_lo = warp * 16 + g4, r_hi = r_lo + 8;
-  const int seen_lo = r_lo < w.rows ? chunk_seen(a, w, w.row0 + r_lo) : 0;
-  const int seen_hi = r_hi < w.rows ? chunk_seen(a, w, w.row0 + r_hi) : 0;
+  const int seen_lo = r_lo < w.rows ? chunk_seen(a, w, r_lo) : 0;
+  const int seen_hi = r_hi < w.rows ? chunk_seen(a, w, r_hi) : 0;
   float m_lo = -INFINITY, m_hi = -INFINITY, l_lo = 0.f, l_hi = 0.f;
   float o[D / 8][4];
 #pragma unroll
@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(kChunkThreads) chunk_mma_kernel(const ChunkArg
     const float inv = m == -INFINITY ? 0.f : 1.f / l;
     if (a.lse && t4 == 0) a.lse[at] = m == -INFINITY ? -INFINITY : m + log2f(l);
     using E = Elem<DT>;
-    typename E::T *out = reinterpret_cast<typename E::T *>(a.out.p + chunk_row(a.out, a, w, r));
+    typename E::T *out = reinterpret_cast<typename E::T *>(chunk_row(a.out, a, w, r));
 #pragma unroll
     for (int n = 0; n < D / 8; ++n) {
       out[8 * n + 2 * t4] = E::from(o[n][2 * half] * inv);

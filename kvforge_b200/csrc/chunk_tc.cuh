@@ -250,7 +250,7 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
   for (int g = 0; g < 2; ++g) {
     if (TWO) {
       const int rows = min(w.rows - g * kTcRows, kTcRows);
-      const int seen = rows > 0 ? chunk_seen(a, w, w.row0 + g * kTcRows + rows - 1) : 0;
+      const int seen = rows > 0 ? chunk_seen(a, w, g * kTcRows + rows - 1) : 0;
       nw[g] = seen > w.t0 ? min(n, (seen - w.t0 + kTcStep - 1) / kTcStep) : 0;
     } else {
       nw[g] = (n + 1 - g) / 2;
@@ -297,7 +297,7 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
         const int rt = r0 + k * RPW, rr = (TWO ? grp * kTcRows : 0) + rt;
         raw[k] = make_uint4(0u, 0u, 0u, 0u);
         if (rr < w.rows) {
-          const uint8_t *src = a.q.p + chunk_row(a.q, a, w, rr) + 16 * li;
+          const uint8_t *src = chunk_row(a.q, a, w, rr) + 16 * li;
           if (a.q.vec) {
             raw[k] = __ldg(reinterpret_cast<const uint4 *>(src));
           } else {
@@ -341,7 +341,7 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
     bool ok = tc_wait_warp(bar(&sh.qready), 0u, abort_flag);  // without TWO group 1 has group 0's rows
     const float c = a.scale_log2 * __uint_as_float((uint32_t)(sh.qexp[row] - 14) << 23);  // softmax scale of the row
     // a lane without a row goes along (its query is zero); a warp without one only signs off
-    const int seen = live ? chunk_seen(a, w, w.row0 + row) : 0x7fffffff;
+    const int seen = live ? chunk_seen(a, w, row) : 0x7fffffff;
     const bool idle = __all_sync(0xffffffffu, !live);
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
     const uint32_t ts = tbase + lanes + S_COL + 128u * grp, to = tbase + lanes + O_COL + (uint32_t)(D * grp);
@@ -540,7 +540,7 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
                        : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
                        : "r"(stage + rw * 64u + ((uint32_t)((lane ^ (rw >> 1)) & 3) << 4)));
           if (rr < w.rows) {
-            uint8_t *out = a.out.p + chunk_row(a.out, a, w, rr) + 64 * q + 16 * (lane & 3);
+            uint8_t *out = chunk_row(a.out, a, w, rr) + 64 * q + 16 * (lane & 3);
             if (a.out.vec) {
               *reinterpret_cast<uint4 *>(out) = make_uint4(x[0], x[1], x[2], x[3]);
             } else {
