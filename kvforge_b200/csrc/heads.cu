@@ -44,7 +44,8 @@ struct HeadsArgs {
   const float *cos, *sin;
   int rot, positions, interleaved;
   const int *pos, *lens;
-  int B, T, units;       // units: warps per token
+  int B, T;
+  int q_units, k_units, units;  // warps per token: of its query heads, of its keys and of its values
   CacheRows cache;
   uint8_t *kd, *vd;
   void *km, *vm;
@@ -52,153 +53,178 @@ struct HeadsArgs {
 };
 
 __device__ __forceinline__ void load_weight8(const Norm &n, int li, float (&w)[8]) {
-#pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const int c = 8 * li + k;
-    w[k] = n.dtype == KVF_DT_F32   ? __ldg(reinterpret_cast<const float *>(n.w) + c)
-           : n.dtype == KVF_DT_F16 ? __half2float(__ldg(reinterpret_cast<const __half *>(n.w) + c))
-                                   : __bfloat162float(__ldg(reinterpret_cast<const __nv_bfloat16 *>(n.w) + c));
-  }
+  const bool vec = (reinterpret_cast<uintptr_t>(n.w) & 15u) == 0;
+  const uint8_t *p = reinterpret_cast<const uint8_t *>(n.w) + 8 * li * dtype_bytes(n.dtype);
+  if (n.dtype == KVF_DT_F32)
+    load8<KVF_DT_F32>(p, vec, w);
+  else if (n.dtype == KVF_DT_F16)
+    load8<KVF_DT_F16>(p, vec, w);
+  else
+    load8<KVF_DT_BF16>(p, vec, w);
 }
 
-// One warp takes R * (32 / (D / 8)) head vectors of one token, R per group of
-// D / 8 lanes, so the token's angles are read once for R heads and R rows are
-// in flight per lane. Rows are numbered query heads, then KV heads of k, then of v.
-template <int DT, int D, int R>
+// One warp takes up to R * (32 / (D / 8)) head vectors of one token and of one
+// kind (queries, keys or values), R per group of D / 8 lanes: its weight and the
+// token's angles are read once for R rows, R loads are in flight per lane, and
+// the R roots are taken by R lanes at once. CACHE: keys and values are part of
+// the call.
+template <int DT, int D, int R, bool CACHE>
 __global__ void __launch_bounds__(256) heads_kernel(const HeadsArgs a) {
   constexpr int LPR = D / 8;     // lanes per row
   constexpr int RPW = 32 / LPR;  // rows per warp at a time
   const int lane = threadIdx.x & 31;
   const int li = lane % LPR;
-  const long long wid = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-  const long long token = wid / a.units;
-  if (token >= (long long)a.B * a.T) return;
-  const int b = (int)(token / a.T), j = (int)(token - (long long)b * a.T);
+  const unsigned wid = blockIdx.x * 8u + (threadIdx.x >> 5);
+  const unsigned token = wid / (unsigned)a.units;
+  const unsigned bu = token / (unsigned)a.T;
+  if (bu >= (unsigned)a.B) return;
+  const int b = (int)bu, j = (int)(token - bu * (unsigned)a.T);
   if (a.lens && j >= a.lens[b]) return;
-  const int r0 = (int)(wid - token * a.units) * (R * RPW) + lane / LPR;
-  const int rows = a.q.heads + a.k.heads + a.v.heads;
+  int unit = (int)(wid - token * (unsigned)a.units), kind = 0;
+  if (CACHE && unit >= a.q_units) {
+    unit -= a.q_units;
+    kind = 1;
+    if (unit >= a.k_units) {
+      unit -= a.k_units;
+      kind = 2;
+    }
+  }
+  const Rows &src = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
+  const int r0 = unit * (R * RPW) + lane / LPR;
   const long long t = a.pos ? (long long)a.pos[b] + j : j;
   const bool bad_pos = t < 0 || (a.rot && t >= a.positions);
 
   float e[R][8];
+  const uint8_t *in = src.p + b * src.sb + j * src.st + 8 * li * dtype_bytes(DT);
 #pragma unroll
   for (int i = 0; i < R; ++i) {
-    int r = r0 + i * RPW;
-    const Rows *src = &a.q;
-    if (r >= a.q.heads) {
-      r -= a.q.heads;
-      src = &a.k;
-      if (r >= a.k.heads) {
-        r -= a.k.heads;
-        src = &a.v;
-      }
-    }
-    if (r0 + i * RPW < rows) {
-      load8<DT>(src->p + b * src->sb + j * src->st + r * src->sh + 8 * li * dtype_bytes(DT), src->vec, e[i]);
+    const int r = r0 + i * RPW;
+    if (r < src.heads) {
+      load8<DT>(in + r * src.sh, src.vec, e[i]);
     } else {
 #pragma unroll
       for (int k = 0; k < 8; ++k) e[i][k] = 0.f;
     }
   }
 
-  // Angles of this lane's channels. Half-split pairs: channel c < rot/2 turns
-  // with c + rot/2, rot/16 lanes further; both halves use angle c mod rot/2.
+  const bool turning = kind < 2 && a.rot && !bad_pos;  // the same for the whole warp
   float cs[8], sn[8];
-  const bool turns = a.rot && !bad_pos && 8 * li < a.rot;
   const int half = a.rot >> 1;
+  const bool turns = turning && 8 * li < a.rot, low = 8 * li < half;
   if (turns) {
+    // Angles of this lane's channels. Half-split pairs: channel c < rot/2 turns
+    // with c + rot/2, rot/16 lanes further; both halves use angle c mod rot/2, and
+    // the lower one the sine's negative.
     const float *c = a.cos + t * half, *s = a.sin + t * half;
     if (a.interleaved) {
       const float4 c4 = *reinterpret_cast<const float4 *>(c + 4 * li), s4 = *reinterpret_cast<const float4 *>(s + 4 * li);
       cs[0] = c4.x; cs[1] = c4.y; cs[2] = c4.z; cs[3] = c4.w;
       sn[0] = s4.x; sn[1] = s4.y; sn[2] = s4.z; sn[3] = s4.w;
     } else {
-      const int at = 8 * li < half ? 8 * li : 8 * li - half;
-      load8<KVF_DT_F32>(c + at, true, cs);
-      load8<KVF_DT_F32>(s + at, true, sn);
+      const int at = low ? 8 * li : 8 * li - half;
+#pragma unroll
+      for (int k = 0; k < 8; k += 4) {
+        const float4 c4 = *reinterpret_cast<const float4 *>(c + at + k), s4 = *reinterpret_cast<const float4 *>(s + at + k);
+        cs[k] = c4.x; cs[k + 1] = c4.y; cs[k + 2] = c4.z; cs[k + 3] = c4.w;
+        sn[k] = s4.x; sn[k + 1] = s4.y; sn[k + 2] = s4.z; sn[k + 3] = s4.w;
+      }
+      if (low)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sn[k] = -sn[k];
     }
   }
-  const bool low = 8 * li < half;
-  const int partner = (lane & ~(LPR - 1)) + (turns ? (low ? li + (a.rot >> 4) : li - (a.rot >> 4)) : li);
 
+  const Norm &nm = kind == 0 ? a.qn : a.kn;
+  if (kind < 2 && nm.w) {
+    float sum[R], inv[R];
 #pragma unroll
-  for (int i = 0; i < R; ++i) {
-    const int row = r0 + i * RPW;
-    const int cls = row < a.q.heads ? 0 : row < a.q.heads + a.k.heads ? 1 : 2;
-    if (__all_sync(0xffffffffu, row >= rows)) break;
-    float x[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) x[k] = e[i][k];
-
-    const Norm &nm = cls == 0 ? a.qn : a.kn;
-    const bool normed = cls < 2 && nm.w;
-    if (__any_sync(0xffffffffu, normed)) {
+    for (int i = 0; i < R; ++i) {
       float s[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) s[k] = __fmul_rn(x[k], x[k]);
-      float sum = __fadd_rn(__fadd_rn(__fadd_rn(s[0], s[1]), __fadd_rn(s[2], s[3])),
-                            __fadd_rn(__fadd_rn(s[4], s[5]), __fadd_rn(s[6], s[7])));
+      for (int k = 0; k < 8; ++k) s[k] = __fmul_rn(e[i][k], e[i][k]);
+      sum[i] = __fadd_rn(__fadd_rn(__fadd_rn(s[0], s[1]), __fadd_rn(s[2], s[3])),
+                         __fadd_rn(__fadd_rn(s[4], s[5]), __fadd_rn(s[6], s[7])));
 #pragma unroll
-      for (int off = 1; off < LPR; off <<= 1) sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, off));
-      if (normed) {
-        const float inv = __fdiv_rn(1.f, __fsqrt_rn(__fadd_rn(__fmul_rn(sum, 1.f / D), nm.eps)));
-        float w[8];
-        load_weight8(nm, li, w);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) x[k] = __fmul_rn(__fmul_rn(x[k], inv), w[k]);
-      }
+      for (int off = 1; off < LPR; off <<= 1) sum[i] = __fadd_rn(sum[i], __shfl_xor_sync(0xffffffffu, sum[i], off));
     }
-    if (a.rot) {
-      if (a.interleaved) {
-        if (turns && cls < 2) {
+    float mine = sum[0];
+#pragma unroll
+    for (int i = 1; i < R; ++i) mine = li % R == i ? sum[i] : mine;
+    const float root = __fdiv_rn(1.f, __fsqrt_rn(__fadd_rn(__fmul_rn(mine, 1.f / D), nm.eps)));
+#pragma unroll
+    for (int i = 0; i < R; ++i) inv[i] = R == 1 ? root : __shfl_sync(0xffffffffu, root, (lane & ~(LPR - 1)) + i);
+    float w[8];
+    load_weight8(nm, li, w);
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) e[i][k] = __fmul_rn(__fmul_rn(e[i][k], inv[i]), w[k]);
+  }
+  if (turning) {
+    if (a.interleaved) {
+      if (turns) {
+#pragma unroll
+        for (int i = 0; i < R; ++i)
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const float u = x[2 * k], w = x[2 * k + 1];
-            x[2 * k] = __fsub_rn(__fmul_rn(u, cs[k]), __fmul_rn(w, sn[k]));
-            x[2 * k + 1] = __fadd_rn(__fmul_rn(u, sn[k]), __fmul_rn(w, cs[k]));
+            const float u = e[i][2 * k], w = e[i][2 * k + 1];
+            e[i][2 * k] = __fsub_rn(__fmul_rn(u, cs[k]), __fmul_rn(w, sn[k]));
+            e[i][2 * k + 1] = __fadd_rn(__fmul_rn(u, sn[k]), __fmul_rn(w, cs[k]));
           }
-        }
-      } else {
+      }
+    } else {
+      const int partner = (lane & ~(LPR - 1)) + (turns ? (low ? li + (a.rot >> 4) : li - (a.rot >> 4)) : li);
+#pragma unroll
+      for (int i = 0; i < R; ++i)
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const float o = __shfl_sync(0xffffffffu, x[k], partner);
-          if (turns && cls < 2)
-            x[k] = low ? __fsub_rn(__fmul_rn(x[k], cs[k]), __fmul_rn(o, sn[k]))
-                       : __fadd_rn(__fmul_rn(o, sn[k]), __fmul_rn(x[k], cs[k]));
+          const float o = __shfl_sync(0xffffffffu, e[i][k], partner);
+          if (turns) e[i][k] = __fadd_rn(__fmul_rn(e[i][k], cs[k]), __fmul_rn(o, sn[k]));
         }
-      }
     }
+  }
 
-    const bool live = row < rows;
-    if (live && cls == 0) {
-      if (bad_pos) {
-        if (li == 0) atomicOr(&g_kvfb_heads_error, 1u);
-      } else {
-        store8<DT>(a.q_out.p + b * a.q_out.sb + j * a.q_out.st + row * a.q_out.sh + 8 * li * dtype_bytes(DT),
-                   a.q_out.vec, x);
+  if (!CACHE || kind == 0) {
+    if (bad_pos) {
+      if (lane == 0) atomicOr(&g_kvfb_heads_error, 1u);
+      return;
+    }
+    uint8_t *out = a.q_out.p + b * a.q_out.sb + j * a.q_out.st + 8 * li * dtype_bytes(DT);
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int r = r0 + i * RPW;
+      if (r < a.q.heads) store8<DT>(out + r * a.q_out.sh, a.q_out.vec, e[i]);
+    }
+    return;
+  }
+  if (CACHE) {
+    // Heads of a token lie one row apart (token-major) or a whole sequence or page apart.
+    const long long row0 = bad_pos ? -1 : a.cache.row(b, 0, t);
+    if (row0 < 0) {
+      if (lane == 0) atomicOr(&g_kvfb_heads_error, 1u);
+      return;
+    }
+    const long long hstep = !a.cache.head_major ? 1 : a.cache.paged ? 1ll << a.cache.bt_shift : a.cache.n;
+    uint8_t *data = kind == 1 ? a.kd : a.vd;
+    uint32_t *meta = reinterpret_cast<uint32_t *>(kind == 1 ? a.km : a.vm);
+    const int lpg = a.group >> 3, gshift = __popc(a.group - 1);  // group is a power of two
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int r = r0 + i * RPW;
+      if (__all_sync(0xffffffffu, r >= src.heads)) return;
+      const bool live = r < src.heads;
+      const long long dr = row0 + r * hstep;
+      if (a.fmt == KVF_FMT_F16) {
+        if (live) store8<KVF_DT_F16>(data + (dr * D + 8 * li) * 2, true, e[i]);
+        continue;
       }
-    }
-    if (!__any_sync(0xffffffffu, live && cls > 0)) continue;
-    const int h = cls == 1 ? row - a.q.heads : row - a.q.heads - a.k.heads;
-    long long dr = -1;
-    if (live && cls > 0) {
-      dr = bad_pos ? -1 : a.cache.row(b, h, t);
-      if (dr < 0 && li == 0) atomicOr(&g_kvfb_heads_error, 1u);
-    }
-    uint8_t *data = cls == 1 ? a.kd : a.vd;
-    if (a.fmt == KVF_FMT_F16) {
-      if (dr >= 0) store8<KVF_DT_F16>(data + (dr * D + 8 * li) * 2, true, x);
-      continue;
-    }
-    const GroupScale g = group_scale8(x, li, a.group, a.fmt == KVF_FMT_INT8 ? 255 : 15);
-    if (dr >= 0) {
-      const int lpg = a.group >> 3;
-      if ((li & (lpg - 1)) == 0)
-        reinterpret_cast<uint32_t *>(cls == 1 ? a.km : a.vm)[dr * (D / a.group) + li / lpg] = g.word;
+      const GroupScale g = group_scale8(e[i], li, a.group, a.fmt == KVF_FMT_INT8 ? 255 : 15);
+      if (!live) continue;
+      if ((li & (lpg - 1)) == 0) meta[(dr * D + 8 * li) >> gshift] = g.word;
       if (a.fmt == KVF_FMT_INT8)
-        store_codes8<KVF_FMT_INT8>(x, g, data + dr * D, li);
+        store_codes8<KVF_FMT_INT8>(e[i], g, data + dr * D, li);
       else
-        store_codes8<KVF_FMT_INT4>(x, g, data + dr * (D / 2), li);
+        store_codes8<KVF_FMT_INT4>(e[i], g, data + dr * (D / 2), li);
     }
   }
 }
@@ -206,16 +232,28 @@ __global__ void __launch_bounds__(256) heads_kernel(const HeadsArgs a) {
 template <int DT, int D>
 cudaError_t launch_heads(HeadsArgs a, cudaStream_t st) {
   constexpr int RPW = 32 / (D / 8);
-  const int rows = a.q.heads + a.k.heads + a.v.heads;
   const long long tokens = (long long)a.B * a.T;
-  const int r = tokens * ((rows + RPW - 1) / RPW) >= 4 * 148 * 16 ? 4 : 1;
-  a.units = (rows + r * RPW - 1) / (r * RPW);
-  const long long blocks = (tokens * a.units + 7) / 8;
-  if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
-  if (r == 4)
-    heads_kernel<DT, D, 4><<<(unsigned)blocks, 256, 0, st>>>(a);
-  else
-    heads_kernel<DT, D, 1><<<(unsigned)blocks, 256, 0, st>>>(a);
+  // Four rows per lane group where that still gives every SM some 16 warps; one
+  // in short calls, whose time is that of one row.
+  const long long pairs = (a.q.heads + RPW - 1) / RPW + (a.k.heads + RPW - 1) / RPW + (a.v.heads + RPW - 1) / RPW;
+  const int r = tokens * pairs >= 4 * 148 * 16 ? 4 : 1;
+  a.q_units = (a.q.heads + r * RPW - 1) / (r * RPW);
+  a.k_units = (a.k.heads + r * RPW - 1) / (r * RPW);
+  a.units = a.q_units + a.k_units + (a.v.heads + r * RPW - 1) / (r * RPW);
+  const long long warps = tokens * a.units;
+  if (warps > 0xffffffffLL - 8) return cudaErrorInvalidValue;
+  const unsigned blocks = (unsigned)((warps + 7) / 8);
+  if (a.k.heads == 0) {
+    if (r == 4)
+      heads_kernel<DT, D, 4, false><<<blocks, 256, 0, st>>>(a);
+    else
+      heads_kernel<DT, D, 1, false><<<blocks, 256, 0, st>>>(a);
+  } else {
+    if (r == 4)
+      heads_kernel<DT, D, 4, true><<<blocks, 256, 0, st>>>(a);
+    else
+      heads_kernel<DT, D, 1, true><<<blocks, 256, 0, st>>>(a);
+  }
   return cudaGetLastError();
 }
 
@@ -278,10 +316,11 @@ __global__ void __launch_bounds__(256) gather_kernel(const GatherArgs a) {
   constexpr int RPW = 32 / LPR;
   const int lane = threadIdx.x & 31;
   const int li = lane % LPR;
-  const long long wid = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-  const long long token = wid / a.units;
-  if (token >= (long long)a.B * a.T) return;
-  const int b = (int)(token / a.T), j = (int)(token - (long long)b * a.T);
+  const unsigned wid = blockIdx.x * 8u + (threadIdx.x >> 5);
+  const unsigned token = wid / (unsigned)a.units;
+  const unsigned bu = token / (unsigned)a.T;
+  if (bu >= (unsigned)a.B) return;
+  const int b = (int)bu, j = (int)(token - bu * (unsigned)a.T);
   if (a.lens && j >= a.lens[b]) return;
   const long long t = a.pos ? (long long)a.pos[b] + j : j;
   if (a.seq_lens && t >= a.seq_lens[b]) return;
@@ -293,7 +332,7 @@ __global__ void __launch_bounds__(256) gather_kernel(const GatherArgs a) {
   }
   // Heads of a token lie one row apart (token-major) or a whole sequence or page apart.
   const long long hstep = !a.cache.head_major ? 1 : a.cache.paged ? 1ll << a.cache.bt_shift : a.cache.n;
-  const int r0 = (int)(wid - token * a.units) * (R * RPW) + lane / LPR;
+  const int r0 = (int)(wid - token * (unsigned)a.units) * (R * RPW) + lane / LPR;
   uint4 raw[R];
   uint32_t mw[R];
 #pragma unroll
@@ -350,8 +389,9 @@ template <int FMT, int DT, int D>
 cudaError_t launch_gather(GatherArgs a, cudaStream_t st) {
   constexpr int RPW = 32 / (D / 8), R = 4;
   a.units = (2 * a.k.heads + R * RPW - 1) / (R * RPW);
-  const long long blocks = ((long long)a.B * a.T * a.units + 7) / 8;
-  if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+  const long long warps = (long long)a.B * a.T * a.units;
+  if (warps > 0xffffffffLL - 8) return cudaErrorInvalidValue;
+  const long long blocks = (warps + 7) / 8;
   gather_kernel<FMT, DT, D, R><<<(unsigned)blocks, 256, 0, st>>>(a);
   return cudaGetLastError();
 }
