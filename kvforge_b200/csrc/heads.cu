@@ -69,7 +69,7 @@ __device__ __forceinline__ void load_weight8(const Norm &n, int li, float (&w)[8
 // the R roots are taken by R lanes at once. CACHE: keys and values are part of
 // the call.
 template <int DT, int D, int R, bool CACHE>
-__global__ void __launch_bounds__(256) heads_kernel(const HeadsArgs a) {
+__global__ void __launch_bounds__(256, 4) heads_kernel(const HeadsArgs a) {
   constexpr int LPR = D / 8;     // lanes per row
   constexpr int RPW = 32 / LPR;  // rows per warp at a time
   const int lane = threadIdx.x & 31;
@@ -94,17 +94,14 @@ __global__ void __launch_bounds__(256) heads_kernel(const HeadsArgs a) {
   const long long t = a.pos ? (long long)a.pos[b] + j : j;
   const bool bad_pos = t < 0 || (a.rot && t >= a.positions);
 
-  float e[R][8];
+  // Rows stay as they lie in memory until they are worked on: R of them in
+  // flight take 4 R registers (8 R for fp32).
+  Raw8<DT> raw[R];
   const uint8_t *in = src.p + b * src.sb + j * src.st + 8 * li * dtype_bytes(DT);
 #pragma unroll
   for (int i = 0; i < R; ++i) {
-    const int r = r0 + i * RPW;
-    if (r < src.heads) {
-      load8<DT>(in + r * src.sh, src.vec, e[i]);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) e[i][k] = 0.f;
-    }
+    const int r = min(r0 + i * RPW, src.heads - 1);
+    raw[i] = load_raw8<DT>(in + r * src.sh, src.vec);
   }
 
   const bool turning = kind < 2 && a.rot && !bad_pos;  // the same for the whole warp
@@ -135,97 +132,105 @@ __global__ void __launch_bounds__(256) heads_kernel(const HeadsArgs a) {
   }
 
   const Norm &nm = kind == 0 ? a.qn : a.kn;
-  if (kind < 2 && nm.w) {
-    float sum[R], inv[R];
+  const bool normed = kind < 2 && nm.w;
+  float root = 0.f, w[8];
+  if (normed) {
+    load_weight8(nm, li, w);
+    float mine = 0.f;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       float s[8];
+      values8<DT>(raw[i], s);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) s[k] = __fmul_rn(e[i][k], e[i][k]);
-      sum[i] = __fadd_rn(__fadd_rn(__fadd_rn(s[0], s[1]), __fadd_rn(s[2], s[3])),
-                         __fadd_rn(__fadd_rn(s[4], s[5]), __fadd_rn(s[6], s[7])));
+      for (int k = 0; k < 8; k += 2) mul2(s[k], s[k + 1], s[k], s[k + 1], s[k], s[k + 1]);
+      float sum = __fadd_rn(__fadd_rn(__fadd_rn(s[0], s[1]), __fadd_rn(s[2], s[3])),
+                            __fadd_rn(__fadd_rn(s[4], s[5]), __fadd_rn(s[6], s[7])));
 #pragma unroll
-      for (int off = 1; off < LPR; off <<= 1) sum[i] = __fadd_rn(sum[i], __shfl_xor_sync(0xffffffffu, sum[i], off));
+      for (int off = 1; off < LPR; off <<= 1) sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, off));
+      mine = i == 0 || li % R == i ? sum : mine;
     }
-    float mine = sum[0];
-#pragma unroll
-    for (int i = 1; i < R; ++i) mine = li % R == i ? sum[i] : mine;
-    const float root = __fdiv_rn(1.f, __fsqrt_rn(__fadd_rn(__fmul_rn(mine, 1.f / D), nm.eps)));
-#pragma unroll
-    for (int i = 0; i < R; ++i) inv[i] = R == 1 ? root : __shfl_sync(0xffffffffu, root, (lane & ~(LPR - 1)) + i);
-    float w[8];
-    load_weight8(nm, li, w);
-#pragma unroll
-    for (int i = 0; i < R; ++i)
-#pragma unroll
-      for (int k = 0; k < 8; ++k) e[i][k] = __fmul_rn(__fmul_rn(e[i][k], inv[i]), w[k]);
+    root = __fdiv_rn(1.f, __fsqrt_rn(__fadd_rn(__fmul_rn(mine, 1.f / D), nm.eps)));
   }
-  if (turning) {
-    if (a.interleaved) {
-      if (turns) {
-#pragma unroll
-        for (int i = 0; i < R; ++i)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float u = e[i][2 * k], w = e[i][2 * k + 1];
-            e[i][2 * k] = __fsub_rn(__fmul_rn(u, cs[k]), __fmul_rn(w, sn[k]));
-            e[i][2 * k + 1] = __fadd_rn(__fmul_rn(u, sn[k]), __fmul_rn(w, cs[k]));
-          }
-      }
-    } else {
-      const int partner = (lane & ~(LPR - 1)) + (turns ? (low ? li + (a.rot >> 4) : li - (a.rot >> 4)) : li);
-#pragma unroll
-      for (int i = 0; i < R; ++i)
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float o = __shfl_sync(0xffffffffu, e[i][k], partner);
-          if (turns) e[i][k] = __fadd_rn(__fmul_rn(e[i][k], cs[k]), __fmul_rn(o, sn[k]));
-        }
-    }
-  }
+  const int partner = (lane & ~(LPR - 1)) + (turns ? (low ? li + (a.rot >> 4) : li - (a.rot >> 4)) : li);
 
+  uint8_t *out = nullptr, *data = nullptr;
+  uint32_t *meta = nullptr;
+  long long row0 = 0, hstep = 0;
   if (!CACHE || kind == 0) {
     if (bad_pos) {
       if (lane == 0) atomicOr(&g_kvfb_heads_error, 1u);
       return;
     }
-    uint8_t *out = a.q_out.p + b * a.q_out.sb + j * a.q_out.st + 8 * li * dtype_bytes(DT);
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const int r = r0 + i * RPW;
-      if (r < a.q.heads) store8<DT>(out + r * a.q_out.sh, a.q_out.vec, e[i]);
-    }
-    return;
-  }
-  if (CACHE) {
+    out = a.q_out.p + b * a.q_out.sb + j * a.q_out.st + 8 * li * dtype_bytes(DT);
+  } else {
     // Heads of a token lie one row apart (token-major) or a whole sequence or page apart.
-    const long long row0 = bad_pos ? -1 : a.cache.row(b, 0, t);
+    row0 = bad_pos ? -1 : a.cache.row(b, 0, t);
     if (row0 < 0) {
       if (lane == 0) atomicOr(&g_kvfb_heads_error, 1u);
       return;
     }
-    const long long hstep = !a.cache.head_major ? 1 : a.cache.paged ? 1ll << a.cache.bt_shift : a.cache.n;
-    uint8_t *data = kind == 1 ? a.kd : a.vd;
-    uint32_t *meta = reinterpret_cast<uint32_t *>(kind == 1 ? a.km : a.vm);
-    const int lpg = a.group >> 3, gshift = __popc(a.group - 1);  // group is a power of two
+    hstep = !a.cache.head_major ? 1 : a.cache.paged ? 1ll << a.cache.bt_shift : a.cache.n;
+    data = kind == 1 ? a.kd : a.vd;
+    meta = reinterpret_cast<uint32_t *>(kind == 1 ? a.km : a.vm);
+  }
+
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const int r = r0 + i * RPW;
-      if (__all_sync(0xffffffffu, r >= src.heads)) return;
-      const bool live = r < src.heads;
-      const long long dr = row0 + r * hstep;
-      if (a.fmt == KVF_FMT_F16) {
-        if (live) store8<KVF_DT_F16>(data + (dr * D + 8 * li) * 2, true, e[i]);
-        continue;
+  for (int i = 0; i < R; ++i) {
+    const int r = r0 + i * RPW;
+    if (__all_sync(0xffffffffu, r >= src.heads)) return;
+    const bool live = r < src.heads;
+    float e[8];
+    values8<DT>(raw[i], e);
+    if (normed) {
+      const float inv = R == 1 ? root : __shfl_sync(0xffffffffu, root, (lane & ~(LPR - 1)) + i);
+#pragma unroll
+      for (int k = 0; k < 8; k += 2) {
+        mul2(e[k], e[k + 1], e[k], e[k + 1], inv, inv);
+        mul2(e[k], e[k + 1], e[k], e[k + 1], w[k], w[k + 1]);
       }
-      const GroupScale g = group_scale8(e[i], li, a.group, a.fmt == KVF_FMT_INT8 ? 255 : 15);
-      if (!live) continue;
-      if ((li & (lpg - 1)) == 0) meta[(dr * D + 8 * li) >> gshift] = g.word;
-      if (a.fmt == KVF_FMT_INT8)
-        store_codes8<KVF_FMT_INT8>(e[i], g, data + dr * D, li);
-      else
-        store_codes8<KVF_FMT_INT4>(e[i], g, data + dr * (D / 2), li);
     }
+    if (turning) {
+      if (a.interleaved) {
+        if (turns) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float x = e[2 * k], y = e[2 * k + 1];
+            e[2 * k] = __fsub_rn(__fmul_rn(x, cs[k]), __fmul_rn(y, sn[k]));
+            e[2 * k + 1] = __fadd_rn(__fmul_rn(x, sn[k]), __fmul_rn(y, cs[k]));
+          }
+        }
+      } else {
+        float o[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) o[k] = __shfl_sync(0xffffffffu, e[k], partner);
+        if (turns) {
+#pragma unroll
+          for (int k = 0; k < 8; k += 2) {
+            mul2(e[k], e[k + 1], e[k], e[k + 1], cs[k], cs[k + 1]);
+            mul2(o[k], o[k + 1], o[k], o[k + 1], sn[k], sn[k + 1]);
+            // scalar sums: a packed one may be contracted with its products
+            e[k] = __fadd_rn(e[k], o[k]);
+            e[k + 1] = __fadd_rn(e[k + 1], o[k + 1]);
+          }
+        }
+      }
+    }
+    if (!CACHE || kind == 0) {
+      if (live) store8<DT>(out + r * a.q_out.sh, a.q_out.vec, e);
+      continue;
+    }
+    const long long dr = row0 + r * hstep;
+    if (a.fmt == KVF_FMT_F16) {
+      if (live) store8<KVF_DT_F16>(data + (dr * D + 8 * li) * 2, true, e);
+      continue;
+    }
+    const GroupScale g = group_scale8(e, li, a.group, a.fmt == KVF_FMT_INT8 ? 255 : 15);
+    if (!live) continue;
+    if ((li & ((a.group >> 3) - 1)) == 0) meta[(dr * D + 8 * li) >> __popc(a.group - 1)] = g.word;  // group: a power of two
+    if (a.fmt == KVF_FMT_INT8)
+      store_codes8<KVF_FMT_INT8>(e, g, data + dr * D, li);
+    else
+      store_codes8<KVF_FMT_INT4>(e, g, data + dr * (D / 2), li);
   }
 }
 
@@ -233,10 +238,11 @@ template <int DT, int D>
 cudaError_t launch_heads(HeadsArgs a, cudaStream_t st) {
   constexpr int RPW = 32 / (D / 8);
   const long long tokens = (long long)a.B * a.T;
-  // Four rows per lane group where that still gives every SM some 16 warps; one
+  // Several rows per lane group where that still gives every SM some 32 warps; one
   // in short calls, whose time is that of one row.
+  constexpr int R = DT == KVF_DT_F32 ? 2 : 4;
   const long long pairs = (a.q.heads + RPW - 1) / RPW + (a.k.heads + RPW - 1) / RPW + (a.v.heads + RPW - 1) / RPW;
-  const int r = tokens * pairs >= 4 * 148 * 16 ? 4 : 1;
+  const int r = tokens * pairs >= R * 148 * 32 ? R : 1;
   a.q_units = (a.q.heads + r * RPW - 1) / (r * RPW);
   a.k_units = (a.k.heads + r * RPW - 1) / (r * RPW);
   a.units = a.q_units + a.k_units + (a.v.heads + r * RPW - 1) / (r * RPW);
@@ -244,13 +250,13 @@ cudaError_t launch_heads(HeadsArgs a, cudaStream_t st) {
   if (warps > 0xffffffffLL - 8) return cudaErrorInvalidValue;
   const unsigned blocks = (unsigned)((warps + 7) / 8);
   if (a.k.heads == 0) {
-    if (r == 4)
-      heads_kernel<DT, D, 4, false><<<blocks, 256, 0, st>>>(a);
+    if (r == R)
+      heads_kernel<DT, D, R, false><<<blocks, 256, 0, st>>>(a);
     else
       heads_kernel<DT, D, 1, false><<<blocks, 256, 0, st>>>(a);
   } else {
-    if (r == 4)
-      heads_kernel<DT, D, 4, true><<<blocks, 256, 0, st>>>(a);
+    if (r == R)
+      heads_kernel<DT, D, R, true><<<blocks, 256, 0, st>>>(a);
     else
       heads_kernel<DT, D, 1, true><<<blocks, 256, 0, st>>>(a);
   }

@@ -69,6 +69,53 @@ template <int DT> __device__ __forceinline__ void load8(const void *p, bool vec,
   }
 }
 
+// Eight channels as they lie in memory, and their values.
+template <int DT> struct Raw8 {
+  uint4 a[DT == KVF_DT_F32 ? 2 : 1];
+};
+template <int DT> __device__ __forceinline__ Raw8<DT> load_raw8(const void *p, bool vec) {
+  Raw8<DT> r;
+  if (vec) {
+#pragma unroll
+    for (int k = 0; k < (DT == KVF_DT_F32 ? 2 : 1); ++k) r.a[k] = __ldcs(reinterpret_cast<const uint4 *>(p) + k);
+  } else if (DT == KVF_DT_F32) {
+    const uint32_t *e = reinterpret_cast<const uint32_t *>(p);
+#pragma unroll
+    for (int k = 0; k < (DT == KVF_DT_F32 ? 2 : 1); ++k) r.a[k] = make_uint4(e[4 * k], e[4 * k + 1], e[4 * k + 2], e[4 * k + 3]);
+  } else {
+    const uint16_t *e = reinterpret_cast<const uint16_t *>(p);
+    r.a[0] = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16,
+                        e[6] | (uint32_t)e[7] << 16);
+  }
+  return r;
+}
+template <int DT> __device__ __forceinline__ void values8(const Raw8<DT> &r, float (&e)[8]) {
+  if (DT == KVF_DT_F32) {
+#pragma unroll
+    for (int k = 0; k < (DT == KVF_DT_F32 ? 2 : 1); ++k) {
+      e[4 * k] = __uint_as_float(r.a[k].x);
+      e[4 * k + 1] = __uint_as_float(r.a[k].y);
+      e[4 * k + 2] = __uint_as_float(r.a[k].z);
+      e[4 * k + 3] = __uint_as_float(r.a[k].w);
+    }
+  } else {
+    const uint32_t w[4] = {r.a[0].x, r.a[0].y, r.a[0].z, r.a[0].w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 f = widen2<DT>(w[k]);
+      e[2 * k] = f.x;
+      e[2 * k + 1] = f.y;
+    }
+  }
+}
+
+// Two products, each rounded to nearest, in one instruction.
+__device__ __forceinline__ void mul2(float &x, float &y, float a, float b, float c, float d) {
+  asm("{\n\t.reg .b64 u, v, w;\n\tmov.b64 u, {%2, %3};\n\tmov.b64 v, {%4, %5};\n\tmul.rn.f32x2 w, u, v;\n\t"
+      "mov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(x), "=f"(y)
+      : "f"(a), "f"(b), "f"(c), "f"(d));
+}
 template <int DT> __device__ __forceinline__ void store8(void *p, bool vec, const float (&e)[8]) {
   using T = typename Elem<DT>::T;
   if (!vec) {
