@@ -47,26 +47,6 @@ __device__ __forceinline__ int code(float x, float zero, float sc, int levels) {
   return q < 0 ? 0 : (q > levels ? levels : (int)q);
 }
 
-// code() without the division in the common case. With a = x - zero (fp32,
-// as the host computes it) and r = 1/sc rounded to nearest, t' = a * r is
-// within 3 * 2^-24 |t| of the host's t = a / sc (both correctly rounded), so
-// for |t'| < 1024 the two differ by less than 2^-12. When t' is further than
-// that from every half-integer, t lies strictly between the same two
-// half-integers as t', and round-half-away(t) = rint(t'); otherwise (and for
-// |t'| >= 1024, NaN or infinities, including sc = 0) the exact code() decides.
-__device__ __forceinline__ int code_fast(float x, float zero, float sc, float rsc, int levels) {
-  const float a = __fsub_rn(x, zero);
-  const float t = __fmul_rn(a, rsc);
-  if (fabsf(t) < 1024.f) {
-    const float q = rintf(t);
-    if (fabsf(__fsub_rn(t, q)) < 0.5f - 0x1p-12f) {
-      const int qi = (int)q;
-      return qi < 0 ? 0 : (qi > levels ? levels : qi);
-    }
-  }
-  return code(x, zero, sc, levels);
-}
-
 // One group of a row held as eight channels per lane (group / 8 adjacent
 // lanes, a power of two): its (scale, zero) word and their fp32 values.
 struct GroupScale {
@@ -74,16 +54,16 @@ struct GroupScale {
   float zero, sc, rsc;
 };
 
-// Scale and zero of lane li's group, combined across the group's lanes with
-// shuffles (every lane of the warp takes part). The combination keeps the
-// host loop's results bit for bit: a lane that does not hold the group's first
-// element folds its values into +inf / -inf (NaNs never replace a running
-// value in the host loop, which starts from the first element), the first lane
-// starts from that element (a NaN there stays NaN), and two adjacent ranges
-// combine as the loop would have met them, earlier range first (ties keep the
-// earlier value).
-__device__ __forceinline__ GroupScale group_scale8(const float (&e)[8], int li, int group, int levels) {
-  const int lpg = group >> 3;  // lanes per group
+// Range of lane li's group by the host loop's comparisons (first-wins), combined
+// across the group's lanes with shuffles (every lane of the warp takes part). A
+// lane that does not hold the group's first element folds its values into +inf /
+// -inf (NaNs never replace a running value in the host loop, which starts from
+// the first element), the first lane starts from that element (a NaN there stays
+// NaN), and two adjacent ranges combine as the loop would have met them, earlier
+// range first (ties keep the earlier value).
+__device__ __noinline__ float2 group_range8_exact(float e0, float e1, float e2, float e3, float e4, float e5, float e6,
+                                                  float e7, int li, int lpg) {
+  const float e[8] = {e0, e1, e2, e3, e4, e5, e6, e7};
   const bool first = (li & (lpg - 1)) == 0;
   float lo = first ? e[0] : INFINITY, hi = first ? e[0] : -INFINITY;
 #pragma unroll
@@ -101,6 +81,37 @@ __device__ __forceinline__ GroupScale group_scale8(const float (&e)[8], int li, 
     lo = (blo < alo) ? blo : alo;
     hi = (ahi < bhi) ? bhi : ahi;
   }
+  return make_float2(lo, hi);
+}
+
+__device__ __forceinline__ float min3f(float a, float b, float c) {
+  float r;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float max3f(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// Scale and zero of lane li's group, bit for bit the host loop's. The hardware's
+// minimum and maximum give its range except where the group starts with a NaN
+// (which the host keeps and they drop) or where its least value is a zero, whose
+// sign the host takes from the first one; those go by group_range8_exact.
+__device__ __forceinline__ GroupScale group_scale8(const float (&e)[8], int li, int group, int levels) {
+  const int lpg = group >> 3;  // lanes per group
+  float lo = fminf(min3f(min3f(min3f(e[0], e[1], e[2]), e[3], e[4]), e[5], e[6]), e[7]);
+  float hi = fmaxf(max3f(max3f(max3f(e[0], e[1], e[2]), e[3], e[4]), e[5], e[6]), e[7]);
+  for (int off = 1; off < lpg; off <<= 1) {
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, off));
+    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, off));
+  }
+  if (__any_sync(0xffffffffu, !(lo != 0.f && lo == lo) || e[0] != e[0])) {
+    const float2 r = group_range8_exact(e[0], e[1], e[2], e[3], e[4], e[5], e[6], e[7], li, lpg);
+    lo = r.x;
+    hi = r.y;
+  }
   const __half zero_h = __float2half_rn(lo);
   float scale = __fdiv_rn(__fsub_rn(hi, lo), (float)levels);
   if (scale <= 0.f) scale = 1.f;
@@ -113,21 +124,54 @@ __device__ __forceinline__ GroupScale group_scale8(const float (&e)[8], int li, 
   return g;
 }
 
+// code() of eight values. Without the division in the common case: with a = x -
+// zero (fp32, as the host computes it) and r = 1/sc rounded to nearest, t = a * r
+// is within 3 * 2^-24 |t| of the host's a / sc (both correctly rounded), so for
+// |t| < 1024 the two differ by less than 2^-12. Where t clamped to [0, levels] is
+// further than that from every half-integer, the nearest integer is the host's
+// code (clamping and rounding to nearest commute: the ends are integers). Otherwise
+// (and for |t| >= 1024, infinities and a zero scale) the exact code() decides;
+// a NaN is code 0 either way. Adding 1.5 * 2^23 leaves the integer in the low bits.
+__device__ __noinline__ void codes8_exact(float x0, float x1, float x2, float x3, float x4, float x5, float x6, float x7,
+                                          float zero, float sc, int levels, uint32_t &lo, uint32_t &hi) {
+  lo = (uint32_t)code(x0, zero, sc, levels) | (uint32_t)code(x1, zero, sc, levels) << 8 |
+       (uint32_t)code(x2, zero, sc, levels) << 16 | (uint32_t)code(x3, zero, sc, levels) << 24;
+  hi = (uint32_t)code(x4, zero, sc, levels) | (uint32_t)code(x5, zero, sc, levels) << 8 |
+       (uint32_t)code(x6, zero, sc, levels) << 16 | (uint32_t)code(x7, zero, sc, levels) << 24;
+}
+__device__ __forceinline__ void codes8(const float (&e)[8], const GroupScale &g, int levels, uint32_t &lo, uint32_t &hi) {
+  const float top = (float)levels, big = 12582912.f;
+  float far = 0.f, off = 0.f;
+  uint32_t y[8];
+#pragma unroll
+  for (int k = 0; k < 8; k += 2) {
+    const float t0 = __fmul_rn(__fsub_rn(e[k], g.zero), g.rsc), t1 = __fmul_rn(__fsub_rn(e[k + 1], g.zero), g.rsc);
+    far = max3f(far, fabsf(t0), fabsf(t1));
+    const float c0 = fminf(fmaxf(t0, 0.f), top), c1 = fminf(fmaxf(t1, 0.f), top);
+    const float y0 = __fadd_rn(c0, big), y1 = __fadd_rn(c1, big);
+    off = max3f(off, fabsf(__fsub_rn(c0, __fsub_rn(y0, big))), fabsf(__fsub_rn(c1, __fsub_rn(y1, big))));
+    y[k] = __float_as_uint(y0);
+    y[k + 1] = __float_as_uint(y1);
+  }
+  lo = __byte_perm(__byte_perm(y[0], y[1], 0x0040), __byte_perm(y[2], y[3], 0x0040), 0x5410);
+  hi = __byte_perm(__byte_perm(y[4], y[5], 0x0040), __byte_perm(y[6], y[7], 0x0040), 0x5410);
+  if (!(far < 1024.f && off < 0.5f - 0x1p-12f))
+    codes8_exact(e[0], e[1], e[2], e[3], e[4], e[5], e[6], e[7], g.zero, g.sc, levels, lo, hi);
+}
+
 // Lane li's eight codes of a row whose payload starts at `row` (8-byte aligned
 // for int8, 4-byte for int4).
 template <int FMT>
 __device__ __forceinline__ void store_codes8(const float (&e)[8], const GroupScale &g, uint8_t *row, int li) {
-  const int levels = FMT == KVF_FMT_INT8 ? 255 : 15;
-  uint32_t c[8];
-#pragma unroll
-  for (int k = 0; k < 8; ++k) c[k] = (uint32_t)code_fast(e[k], g.zero, g.sc, g.rsc, levels);
+  uint32_t lo, hi;
+  codes8(e, g, FMT == KVF_FMT_INT8 ? 255 : 15, lo, hi);
   if (FMT == KVF_FMT_INT8) {
-    const uint2 w = make_uint2(c[0] | (c[1] << 8) | (c[2] << 16) | (c[3] << 24),
-                               c[4] | (c[5] << 8) | (c[6] << 16) | (c[7] << 24));
-    reinterpret_cast<uint2 *>(row)[li] = w;
+    reinterpret_cast<uint2 *>(row)[li] = make_uint2(lo, hi);
   } else {
-    reinterpret_cast<uint32_t *>(row)[li] =
-        c[0] | (c[1] << 4) | (c[2] << 8) | (c[3] << 12) | (c[4] << 16) | (c[5] << 20) | (c[6] << 24) | (c[7] << 28);
+    // bytes 0, 1, 2, 3 hold codes 0 .. 15: neighbours share a byte, the odd one above
+    lo |= lo >> 4;
+    hi |= hi >> 4;
+    reinterpret_cast<uint32_t *>(row)[li] = __byte_perm(lo, hi, 0x6420);
   }
 }
 
