@@ -5,7 +5,9 @@
 // (11 significant bits each, the exponent range of fp32, so nothing has to be
 // scaled), and a product is hi*hi + lo*hi + hi*lo accumulated in fp32: relative
 // error about 2^-21 per product. f16 caches need no lo for K and V, whose 11
-// bits tf32 holds.
+// bits tf32 holds. The tensor cores' own sums are short (32 channels of a score,
+// one step of an output): they round towards zero, and what they leave is added
+// in fp32 to nearest.
 //
 // Four warps of 16 rows share tiles of 64 tokens, dequantised to fp32 in shared
 // memory. Scores stay in registers: the fragment that the score product leaves
@@ -28,17 +30,20 @@ __host__ __device__ constexpr int chunk_mma_smem(int d) {
   return (kChunkRows * (d + 8) + kChunkTokens * (d + 8) + kChunkTokens * (d + 4)) * 4 + 16;
 }
 
-__device__ __forceinline__ uint32_t tf32(float x) {
-  uint32_t r;
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
-  return r;
-}
-
-// x = hi + lo; an infinity or NaN stays in hi alone.
+// x = hi + lo: hi is x rounded to tf32's 11 bits, lo the exact rest, of which the
+// tensor cores take the upper 11 bits (off by at most 2^-23 of x).
 __device__ __forceinline__ void split(float x, uint32_t &hi, uint32_t &lo) {
-  hi = tf32(x);
-  const float r = __fsub_rn(x, __uint_as_float(hi));
-  lo = fabsf(r) < INFINITY ? tf32(r) : 0u;
+  hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+  lo = __float_as_uint(__fsub_rn(x, __uint_as_float(hi)));
+}
+// K and V of an f16 cache are tf32 numbers as they are (infinities stay so).
+template <bool LO> __device__ __forceinline__ void split_if(float x, uint32_t &hi, uint32_t &lo) {
+  if (LO) {
+    split(x, hi, lo);
+  } else {
+    hi = __float_as_uint(x);
+    lo = 0u;
+  }
 }
 
 __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
@@ -106,24 +111,33 @@ __global__ void __launch_bounds__(kChunkThreads) chunk_mma_kernel(const ChunkArg
     for (int n = 0; n < kChunkTokens / 8; ++n)
 #pragma unroll
       for (int k = 0; k < 4; ++k) s[n][k] = 0.f;
-#pragma unroll 2
-    for (int c = 0; c < D; c += 8) {
-      const float2 q0 = *reinterpret_cast<const float2 *>(sq + r_lo * QS + c + 2 * t4);
-      const float2 q1 = *reinterpret_cast<const float2 *>(sq + r_hi * QS + c + 2 * t4);
-      uint32_t qh[4], ql[4];
-      split(q0.x, qh[0], ql[0]);
-      split(q1.x, qh[1], ql[1]);
-      split(q0.y, qh[2], ql[2]);
-      split(q1.y, qh[3], ql[3]);
+#pragma unroll 1
+    for (int c0 = 0; c0 < D; c0 += 32) {
+      uint32_t qh[4][4], ql[4][4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 q0 = *reinterpret_cast<const float2 *>(sq + r_lo * QS + c0 + 8 * k + 2 * t4);
+        const float2 q1 = *reinterpret_cast<const float2 *>(sq + r_hi * QS + c0 + 8 * k + 2 * t4);
+        split(q0.x, qh[k][0], ql[k][0]);
+        split(q1.x, qh[k][1], ql[k][1]);
+        split(q0.y, qh[k][2], ql[k][2]);
+        split(q1.y, qh[k][3], ql[k][3]);
+      }
 #pragma unroll
       for (int n = 0; n < kChunkTokens / 8; ++n) {
-        const float2 k2 = *reinterpret_cast<const float2 *>(sk + (8 * n + g4) * KS + c + 2 * t4);
-        uint32_t kh[2], kl[2];
-        split(k2.x, kh[0], kl[0]);
-        split(k2.y, kh[1], kl[1]);
-        if (DT != KVF_DT_BF16 && DT != KVF_DT_F16) mma_tf32(s[n], ql, kh);  // 16-bit queries are tf32 numbers
-        if (LO) mma_tf32(s[n], qh, kl);
-        mma_tf32(s[n], qh, kh);
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 k2 = *reinterpret_cast<const float2 *>(sk + (8 * n + g4) * KS + c0 + 8 * k + 2 * t4);
+          uint32_t kh[2], kl[2];
+          split_if<LO>(k2.x, kh[0], kl[0]);
+          split_if<LO>(k2.y, kh[1], kl[1]);
+          mma_tf32(acc, ql[k], kh);
+          if (LO) mma_tf32(acc, qh[k], kl);
+          mma_tf32(acc, qh[k], kh);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s[n][k] += acc[k];
       }
     }
 
@@ -160,14 +174,14 @@ __global__ void __launch_bounds__(kChunkThreads) chunk_mma_kernel(const ChunkArg
         l_lo += s[n][k];
         l_hi += s[n][2 + k];
       }
-#pragma unroll
-    for (int n = 0; n < D / 8; ++n) {
-      o[n][0] *= f_lo;
-      o[n][1] *= f_lo;
-      o[n][2] *= f_hi;
-      o[n][3] *= f_hi;
-    }
     if (*reinterpret_cast<volatile int *>(odd)) {
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n) {
+        o[n][0] *= f_lo;
+        o[n][1] *= f_lo;
+        o[n][2] *= f_hi;
+        o[n][3] *= f_hi;
+      }
       // 0 * inf would carry an infinity or NaN into rows that do not see its
       // token: such a step is added token by token, each row what it sees.
       for (int u = 0; u < kChunkTokens; ++u) {
@@ -193,23 +207,31 @@ __global__ void __launch_bounds__(kChunkThreads) chunk_mma_kernel(const ChunkArg
       }
       continue;
     }
+    uint32_t ph[kChunkTokens / 8][4], pl[kChunkTokens / 8][4];
 #pragma unroll
     for (int u = 0; u < kChunkTokens / 8; ++u) {
-      uint32_t ph[4], pl[4];
-      split(s[u][0], ph[0], pl[0]);
-      split(s[u][2], ph[1], pl[1]);
-      split(s[u][1], ph[2], pl[2]);
-      split(s[u][3], ph[3], pl[3]);
-      const float *v0 = sv + (8 * u + 2 * t4) * VS + g4;
+      split(s[u][0], ph[u][0], pl[u][0]);
+      split(s[u][2], ph[u][1], pl[u][1]);
+      split(s[u][1], ph[u][2], pl[u][2]);
+      split(s[u][3], ph[u][3], pl[u][3]);
+    }
+    const float *v0 = sv + 2 * t4 * VS + g4;
 #pragma unroll
-      for (int n = 0; n < D / 8; ++n) {
+    for (int n = 0; n < D / 8; ++n) {
+      float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int u = 0; u < kChunkTokens / 8; ++u) {
         uint32_t vh[2], vl[2];
-        split(v0[8 * n], vh[0], vl[0]);
-        split(v0[VS + 8 * n], vh[1], vl[1]);
-        mma_tf32(o[n], pl, vh);
-        if (LO) mma_tf32(o[n], ph, vl);
-        mma_tf32(o[n], ph, vh);
+        split_if<LO>(v0[8 * u * VS + 8 * n], vh[0], vl[0]);
+        split_if<LO>(v0[(8 * u + 1) * VS + 8 * n], vh[1], vl[1]);
+        mma_tf32(acc, pl[u], vh);
+        if (LO) mma_tf32(acc, ph[u], vl);
+        mma_tf32(acc, ph[u], vh);
       }
+      o[n][0] = fmaf(o[n][0], f_lo, acc[0]);
+      o[n][1] = fmaf(o[n][1], f_lo, acc[1]);
+      o[n][2] = fmaf(o[n][2], f_hi, acc[2]);
+      o[n][3] = fmaf(o[n][3], f_hi, acc[3]);
     }
   }
 
