@@ -109,8 +109,8 @@ ChunkRows chunk_rows(const kvf_heads &r) {
 }
 
 // Splits of each tile's tokens. Tensor-core kernel: the blocks run one per SM,
-// a block costs its steps and about three more to start and end; the count
-// that makes the waves shortest.
+// a block costs its steps and about six more to start and end, and writing and
+// merging partials about sixteen; the count that makes the waves shortest.
 int pick_splits(int B, int T, int H, int Hkv, int n, int dtype) {
   const long long rows = (long long)T * (H / Hkv);
   const int sms = device_sm_count();
@@ -126,7 +126,7 @@ int pick_splits(int B, int T, int H, int Hkv, int n, int dtype) {
   long long best = -1;
   int s = 1;
   for (int k = 1; k <= std::min(64, std::max(1, steps / 2)); ++k) {
-    const long long cost = (blocks * k + sms - 1) / sms * ((steps + k - 1) / k + 3 + (k > 1 ? 2 : 0));
+    const long long cost = (blocks * k + sms - 1) / sms * ((steps + k - 1) / k + 6) + (k > 1 ? 16 : 0);
     if (best < 0 || cost < best) {
       best = cost;
       s = k;

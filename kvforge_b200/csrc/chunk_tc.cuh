@@ -576,24 +576,30 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
         const uint32_t raw = sbase + L::OFF_RAW + (uint32_t)(op * RSLOTS + rs) * L::RAWB;
         const uint32_t meta = sbase + L::OFF_META + (uint32_t)(op * RSLOTS + rs) * L::METAB;
         const int tok = w.t0 + i * kTcHalf;
+        // All pieces of the half first, so that their loads overlap.
+        constexpr int N = CPR / 2;
+        uint32_t in[N][4], sz[N];
 #pragma unroll
-        for (int k = 0; k < CPR / 2; ++k) {
+        for (int k = 0; k < N; ++k) {
           const int rr = r0 + k * RPP;             // row of the half step
           // the raw tile has TMA's swizzle of its row width
           const int pc = RB == 128 ? ch ^ (rr & 7) : RB == 64 ? ch ^ ((rr >> 1) & 3) : ch ^ ((rr >> 2) & 1);
-          uint32_t in[4], sz;
           asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                       : "=r"(in[0]), "=r"(in[1]), "=r"(in[2]), "=r"(in[3])
+                       : "=r"(in[k][0]), "=r"(in[k][1]), "=r"(in[k][2]), "=r"(in[k][3])
                        : "r"(raw + (uint32_t)(rr * RB + pc * 16)));
-          asm volatile("ld.shared.u32 %0, [%1];" : "=r"(sz) : "r"(meta + (uint32_t)((rr * a.gpr + gword) * 4)));
-          if (tok + rr >= w.t1) sz = 0u;           // a row that nobody sees: zeros, whatever its page holds
-          const uint32_t s2 = ptx::prmt(sz, sz, 0x1010), z2 = ptx::prmt(sz, sz, 0x3232);
+          asm volatile("ld.shared.u32 %0, [%1];" : "=r"(sz[k]) : "r"(meta + (uint32_t)((rr * a.gpr + gword) * 4)));
+        }
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          const int rr = r0 + k * RPP;
+          if (tok + rr >= w.t1) sz[k] = 0u;        // a row that nobody sees: zeros, whatever its page holds
+          const uint32_t s2 = ptx::prmt(sz[k], sz[k], 0x1010), z2 = ptx::prmt(sz[k], sz[k], 0x3232);
           uint32_t o[4 * P16];
           if (FMT == KVF_FMT_INT8) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
               // bytes under the exponent of 1024: half2 of 1024 + code, exact; less 1024, exact
-              const uint32_t lo = ptx::prmt(in[q], 0x64646464u, 0x4140), hi = ptx::prmt(in[q], 0x64646464u, 0x4342);
+              const uint32_t lo = ptx::prmt(in[k][q], 0x64646464u, 0x4140), hi = ptx::prmt(in[k][q], 0x64646464u, 0x4342);
               o[2 * q] = ptx::hfma2_u32(ptx::hsub2_u32(lo, 0x64006400u), s2, z2);
               o[2 * q + 1] = ptx::hfma2_u32(ptx::hsub2_u32(hi, 0x64006400u), s2, z2);
             }
@@ -604,7 +610,7 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
 #pragma unroll
               for (int u = 0; u < 4; ++u)
                 v[u] = ptx::hfma2_u32(
-                    ptx::hsub2_u32(ptx::lop3_and_or(in[q] >> (4 * u), 0x000F000Fu, 0x64006400u), 0x64006400u), s2, z2);
+                    ptx::hsub2_u32(ptx::lop3_and_or(in[k][q] >> (4 * u), 0x000F000Fu, 0x64006400u), 0x64006400u), s2, z2);
               o[4 * q] = ptx::prmt(v[0], v[1], 0x5410);
               o[4 * q + 1] = ptx::prmt(v[2], v[3], 0x5410);
               o[4 * q + 2] = ptx::prmt(v[0], v[1], 0x7632);
@@ -838,12 +844,24 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
         if (!take_v(i)) break;
         const int next = i + STRIDE;
         const bool more = next < n;
-        for (int h = 0; h < 2 && ok; ++h) {
-          if (j < nw[g] && !values(i, j, h)) break;
-          if (h == 1) release(&sh.vempty[i % SLOTS]);
-          if (more && (h == 1 || take_k(next)) && j + 1 < nw[g]) scores(next, h);
+        // The first half's next scores go between the two products, unless the
+        // K tile is late: the second product does not wait for it.
+        if (j < nw[g] && !values(i, j, 0)) break;
+        const bool between = more && __all_sync(0xffffffffu, ptx::mbar_test_wait(bar(&sh.kfull[next % SLOTS]),
+                                                                               (uint32_t)((next / SLOTS) & 1)));
+        if (between) {
+          tc::fence_after();
+          if (j + 1 < nw[g]) scores(next, 0);
         }
-        if (more && ok) release(&sh.kempty[next % SLOTS]);
+        if (j < nw[g] && !values(i, j, 1)) break;
+        release(&sh.vempty[i % SLOTS]);
+        if (more && (between || take_k(next))) {
+          if (j + 1 < nw[g]) {
+            if (!between) scores(next, 0);
+            scores(next, 1);
+          }
+          release(&sh.kempty[next % SLOTS]);
+        }
       }
       if (!ok && lane == 0) {
         atomicOr(&g_kvfb_chunk_error, 1u);
