@@ -697,51 +697,69 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
     if (lane == 0) ptx::prefetch_tmap(map);
     const uint64_t pol = ptx::policy_evict_last();
     const bool paged = a.cache.paged != 0;
-    const int bts = paged ? a.cache.bt_shift : 30;
+    const int bts = paged ? a.cache.bt_shift : 30, bmask = (1 << bts) - 1;
     const int tbs = min(bts, 6);             // log2 of the tokens of a box
-    const int span = L::RAW ? kTcHalf : kTcStep, boxes = span >> tbs;
+    const int span = L::RAW ? kTcHalf : kTcStep, boxes = span >> tbs;  // 1 to 8 boxes an item
     const int count = L::RAW ? 2 * n : n;
+    const int box = lane & (boxes - 1);
     const int *table = paged ? a.cache.table + (long long)w.b * a.cache.max_blocks : nullptr;
-    // Page (or sequence) of box `lane` of item i; -1 where there is nothing to read.
+    // Page (or sequence) of box `box` of item i; -1 where there is nothing to read.
     auto page_of = [&](int i) -> int {
-      const int t = w.t0 + i * span + ((lane % boxes) << tbs);
+      const int t = w.t0 + i * span + (box << tbs);
+      int page = paged ? -1 : w.b;
       if (i >= count || t >= w.t1) return -1;
-      return paged ? max(__ldg(table + (t >> bts)), -1) : w.b;
+      if (paged) page = __ldg(table + (t >> bts));
+      return page;
     };
+    // One elected lane issues an item's boxes; coordinates come from the lanes
+    // that hold them.
+    auto fill = [&](uint32_t dst, uint32_t full, uint32_t bytes, int t, int page) {
+      const int my = max(page, -1);
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        if (x < boxes) {
+          const int pg = __shfl_sync(0xffffffffu, my, x);
+          if (tc::elect_one()) {
+            if (x == 0) ptx::mbar_arrive_expect_tx(full, bytes);
+            const int c1 = paged ? (t + (x << tbs)) & bmask : t + (x << tbs);
+            if (L::RAW) {
+              ptx::tma_g2s_4d(dst + ((uint32_t)x << tbs) * RB, map, 0, c1, w.h, pg, full, pol);
+            } else {
+#pragma unroll
+              for (int blk = 0; blk < KB; ++blk)
+                ptx::tma_g2s_4d(dst + blk * BLK + ((uint32_t)x << tbs) * 128u, map, 128 * blk, c1, w.h, pg, full, pol);
+            }
+          }
+          __syncwarp();
+        }
+      }
+    };
+    // Metadata row of token tok in a page (or sequence) of 2^32 rows at most: fewer fit a GPU.
+    const unsigned heads = (unsigned)a.cache.Hkv, hd = (unsigned)w.h;
+    const unsigned pstep = paged ? heads << bts : heads * (unsigned)a.cache.n;
+    const unsigned tstep = a.cache.head_major ? 1u : heads;
+    const unsigned hoff = !a.cache.head_major ? hd : paged ? hd << bts : hd * (unsigned)a.cache.n;
     bool ok = true;
     int page = page_of(0), i = 0;
     for (; i < count; ++i) {
-      const int next = page_of(i + 1);
       const int t = w.t0 + i * span;
-      const int c1 = paged ? (t + ((lane % boxes) << tbs)) & ((1 << bts) - 1) : t + ((lane % boxes) << tbs);
-      if (L::RAW) {
-        constexpr int R = RSLOTS > 0 ? RSLOTS : 1;
-        const int s = i % R;
-        if (i >= R && !tc_wait_warp(bar(&sh.rempty[op][s]), (uint32_t)((i / R - 1) & 1), abort_flag)) {
+      if constexpr (L::RAW) {
+        const int s = i % RSLOTS;
+        if (i >= RSLOTS && !tc_wait_warp(bar(&sh.rempty[op][s]), (uint32_t)((i / RSLOTS - 1) & 1), abort_flag)) {
           ok = false;
           break;
         }
         const uint32_t full = bar(&sh.rfull[op][s]);
-        const uint32_t dst = sbase + L::OFF_RAW + (uint32_t)(op * RSLOTS + s) * L::RAWB;
-        ptx::mbar_arrive_expect_tx_if(full, L::RAWB, lane == 0);
-        __syncwarp();
-        ptx::tma_g2s_4d_if(dst + ((uint32_t)lane << tbs) * RB, map, 0, c1, w.h, page, full, pol, lane < boxes);
+        fill(sbase + L::OFF_RAW + (uint32_t)(op * RSLOTS + s) * L::RAWB, full, L::RAWB, t, page);
         const uint32_t *meta = op ? a.vm : a.km;
         const uint32_t md = sbase + L::OFF_META + (uint32_t)(op * RSLOTS + s) * L::METAB;
 #pragma unroll
         for (int k = 0; k < kTcHalf / 32; ++k) {
           const int rr = lane + 32 * k, tok = t + rr;
           const int pg = __shfl_sync(0xffffffffu, page, rr >> tbs);
-          long long row;
-          if (paged) {
-            const long long tl = tok & ((1 << bts) - 1), base = ((long long)pg * a.cache.Hkv) << bts;
-            row = a.cache.head_major ? base + ((long long)w.h << bts) + tl : base + tl * a.cache.Hkv + w.h;
-          } else {
-            row = a.cache.head_major ? ((long long)w.b * a.cache.Hkv + w.h) * a.cache.n + tok
-                                     : ((long long)w.b * a.cache.n + tok) * a.cache.Hkv + w.h;
-          }
+          const unsigned row = (unsigned)pg * pstep + (unsigned)(tok & bmask) * tstep + hoff;
           const bool there = tok < w.t1 && pg >= 0;
-          const uint32_t *src = there ? meta + row * a.gpr : meta;
+          const uint32_t *src = there ? meta + (size_t)row * a.gpr : meta;
           const uint32_t d = md + (uint32_t)(rr * a.gpr * 4);
           if (a.gpr == 1)
             ptx::cp_async_4_zfill(d, src, there ? 4u : 0u);
@@ -757,14 +775,10 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
           ok = false;
           break;
         }
-        const uint32_t full = bar(!op ? &sh.kfull[s] : i < first_masked ? &sh.vfull[s] : &sh.vraw[s]);
-        const int blk = lane / boxes;  // 64-channel block of this lane's box
-        ptx::mbar_arrive_expect_tx_if(full, TILE, lane == 0);
-        __syncwarp();
-        ptx::tma_g2s_4d_if((op ? svr : skr) + s * TILE + blk * BLK + ((uint32_t)(lane % boxes) << tbs) * 128u, map,
-                           128 * blk, c1, w.h, page, full, pol, lane < boxes * KB);
+        fill((op ? svr : skr) + s * TILE, bar(!op ? &sh.kfull[s] : i < first_masked ? &sh.vfull[s] : &sh.vraw[s]), TILE, t,
+             page);
       }
-      page = next;
+      page = page_of(i + 1);
     }
     if (!ok && lane == 0) {
       atomicOr(&g_kvfb_chunk_error, 1u);
