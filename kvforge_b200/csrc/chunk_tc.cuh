@@ -23,9 +23,8 @@
 //          neither waits on the other's weights: S = Q K^T into tensor memory, O += P V
 //          with P read from tensor memory, where the softmax group writes it over its
 //          scores, and V read MN-major. The other two are the producers of K and of V:
-//          TMA boxes per page, metadata rows by cp.async. A box of tokens that nobody
-//          sees, or of a block mapped to a negative page, is asked for at page -1,
-//          which TMA fills with zeros.
+//          TMA boxes per page. A box of tokens that nobody sees, or of a block mapped
+//          to a negative page, is asked for at page -1, which TMA fills with zeros.
 // The running maximum a row's weights are taken against is raised only when 64
 // of them add up to more than 256 (weights up to that fit fp16, and their sum
 // fp32), so the output in tensor memory is rescaled rarely, a step's scores are
@@ -115,7 +114,7 @@ template <bool RAW, bool TWO> __device__ __forceinline__ uint32_t tc_bar_count(i
          : i < 36 ? 4u                // vfixed
          : i < 37 ? (TWO ? 8u : 4u)   // qready: the warps that load queries
          : i < 38 ? 2u                // done: both issuers
-         : i < 54 ? 33u               // rfull: the boxes' bytes, and 32 lanes of cp.async
+         : i < 54 ? 1u                // rfull: the boxes' bytes
                   : 4u;               // rempty: converter warps
 }
 static_assert(sizeof(TcShared) <= 1024, "misc area");
@@ -564,6 +563,43 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
       const int ch = lt % CPR, r0 = lt / CPR;
       const int gword = (ch * (16 * D / RB)) >> a.group_shift;  // metadata word of the piece
       const uint32_t ring = op ? svr : skr;
+      // Metadata rows: a warp fetches those of the 16 rows that it converts itself,
+      // one to a lane, RSLOTS halves ahead (cp.async into its own part of the slot's
+      // area), so nobody else has to be told. The page of the half after is looked
+      // up one half earlier. Row numbers fit 32 bits: fewer rows fit a GPU.
+      constexpr int WR = 32 / CPR;                 // adjacent rows of a warp
+      const bool paged = a.cache.paged != 0;
+      const int bts = paged ? a.cache.bt_shift : 30, bmask = (1 << bts) - 1;
+      const unsigned heads = (unsigned)a.cache.Hkv, hd = (unsigned)w.h;
+      const unsigned pstep = paged ? heads << bts : heads * (unsigned)a.cache.n;
+      const unsigned tstep = a.cache.head_major ? 1u : heads;
+      const unsigned hoff = !a.cache.head_major ? hd : paged ? hd << bts : hd * (unsigned)a.cache.n;
+      const int *table = paged ? a.cache.table + (long long)w.b * a.cache.max_blocks : nullptr;
+      const uint32_t *mcache = op ? a.vm : a.km;
+      const int mrow = lane < 16 ? (lane / WR) * RPP + (lt >> 5) * WR + lane % WR : 0;  // row of the half
+      auto page_of = [&](int i) -> int {
+        const int t = w.t0 + i * kTcHalf + mrow;
+        if (i >= 2 * n || t >= w.t1) return -1;
+        return paged ? __ldg(table + (t >> bts)) : w.b;
+      };
+      auto fetch_meta = [&](int i, int page) {     // half i into its slot
+        if (i < 2 * n && lane < 16) {
+          const int t = w.t0 + i * kTcHalf + mrow;
+          const bool there = page >= 0;            // else zeros
+          const unsigned row = (unsigned)page * pstep + (unsigned)(t & bmask) * tstep + hoff;
+          const uint32_t *src = there ? mcache + (size_t)row * a.gpr : mcache;
+          const uint32_t d = sbase + L::OFF_META + (uint32_t)(op * RSLOTS + i % RSLOTS) * L::METAB + (uint32_t)(mrow * a.gpr * 4);
+          if (a.gpr == 1)
+            ptx::cp_async_4_zfill(d, src, there ? 4u : 0u);
+          else if (a.gpr == 2)
+            ptx::cp_async_8_zfill(d, src, there ? 8u : 0u);
+          else
+            ptx::cp_async_16_zfill(d, src, there ? 16u : 0u);
+        }
+        ptx::cp_async_commit();
+      };
+      for (int i = 0; i < RSLOTS; ++i) fetch_meta(i, page_of(i));
+      int page = page_of(RSLOTS);
       for (int i = 0; i < 2 * n; ++i) {
         const int rs = i % RSLOTS, s = (i >> 1) % SLOTS, use = (i >> 1) / SLOTS;
         const bool masked = op && (i >> 1) >= first_masked;
@@ -575,7 +611,8 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
         }
         const uint32_t raw = sbase + L::OFF_RAW + (uint32_t)(op * RSLOTS + rs) * L::RAWB;
         const uint32_t meta = sbase + L::OFF_META + (uint32_t)(op * RSLOTS + rs) * L::METAB;
-        const int tok = w.t0 + i * kTcHalf;
+        ptx::cp_async_wait<RSLOTS - 1>();
+        __syncwarp();
         // All pieces of the half first, so that their loads overlap.
         constexpr int N = CPR / 2;
         uint32_t in[N][4], sz[N];
@@ -592,7 +629,7 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
 #pragma unroll
         for (int k = 0; k < N; ++k) {
           const int rr = r0 + k * RPP;
-          if (tok + rr >= w.t1) sz[k] = 0u;        // a row that nobody sees: zeros, whatever its page holds
+          // (a row that nobody sees has zero metadata: zeros, whatever its page holds)
           const uint32_t s2 = ptx::prmt(sz[k], sz[k], 0x1010), z2 = ptx::prmt(sz[k], sz[k], 0x3232);
           uint32_t o[4 * P16];
           if (FMT == KVF_FMT_INT8) {
@@ -649,6 +686,7 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
                          : "memory");
           }
         }
+        const int next = page_of(i + RSLOTS + 1);
         if (i & 1) {
           if (odd) *reinterpret_cast<volatile int *>(&sh.odd) = 1;
           ptx::fence_proxy_async_smem();
@@ -656,7 +694,10 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
         __syncwarp();
         ptx::mbar_arrive_if(bar(&sh.rempty[op][rs]), lane == 0);
         if (i & 1) ptx::mbar_arrive_if(bar(op ? &sh.vfull[s] : &sh.kfull[s]), lane == 0);
+        fetch_meta(i + RSLOTS, page);
+        page = next;
       }
+      ptx::cp_async_wait<0>();
     } else {
       for (int i = first_masked; i < n; ++i) {
         const int s = i % SLOTS;
@@ -734,11 +775,6 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
         }
       }
     };
-    // Metadata row of token tok in a page (or sequence) of 2^32 rows at most: fewer fit a GPU.
-    const unsigned heads = (unsigned)a.cache.Hkv, hd = (unsigned)w.h;
-    const unsigned pstep = paged ? heads << bts : heads * (unsigned)a.cache.n;
-    const unsigned tstep = a.cache.head_major ? 1u : heads;
-    const unsigned hoff = !a.cache.head_major ? hd : paged ? hd << bts : hd * (unsigned)a.cache.n;
     bool ok = true;
     int page = page_of(0), i = 0;
     for (; i < count; ++i) {
@@ -749,26 +785,7 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
           ok = false;
           break;
         }
-        const uint32_t full = bar(&sh.rfull[op][s]);
-        fill(sbase + L::OFF_RAW + (uint32_t)(op * RSLOTS + s) * L::RAWB, full, L::RAWB, t, page);
-        const uint32_t *meta = op ? a.vm : a.km;
-        const uint32_t md = sbase + L::OFF_META + (uint32_t)(op * RSLOTS + s) * L::METAB;
-#pragma unroll
-        for (int k = 0; k < kTcHalf / 32; ++k) {
-          const int rr = lane + 32 * k, tok = t + rr;
-          const int pg = __shfl_sync(0xffffffffu, page, rr >> tbs);
-          const unsigned row = (unsigned)pg * pstep + (unsigned)(tok & bmask) * tstep + hoff;
-          const bool there = tok < w.t1 && pg >= 0;
-          const uint32_t *src = there ? meta + (size_t)row * a.gpr : meta;
-          const uint32_t d = md + (uint32_t)(rr * a.gpr * 4);
-          if (a.gpr == 1)
-            ptx::cp_async_4_zfill(d, src, there ? 4u : 0u);
-          else if (a.gpr == 2)
-            ptx::cp_async_8_zfill(d, src, there ? 8u : 0u);
-          else
-            ptx::cp_async_16_zfill(d, src, there ? 16u : 0u);
-        }
-        ptx::cp_async_arrive(full);
+        fill(sbase + L::OFF_RAW + (uint32_t)(op * RSLOTS + s) * L::RAWB, bar(&sh.rfull[op][s]), L::RAWB, t, page);
       } else {
         const int s = i % SLOTS;
         if (i >= SLOTS && !tc_wait_warp(bar(op ? &sh.vempty[s] : &sh.kempty[s]), (uint32_t)((i / SLOTS - 1) & 1), abort_flag)) {
