@@ -275,19 +275,22 @@ def _launch(fn: str, device: torch.device, stream, *args) -> None:
     if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):
             return _launch(fn, device, stream, *args)
-    s = stream if stream is not None else torch.cuda.current_stream(device)
-    check(fn, getattr(lib(), fn)(*args, s.cuda_stream))
+    # the handle itself: building a torch.cuda.Stream takes as long as a launch
+    s = torch._C._cuda_getCurrentRawStream(device.index) if stream is None else stream.cuda_stream
+    check(fn, getattr(lib(), fn)(*args, s))
 
 
 def _heads(x: torch.Tensor, what: str, device: torch.device, shape=None) -> KvfHeads:
-    if x.dim() != 4 or (shape is not None and tuple(x.shape) != tuple(shape)):
+    size = x.shape
+    if len(size) != 4 or (shape is not None and size != shape):
         raise ValueError(f"{what} must be [B][T][heads][D]" + (f" = {tuple(shape)}" if shape is not None else ""))
-    if x.dtype not in DTYPES or x.device != device or not x.is_cuda:
+    dtype = DTYPES.get(x.dtype)
+    if dtype is None or x.device != device or not x.is_cuda:
         raise ValueError(f"{what} must be float32, float16 or bfloat16 on {device}")
-    st = x.stride()
-    if st[3] != 1 and x.shape[3] > 1:
+    sb, st, sh, sc = x.stride()
+    if sc != 1 and size[3] > 1:
         raise ValueError(f"{what}: the channels of a head must be adjacent")
-    return KvfHeads(x.data_ptr(), DTYPES[x.dtype], x.shape[2], st[0], st[1], st[2])
+    return KvfHeads(x.data_ptr(), dtype, size[2], sb, st, sh)
 
 
 def _per_sequence(x: Optional[torch.Tensor], what: str, B: int, device: torch.device) -> Optional[int]:

@@ -53,6 +53,11 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], 
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
 
+__device__ __forceinline__ void put8(float *p, const float (&x)[8]) {
+  reinterpret_cast<float4 *>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+  reinterpret_cast<float4 *>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+}
+
 template <int FMT, int DT, int D>
 __global__ void __launch_bounds__(kChunkThreads) chunk_mma_kernel(const ChunkArgs a) {
   constexpr int QS = D + 8, KS = D + 8, VS = D + 4;
@@ -69,8 +74,7 @@ __global__ void __launch_bounds__(kChunkThreads) chunk_mma_kernel(const ChunkArg
     const int r = i / (D / 8), li = i % (D / 8);
     float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (r < w.rows) load8<DT>(chunk_row(a.q, a, w, r) + 8 * li * dtype_bytes(DT), a.q.vec, x);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) sq[r * QS + 8 * li + k] = x[k];
+    put8(sq + r * QS + 8 * li, x);
   }
 
   const int r_lo = warp * 16 + g4, r_hi = r_lo + 8;
@@ -88,6 +92,7 @@ __global__ void __launch_bounds__(kChunkThreads) chunk_mma_kernel(const ChunkArg
     if (tid == 0) *odd = 0;
     __syncthreads();
     const bool masked = t + kChunkTokens > w.seen0;  // some row of the tile does not see all of the step
+#pragma unroll 4
     for (int i = tid; i < kChunkTokens * (D / 8); i += kChunkThreads) {
       const int r = i / (D / 8), li = i % (D / 8);
       float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -97,11 +102,12 @@ __global__ void __launch_bounds__(kChunkThreads) chunk_mma_kernel(const ChunkArg
         cache8<FMT, D>(a.k, a.km, a, row, li, x);
         cache8<FMT, D>(a.v, a.vm, a, row, li, y);
       }
+      put8(sk + r * KS + 8 * li, x);
+      put8(sv + r * VS + 8 * li, y);
+      if (masked) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        sk[r * KS + 8 * li + k] = x[k];
-        sv[r * VS + 8 * li + k] = y[k];
-        if (masked && !(fabsf(y[k]) < INFINITY)) *odd = 1;
+        for (int k = 0; k < 8; ++k)
+          if (!(fabsf(y[k]) < INFINITY)) *odd = 1;
       }
     }
     __syncthreads();
