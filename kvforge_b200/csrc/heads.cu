@@ -50,6 +50,7 @@ struct HeadsArgs {
   uint8_t *kd, *vd;
   void *km, *vm;
   int fmt, group;
+  int paired;            // queries go by paired_rows
 };
 
 __device__ __forceinline__ void load_weight8(const Norm &n, int li, float (&w)[8]) {
@@ -63,13 +64,132 @@ __device__ __forceinline__ void load_weight8(const Norm &n, int li, float (&w)[8
     load8<KVF_DT_BF16>(p, vec, w);
 }
 
+// Four channels as they lie in memory (8- or 16-byte aligned), and their values.
+template <int DT> struct Raw4 {
+  uint32_t a[DT == KVF_DT_F32 ? 4 : 2];
+};
+template <int DT> __device__ __forceinline__ Raw4<DT> load_raw4(const void *p) {
+  Raw4<DT> r;
+  if constexpr (DT == KVF_DT_F32) {
+    const uint4 x = __ldcs(reinterpret_cast<const uint4 *>(p));
+    r.a[0] = x.x; r.a[1] = x.y; r.a[2] = x.z; r.a[3] = x.w;
+  } else {
+    const uint2 x = __ldcs(reinterpret_cast<const uint2 *>(p));
+    r.a[0] = x.x; r.a[1] = x.y;
+  }
+  return r;
+}
+template <int DT> __device__ __forceinline__ void values4(const Raw4<DT> &r, float *e) {
+  if constexpr (DT == KVF_DT_F32) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) e[k] = __uint_as_float(r.a[k]);
+  } else {
+    const float2 x = widen2<DT>(r.a[0]), y = widen2<DT>(r.a[1]);
+    e[0] = x.x; e[1] = x.y; e[2] = y.x; e[3] = y.y;
+  }
+}
+template <int DT> __device__ __forceinline__ void store4(void *p, const float *e) {
+  if constexpr (DT == KVF_DT_F32)
+    *reinterpret_cast<float4 *>(p) = make_float4(e[0], e[1], e[2], e[3]);
+  else
+    *reinterpret_cast<uint2 *>(p) = make_uint2(narrow2<DT>(e[0], e[1]), narrow2<DT>(e[2], e[3]));
+}
+
+// Query rows whose whole width turns in half-split pairs: a lane holds channels
+// 4 li .. 4 li + 3 of both halves, so that a pair is one lane's and the rotation
+// needs no shuffles (of which the other layout has eight a row, and the
+// shared-memory pipe that carries them was as busy as the schedulers: 4 x 4001
+// tokens of 64 heads 123 us with them, 88 us without, 81 us at the copy peak). The sum of squares keeps its tree: four
+// channels in the lane, neighbours by lane, the halves last.
+template <int DT, int D, int R>
+__device__ __forceinline__ void paired_rows(const HeadsArgs &a, int b, int j, long long t, int r0, int li) {
+  constexpr int LPR = D / 8, RPW = 32 / LPR, E = DT == KVF_DT_F32 ? 4 : 2;
+  const int lane = threadIdx.x & 31;
+  Raw4<DT> lo[R], hi[R];
+  const uint8_t *in = a.q.p + b * a.q.sb + j * a.q.st + 4 * li * E;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const uint8_t *p = in + min(r0 + i * RPW, a.q.heads - 1) * a.q.sh;
+    lo[i] = load_raw4<DT>(p);
+    hi[i] = load_raw4<DT>(p + (D / 2) * E);
+  }
+  const float4 c4 = *reinterpret_cast<const float4 *>(a.cos + t * (D / 2) + 4 * li);
+  const float4 s4 = *reinterpret_cast<const float4 *>(a.sin + t * (D / 2) + 4 * li);
+  const float cs[4] = {c4.x, c4.y, c4.z, c4.w}, sn[4] = {s4.x, s4.y, s4.z, s4.w};
+  const bool normed = a.qn.w != nullptr;
+  float root = 0.f, w[8];
+  if (normed) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int c = (k >> 2) * (D / 2) + 4 * li + (k & 3);
+      w[k] = a.qn.dtype == KVF_DT_F32   ? __ldg(reinterpret_cast<const float *>(a.qn.w) + c)
+             : a.qn.dtype == KVF_DT_F16 ? __half2float(__ldg(reinterpret_cast<const __half *>(a.qn.w) + c))
+                                        : __bfloat162float(__ldg(reinterpret_cast<const __nv_bfloat16 *>(a.qn.w) + c));
+    }
+    const bool odd = li & 1;
+    float mine = 0.f;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      float s[8];
+      values4<DT>(lo[i], s);
+      values4<DT>(hi[i], s + 4);
+#pragma unroll
+      for (int k = 0; k < 8; k += 2) mul2(s[k], s[k + 1], s[k], s[k + 1], s[k], s[k + 1]);
+      const float x = __fadd_rn(__fadd_rn(s[0], s[1]), __fadd_rn(s[2], s[3]));
+      const float y = __fadd_rn(__fadd_rn(s[4], s[5]), __fadd_rn(s[6], s[7]));
+      // even lanes go on with the lower half's sum, odd ones with the upper's
+      float sum = __fadd_rn(odd ? y : x, __shfl_xor_sync(0xffffffffu, odd ? x : y, 1));
+#pragma unroll
+      for (int off = 2; off < LPR; off <<= 1) sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, off));
+      sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, 1));
+      mine = i == 0 || li % R == i ? sum : mine;
+    }
+    root = __fdiv_rn(1.f, __fsqrt_rn(__fadd_rn(__fmul_rn(mine, 1.f / D), a.qn.eps)));
+  }
+  uint8_t *out = a.q_out.p + b * a.q_out.sb + j * a.q_out.st + 4 * li * E;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int r = r0 + i * RPW;
+    float x[4], y[4], u[4], v[4];
+    values4<DT>(lo[i], x);
+    values4<DT>(hi[i], y);
+    if (normed) {
+      const float inv = R == 1 ? root : __shfl_sync(0xffffffffu, root, (lane & ~(LPR - 1)) + i);
+#pragma unroll
+      for (int k = 0; k < 4; k += 2) {
+        mul2(x[k], x[k + 1], x[k], x[k + 1], inv, inv);
+        mul2(x[k], x[k + 1], x[k], x[k + 1], w[k], w[k + 1]);
+        mul2(y[k], y[k + 1], y[k], y[k + 1], inv, inv);
+        mul2(y[k], y[k + 1], y[k], y[k + 1], w[4 + k], w[5 + k]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; k += 2) {
+      // scalar sums: a packed one may be contracted with its products
+      float p0, p1, q0, q1;
+      mul2(p0, p1, x[k], x[k + 1], cs[k], cs[k + 1]);
+      mul2(q0, q1, y[k], y[k + 1], sn[k], sn[k + 1]);
+      u[k] = __fsub_rn(p0, q0);
+      u[k + 1] = __fsub_rn(p1, q1);
+      mul2(p0, p1, x[k], x[k + 1], sn[k], sn[k + 1]);
+      mul2(q0, q1, y[k], y[k + 1], cs[k], cs[k + 1]);
+      v[k] = __fadd_rn(p0, q0);
+      v[k + 1] = __fadd_rn(p1, q1);
+    }
+    if (r < a.q.heads) {
+      store4<DT>(out + r * a.q_out.sh, u);
+      store4<DT>(out + r * a.q_out.sh + (D / 2) * E, v);
+    }
+  }
+}
+
 // One warp takes up to R * (32 / (D / 8)) head vectors of one token and of one
 // kind (queries, keys or values), R per group of D / 8 lanes: its weight and the
 // token's angles are read once for R rows, R loads are in flight per lane, and
 // the R roots are taken by R lanes at once. CACHE: keys and values are part of
 // the call.
 template <int DT, int D, int R, bool CACHE>
-__global__ void __launch_bounds__(256, 4) heads_kernel(const HeadsArgs a) {
+__global__ void __launch_bounds__(256, CACHE ? 5 : 3) heads_kernel(const HeadsArgs a) {
   constexpr int LPR = D / 8;     // lanes per row
   constexpr int RPW = 32 / LPR;  // rows per warp at a time
   const int lane = threadIdx.x & 31;
@@ -93,6 +213,13 @@ __global__ void __launch_bounds__(256, 4) heads_kernel(const HeadsArgs a) {
   const int r0 = unit * (R * RPW) + lane / LPR;
   const long long t = a.pos ? (long long)a.pos[b] + j : j;
   const bool bad_pos = t < 0 || (a.rot && t >= a.positions);
+  if (a.paired && kind == 0) {
+    if (!bad_pos)
+      paired_rows<DT, D, R>(a, b, j, t, r0, li);
+    else if (lane == 0)
+      atomicOr(&g_kvfb_heads_error, 1u);
+    return;
+  }
 
   // Rows stay as they lie in memory until they are worked on: R of them in
   // flight take 4 R registers (8 R for fp32).
@@ -238,28 +365,35 @@ template <int DT, int D>
 cudaError_t launch_heads(HeadsArgs a, cudaStream_t st) {
   constexpr int RPW = 32 / (D / 8);
   const long long tokens = (long long)a.B * a.T;
-  // Several rows per lane group where that still gives every SM some 32 warps; one
-  // in short calls, whose time is that of one row.
-  constexpr int R = DT == KVF_DT_F32 ? 2 : 4;
-  const long long pairs = (a.q.heads + RPW - 1) / RPW + (a.k.heads + RPW - 1) / RPW + (a.v.heads + RPW - 1) / RPW;
-  const int r = tokens * pairs >= R * 148 * 32 ? R : 1;
-  a.q_units = (a.q.heads + r * RPW - 1) / (r * RPW);
-  a.k_units = (a.k.heads + r * RPW - 1) / (r * RPW);
-  a.units = a.q_units + a.k_units + (a.v.heads + r * RPW - 1) / (r * RPW);
+  a.paired = a.q.heads && a.rot == D && !a.interleaved && a.q.vec && a.q_out.vec;
+  // Rows per lane group. One in short calls, whose time is that of one row; more
+  // where that still gives every SM some 32 warps. Queries alone: eight (four of
+  // fp32), if a token's heads fill three quarters of such units (4 x 4001 tokens of
+  // 64 heads: 88 us with eight, 97 with four, 129 with two). With keys and values
+  // the quantizer needs the registers: two (8 ragged chunks of 2048 tokens into
+  // int8: 111 us with two, 123 with four, 148 with eight).
+  constexpr int BIG = DT == KVF_DT_F32 ? 4 : 8;
+  const bool cache = a.k.heads > 0;
+  auto units = [](int heads, int r) { return (heads + r * RPW - 1) / (r * RPW); };
+  const long long pairs = units(a.q.heads, 1) + units(a.k.heads, 1) + units(a.v.heads, 1);
+  int r = tokens * pairs >= 2 * 148 * 32 ? 2 : 1;
+  if (!cache && tokens * pairs >= BIG * 148 * 32 && 4 * a.q.heads >= 3 * units(a.q.heads, BIG) * BIG * RPW) r = BIG;
+  a.q_units = units(a.q.heads, r);
+  a.k_units = units(a.k.heads, r);
+  a.units = a.q_units + a.k_units + units(a.v.heads, r);
   const long long warps = tokens * a.units;
   if (warps > 0xffffffffLL - 8) return cudaErrorInvalidValue;
   const unsigned blocks = (unsigned)((warps + 7) / 8);
-  if (a.k.heads == 0) {
-    if (r == R)
-      heads_kernel<DT, D, R, false><<<blocks, 256, 0, st>>>(a);
-    else
-      heads_kernel<DT, D, 1, false><<<blocks, 256, 0, st>>>(a);
-  } else {
-    if (r == R)
-      heads_kernel<DT, D, R, true><<<blocks, 256, 0, st>>>(a);
-    else
-      heads_kernel<DT, D, 1, true><<<blocks, 256, 0, st>>>(a);
-  }
+  if (cache && r == 2)
+    heads_kernel<DT, D, 2, true><<<blocks, 256, 0, st>>>(a);
+  else if (cache)
+    heads_kernel<DT, D, 1, true><<<blocks, 256, 0, st>>>(a);
+  else if (r == BIG)
+    heads_kernel<DT, D, BIG, false><<<blocks, 256, 0, st>>>(a);
+  else if (r == 2)
+    heads_kernel<DT, D, 2, false><<<blocks, 256, 0, st>>>(a);
+  else
+    heads_kernel<DT, D, 1, false><<<blocks, 256, 0, st>>>(a);
   return cudaGetLastError();
 }
 
@@ -393,12 +527,24 @@ __global__ void __launch_bounds__(256) gather_kernel(const GatherArgs a) {
 
 template <int FMT, int DT, int D>
 cudaError_t launch_gather(GatherArgs a, cudaStream_t st) {
-  constexpr int RPW = 32 / (D / 8), R = 4;
-  a.units = (2 * a.k.heads + R * RPW - 1) / (R * RPW);
+  // Rows per lane group: as many as keep three quarters of the lanes busy, four,
+  // or eight of the short int4 rows (65536 tokens of 8 heads: 72 us with eight,
+  // 79 with four; a ragged f16 batch 62 us with four, 65 with eight).
+  constexpr int RPW = 32 / (D / 8), BIG = FMT == KVF_FMT_INT4 ? 8 : 4;
+  const int rows = 2 * a.k.heads;
+  auto units = [&](int r) { return (rows + r * RPW - 1) / (r * RPW); };
+  auto full = [&](int r) { return 4 * rows >= 3 * units(r) * r * RPW; };
+  const int r = full(BIG) ? BIG : full(2) ? 2 : 1;
+  a.units = units(r);
   const long long warps = (long long)a.B * a.T * a.units;
   if (warps > 0xffffffffLL - 8) return cudaErrorInvalidValue;
-  const long long blocks = (warps + 7) / 8;
-  gather_kernel<FMT, DT, D, R><<<(unsigned)blocks, 256, 0, st>>>(a);
+  const unsigned blocks = (unsigned)((warps + 7) / 8);
+  if (r == BIG)
+    gather_kernel<FMT, DT, D, BIG><<<blocks, 256, 0, st>>>(a);
+  else if (r == 2)
+    gather_kernel<FMT, DT, D, 2><<<blocks, 256, 0, st>>>(a);
+  else
+    gather_kernel<FMT, DT, D, 1><<<blocks, 256, 0, st>>>(a);
   return cudaGetLastError();
 }
 

@@ -336,6 +336,75 @@ def test_gather_stops_at_lengths_and_reports_tokens_without_a_row(cuda):
     assert torch.equal(out[1][0], K[0, :, :5].transpose(0, 1).half().to(torch.bfloat16))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d,H,interleaved", [(128, 64, False), (128, 61, True), (64, 64, False), (64, 20, False), (128, 3, False)])
+def test_long_calls_match_short_ones(cuda, dtype, d, H, interleaved):
+    """Enough tokens for several rows per lane, against calls of few tokens and the fp32 operations."""
+    g = _gen(cuda, 14)
+    B, T = 2, 1300
+    rope = api.Rope.build(T + 10, d, interleaved=interleaved, device=cuda)
+    w = 1 + 0.1 * _randn((d,), g)
+    pos = torch.tensor([7, 0], dtype=torch.int32, device=cuda)
+    x = _randn((B, T, H, d), g, dtype)
+    got = api.norm_rope(x, pos, rope, weight=w, eps=EPS)
+    assert torch.equal(got, _fp32(x, pos, rope, w).to(dtype))
+    at = pos + 1000
+    assert torch.equal(got[:, 1000:1003], api.norm_rope(x[:, 1000:1003], at, rope, weight=w, eps=EPS))
+    odd = torch.zeros((B, T, H * d + 1), dtype=dtype, device=cuda)[..., 1:].unflatten(-1, (H, d))
+    assert torch.equal(got, api.norm_rope(x, pos, rope, weight=w, eps=EPS, out=odd))  # rows off 16-byte boundaries
+    assert api.device_errors() == 0
+
+
+@pytest.mark.parametrize("fmt,group,d", [(FMT_F16, 0, 128), (FMT_INT8, 64, 128), (FMT_INT4, 32, 128), (FMT_INT4, 32, 64)])
+@pytest.mark.parametrize("Hkv", [1, 2, 8, 11])
+def test_long_append_and_gather(cuda, fmt, group, d, Hkv):
+    g = _gen(cuda, 15)
+    B, T, n = 2, 1200, 1300
+    place = Placement(ORD_TOKEN, True, 16)
+    cache = _empty_cache(cuda, B, Hkv, n, d, fmt, group, place)
+    k, v = (_randn((B, T, Hkv, d), g, torch.bfloat16) for _ in range(2))
+    q = _randn((B, T, 4 * Hkv, d), g, torch.bfloat16)
+    rope = api.Rope.build(n, d, device=cuda)
+    pos = torch.tensor([100, 3], dtype=torch.int32, device=cuda)
+    out = api.append_rope(cache, k, v, rope, pos=pos, q=q)
+    assert torch.equal(out, _fp32(q, pos, rope, None).to(q.dtype))
+    got = api.gather(cache, T, pos=pos)
+    for x, y in zip((_fp32(k, pos, rope, None), v.float()), got):
+        data, meta = api.quantize(x.contiguous(), fmt, group)
+        one = api.KVCache(fmt=fmt, d=d, group=group, place=Placement(ORD_TOKEN, False, 0), B=B, Hkv=Hkv, n=T, k=data, v=data,
+                          k_meta=meta, v_meta=meta, block_table=None, max_blocks=0, seq_lens=None)
+        assert torch.equal(y, api.gather(one, T)[0])
+    assert api.device_errors() == 0
+
+
+def test_offsets_past_32_bits(cuda):
+    """Pages far into a pool of more than 4 GB: payload and metadata offsets need 64 bits."""
+    g = _gen(cuda, 16)
+    B, T, Hkv, n, d, pages = 1, 20, 2, 32, 128, 1_100_000
+    for fmt, group in ((FMT_INT8, 64), (FMT_F16, 0)):
+        pages = 1_100_000 if fmt == FMT_INT8 else 600_000
+        rows = pages * Hkv * 16
+        k, v = (torch.zeros((rows, api.row_bytes(fmt, d)), dtype=torch.uint8, device=cuda) for _ in range(2))
+        assert k.numel() > 2 ** 32
+        km, vm = (torch.zeros((rows, 2), dtype=torch.int32, device=cuda) if group else None for _ in range(2))
+        table = torch.tensor([[pages - 1, pages - 3]], dtype=torch.int32, device=cuda)
+        cache = api.KVCache(fmt=fmt, d=d, group=group, place=Placement(ORD_TOKEN, True, 16), B=B, Hkv=Hkv, n=n, k=k, v=v,
+                            k_meta=km, v_meta=vm, block_table=table, max_blocks=2,
+                            seq_lens=torch.tensor([T], dtype=torch.int32, device=cuda))
+        kn, vn = (_randn((B, T, Hkv, d), g, torch.bfloat16) for _ in range(2))
+        api.append_rope(cache, kn, vn, pos=torch.zeros(B, dtype=torch.int32, device=cuda))
+        small = _empty_cache(cuda, B, Hkv, n, d, fmt, group, Placement(ORD_TOKEN, False, 0),
+                             seq_lens=np.array([T], dtype=np.int32))
+        api.append_rope(small, kn, vn, pos=torch.zeros(B, dtype=torch.int32, device=cuda))
+        for x, y in zip(api.gather(cache, T), api.gather(small, T)):
+            assert torch.equal(x, y) and bool(x.any())
+        for dtype in (torch.bfloat16, torch.float32):
+            q = _randn((B, T, 8, d), g, dtype)
+            assert torch.equal(api.chunk_attention(q, cache), api.chunk_attention(q, small))
+        assert api.device_errors() == 0
+        del k, v, km, vm, cache
+
+
 def test_heads_on_another_stream_and_in_a_graph(cuda):
     g = _gen(cuda, 12)
     B, T, H, Hkv, n, d = 2, 3, 4, 2, 32, 128
