@@ -502,10 +502,8 @@ def chunk_attention(q: torch.Tensor, cache: KVCache, *, q_lens: Optional[torch.T
     if lse is not None:
         a.lse = lse.data_ptr()
     if workspace is None and B * T:
-        workspace = ChunkWorkspace.allocate(cache, T, H, q.dtype)
-        if stream is not None and workspace.part_o is not None:
-            workspace.part_o.record_stream(stream)
-            workspace.part_ml.record_stream(stream)
+        with torch.cuda.stream(stream):  # memory of the stream that uses it
+            workspace = ChunkWorkspace.allocate(cache, T, H, q.dtype)
     a.splits = workspace.splits if workspace is not None else 1
     if a.splits > 1:
         for x, e in ((workspace.part_o, d), (workspace.part_ml, 2)):

@@ -205,7 +205,7 @@ extern "C" cudaError_t kvf_b200_chunk_attention(const kvf_args *args, int fmt, i
   a.splits = args->splits;
   a.part_o = args->part_o;
   a.part_ml = args->part_ml;
-  if ((long long)T * a.g > (1LL << 30)) return cudaErrorInvalidValue;
+  if ((long long)T * a.g > (1LL << 30) || args->n > (1 << 30)) return cudaErrorInvalidValue;
   if (q->dtype == KVF_DT_F32) {
     void *fn = fmt == KVF_FMT_F16    ? mma_fn<KVF_FMT_F16>(d)
                : fmt == KVF_FMT_INT8 ? mma_fn<KVF_FMT_INT8>(d)

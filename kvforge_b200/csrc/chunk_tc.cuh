@@ -441,10 +441,11 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
       else if (a.lse)
         a.lse[at] = none ? -INFINITY : m + log2f(l);
     }
-    // 32 columns at a time through the warp's part of the query tile, which no MMA
-    // reads any more (without TWO group 1 uses its K tile): threads have rows, stores
-    // take whole rows.
-    const uint32_t stage = (TWO || grp == 0 ? sq + (TWO ? grp * TILE : 0u) : skr + TILE) + (uint32_t)(warp & 3) * 4096u;
+    // 32 columns at a time through shared memory that no MMA reads any more and no
+    // copy will fill: the warp's part of the group's own query tile, or, where both
+    // groups share one, of a K slot that only this group's tiles use. Threads have
+    // rows, stores take whole rows.
+    const uint32_t stage = (TWO ? sq : skr) + grp * TILE + (uint32_t)(warp & 3) * 4096u;
 #pragma unroll 1
     for (int q = 0; q < D / 32; ++q) {
       uint32_t o[32];

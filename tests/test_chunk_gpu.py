@@ -362,3 +362,22 @@ def test_refusals(cuda):
             f()
     assert api.chunk_attention(q[:, :0], cache).numel() == 0
     assert api.device_errors() == 0
+
+
+@pytest.mark.parametrize("fmt,group,d", [(FMT_F16, 0, 128), (FMT_F16, 0, 64), (FMT_INT8, 64, 128), (FMT_INT4, 32, 128)])
+def test_few_rows_over_many_steps(cuda, fmt, group, d):
+    """One row tile taken in turn by both softmax groups, who share its queries: the
+    group that ends first must not disturb the other (uneven numbers of steps,
+    repeated, on every SM at once)."""
+    g = _gen(cuda, 11)
+    B, T, H, Hkv = 40, 4, 32, 4
+    for n in (1, 128, 129, 640, 1153):
+        cache = _cache(cuda, g, B, Hkv, n, d, fmt, group, TOKEN16)
+        q = _randn((B, T, H, d), g, torch.bfloat16)
+        exact = _exact(q, cache, None, True)
+        ws = api.ChunkWorkspace.allocate(cache, T, H, q.dtype, splits=2)
+        first = api.chunk_attention(q, cache, workspace=ws)
+        _check(first, exact, f"n = {n}")
+        for _ in range(20):
+            assert torch.equal(api.chunk_attention(q, cache, workspace=ws), first)
+    assert api.device_errors() == 0

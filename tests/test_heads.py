@@ -97,7 +97,11 @@ def test_chunk_attention_checks():
                dict(a=cache(H=30, splits=1)), dict(a=cache(H=32, splits=0)), dict(a=cache(H=0, splits=1)),
                dict(a=cache(H=32, splits=2)), dict(a=cache(max_blocks=3, **good)), dict(a=cache(k=None, **good)),
                dict(a=cache(group_shift=5, **good)), dict(q=heads(heads=16)), dict(out=heads(heads=32, dtype=1)),
-               dict(out=heads(heads=16)), dict(q=heads(heads=32, p=None)), dict(T=1 << 30)):
+               dict(out=heads(heads=16)), dict(q=heads(heads=32, p=None)), dict(T=1 << 30),
+               dict(a=cache(n=(1 << 30) + 1, max_blocks=1 << 27, **good)), dict(q=heads(heads=32, stride_t=1 << 30)),
+               dict(out=heads(heads=32, stride_h=1 << 30)), dict(a=cache(block_shift=3, **good)),
+               dict(a=cache(block_shift=8, **good)), dict(a=cache(H=8 * 65536, splits=1), q=heads(heads=8 * 65536),
+                                                          out=heads(heads=8 * 65536))):
         assert chunk(**kw) == INVALID, kw
     for kw in (dict(a=cache(v=FAKE + 4, **good)), dict(out=heads(heads=32, p=FAKE + 1)),
                dict(a=cache(H=32, splits=2, part_o=FAKE + 4, part_ml=FAKE))):
