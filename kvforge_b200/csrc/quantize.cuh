@@ -132,14 +132,17 @@ __device__ __forceinline__ GroupScale group_scale8(const float (&e)[8], int li, 
 // code (clamping and rounding to nearest commute: the ends are integers). Otherwise
 // (and for |t| >= 1024, infinities and a zero scale) the exact code() decides;
 // a NaN is code 0 either way. Adding 1.5 * 2^23 leaves the integer in the low bits.
-__device__ __noinline__ void codes8_exact(float x0, float x1, float x2, float x3, float x4, float x5, float x6, float x7,
-                                          float zero, float sc, int levels, uint32_t &lo, uint32_t &hi) {
-  lo = (uint32_t)code(x0, zero, sc, levels) | (uint32_t)code(x1, zero, sc, levels) << 8 |
-       (uint32_t)code(x2, zero, sc, levels) << 16 | (uint32_t)code(x3, zero, sc, levels) << 24;
-  hi = (uint32_t)code(x4, zero, sc, levels) | (uint32_t)code(x5, zero, sc, levels) << 8 |
-       (uint32_t)code(x6, zero, sc, levels) << 16 | (uint32_t)code(x7, zero, sc, levels) << 24;
+__device__ __noinline__ uint2 codes8_exact(float x0, float x1, float x2, float x3, float x4, float x5, float x6, float x7,
+                                           float zero, float sc, int levels) {
+  return make_uint2((uint32_t)code(x0, zero, sc, levels) | (uint32_t)code(x1, zero, sc, levels) << 8 |
+                        (uint32_t)code(x2, zero, sc, levels) << 16 | (uint32_t)code(x3, zero, sc, levels) << 24,
+                    (uint32_t)code(x4, zero, sc, levels) | (uint32_t)code(x5, zero, sc, levels) << 8 |
+                        (uint32_t)code(x6, zero, sc, levels) << 16 | (uint32_t)code(x7, zero, sc, levels) << 24);
 }
-__device__ __forceinline__ void codes8(const float (&e)[8], const GroupScale &g, int levels, uint32_t &lo, uint32_t &hi) {
+// The payload's bytes: eight codes (int8), or four bytes of two codes, the odd
+// channel's above, in x (int4).
+template <int FMT> __device__ __forceinline__ uint2 codes8(const float (&e)[8], const GroupScale &g) {
+  constexpr int levels = FMT == KVF_FMT_INT8 ? 255 : 15;
   const float top = (float)levels, big = 12582912.f;
   float far = 0.f, off = 0.f;
   uint32_t y[8];
@@ -153,26 +156,30 @@ __device__ __forceinline__ void codes8(const float (&e)[8], const GroupScale &g,
     y[k] = __float_as_uint(y0);
     y[k + 1] = __float_as_uint(y1);
   }
-  lo = __byte_perm(__byte_perm(y[0], y[1], 0x0040), __byte_perm(y[2], y[3], 0x0040), 0x5410);
-  hi = __byte_perm(__byte_perm(y[4], y[5], 0x0040), __byte_perm(y[6], y[7], 0x0040), 0x5410);
-  if (!(far < 1024.f && off < 0.5f - 0x1p-12f))
-    codes8_exact(e[0], e[1], e[2], e[3], e[4], e[5], e[6], e[7], g.zero, g.sc, levels, lo, hi);
+  uint2 c;
+  if (FMT == KVF_FMT_INT8)
+    c = make_uint2(__byte_perm(__byte_perm(y[0], y[1], 0x0040), __byte_perm(y[2], y[3], 0x0040), 0x5410),
+                   __byte_perm(__byte_perm(y[4], y[5], 0x0040), __byte_perm(y[6], y[7], 0x0040), 0x5410));
+  else
+    c = make_uint2(__byte_perm(__byte_perm(y[0] + (y[1] << 4), y[2] + (y[3] << 4), 0x0040),
+                               __byte_perm(y[4] + (y[5] << 4), y[6] + (y[7] << 4), 0x0040), 0x5410),
+                   0u);
+  if (!(far < 1024.f && off < 0.5f - 0x1p-12f)) {
+    c = codes8_exact(e[0], e[1], e[2], e[3], e[4], e[5], e[6], e[7], g.zero, g.sc, levels);
+    if (FMT == KVF_FMT_INT4) c.x = __byte_perm(c.x | c.x >> 4, c.y | c.y >> 4, 0x6420);
+  }
+  return c;
 }
 
 // Lane li's eight codes of a row whose payload starts at `row` (8-byte aligned
 // for int8, 4-byte for int4).
 template <int FMT>
 __device__ __forceinline__ void store_codes8(const float (&e)[8], const GroupScale &g, uint8_t *row, int li) {
-  uint32_t lo, hi;
-  codes8(e, g, FMT == KVF_FMT_INT8 ? 255 : 15, lo, hi);
-  if (FMT == KVF_FMT_INT8) {
-    reinterpret_cast<uint2 *>(row)[li] = make_uint2(lo, hi);
-  } else {
-    // bytes 0, 1, 2, 3 hold codes 0 .. 15: neighbours share a byte, the odd one above
-    lo |= lo >> 4;
-    hi |= hi >> 4;
-    reinterpret_cast<uint32_t *>(row)[li] = __byte_perm(lo, hi, 0x6420);
-  }
+  const uint2 c = codes8<FMT>(e, g);
+  if (FMT == KVF_FMT_INT8)
+    reinterpret_cast<uint2 *>(row)[li] = c;
+  else
+    reinterpret_cast<uint32_t *>(row)[li] = c.x;
 }
 
 } // namespace
