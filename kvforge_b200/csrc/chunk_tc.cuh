@@ -716,85 +716,85 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
   } else {
     regs_down<L::LAST_REGS>();
     if (warp == LAST + 1 || warp == LAST + 2) {
-    // ----------------------------------------------------------- producers
-    const int op = warp - LAST - 1;  // 0: K, 1: V
-    const CUtensorMap *map = op ? &tmv : &tmk;
-    if (lane == 0) ptx::prefetch_tmap(map);
-    const uint64_t pol = ptx::policy_evict_last();
-    const bool paged = a.cache.paged != 0;
-    const int bts = paged ? a.cache.bt_shift : 30, bmask = (1 << bts) - 1;
-    const int tbs = min(bts, 6);             // log2 of the tokens of a box
-    const int span = L::RAW ? kTcHalf : kTcStep, boxes = span >> tbs;  // 1 to 8 boxes an item
-    const int count = L::RAW ? 2 * n : n;
-    const int box = lane & (boxes - 1);
-    const int *table = paged ? a.cache.table + (long long)w.b * a.cache.max_blocks : nullptr;
-    // Page (or sequence) of box `box` of item i; -1 where there is nothing to read.
-    auto page_of = [&](int i) -> int {
-      const int t = w.t0 + i * span + (box << tbs);
-      int page = paged ? -1 : w.b;
-      if (i >= count || t >= w.t1) return -1;
-      if (paged) page = __ldg(table + (t >> bts));
-      return page;
-    };
-    // One elected lane issues an item's boxes; coordinates come from the lanes
-    // that hold them.
-    auto fill = [&](uint32_t dst, uint32_t full, uint32_t bytes, int t, int page) {
-      const int my = max(page, -1);
+      // ----------------------------------------------------------- producers
+      const int op = warp - LAST - 1;  // 0: K, 1: V
+      const CUtensorMap *map = op ? &tmv : &tmk;
+      if (lane == 0) ptx::prefetch_tmap(map);
+      const uint64_t pol = ptx::policy_evict_last();
+      const bool paged = a.cache.paged != 0;
+      const int bts = paged ? a.cache.bt_shift : 30, bmask = (1 << bts) - 1;
+      const int tbs = min(bts, 6);             // log2 of the tokens of a box
+      const int span = L::RAW ? kTcHalf : kTcStep, boxes = span >> tbs;  // 1 to 8 boxes an item
+      const int count = L::RAW ? 2 * n : n;
+      const int box = lane & (boxes - 1);
+      const int *table = paged ? a.cache.table + (long long)w.b * a.cache.max_blocks : nullptr;
+      // Page (or sequence) of box `box` of item i; -1 where there is nothing to read.
+      auto page_of = [&](int i) -> int {
+        const int t = w.t0 + i * span + (box << tbs);
+        int page = paged ? -1 : w.b;
+        if (i >= count || t >= w.t1) return -1;
+        if (paged) page = __ldg(table + (t >> bts));
+        return page;
+      };
+      // One elected lane issues an item's boxes; coordinates come from the lanes
+      // that hold them.
+      auto fill = [&](uint32_t dst, uint32_t full, uint32_t bytes, int t, int page) {
+        const int my = max(page, -1);
 #pragma unroll
-      for (int x = 0; x < 8; ++x) {
-        if (x < boxes) {
-          const int pg = __shfl_sync(0xffffffffu, my, x);
-          if (tc::elect_one()) {
-            if (x == 0) ptx::mbar_arrive_expect_tx(full, bytes);
-            const int c1 = paged ? (t + (x << tbs)) & bmask : t + (x << tbs);
-            if (L::RAW) {
-              ptx::tma_g2s_4d(dst + ((uint32_t)x << tbs) * RB, map, 0, c1, w.h, pg, full, pol);
-            } else {
+        for (int x = 0; x < 8; ++x) {
+          if (x < boxes) {
+            const int pg = __shfl_sync(0xffffffffu, my, x);
+            if (tc::elect_one()) {
+              if (x == 0) ptx::mbar_arrive_expect_tx(full, bytes);
+              const int c1 = paged ? (t + (x << tbs)) & bmask : t + (x << tbs);
+              if (L::RAW) {
+                ptx::tma_g2s_4d(dst + ((uint32_t)x << tbs) * RB, map, 0, c1, w.h, pg, full, pol);
+              } else {
 #pragma unroll
-              for (int blk = 0; blk < KB; ++blk)
-                ptx::tma_g2s_4d(dst + blk * BLK + ((uint32_t)x << tbs) * 128u, map, 128 * blk, c1, w.h, pg, full, pol);
+                for (int blk = 0; blk < KB; ++blk)
+                  ptx::tma_g2s_4d(dst + blk * BLK + ((uint32_t)x << tbs) * 128u, map, 128 * blk, c1, w.h, pg, full, pol);
+              }
             }
+            __syncwarp();
           }
-          __syncwarp();
         }
+      };
+      bool ok = true;
+      int page = page_of(0), i = 0;
+      for (; i < count; ++i) {
+        const int t = w.t0 + i * span;
+        if constexpr (L::RAW) {
+          const int s = i % RSLOTS;
+          if (i >= RSLOTS && !tc_wait_warp(bar(&sh.rempty[op][s]), (uint32_t)((i / RSLOTS - 1) & 1), abort_flag)) {
+            ok = false;
+            break;
+          }
+          fill(sbase + L::OFF_RAW + (uint32_t)(op * RSLOTS + s) * L::RAWB, bar(&sh.rfull[op][s]), L::RAWB, t, page);
+        } else {
+          const int s = i % SLOTS;
+          if (i >= SLOTS && !tc_wait_warp(bar(op ? &sh.vempty[s] : &sh.kempty[s]), (uint32_t)((i / SLOTS - 1) & 1), abort_flag)) {
+            ok = false;
+            break;
+          }
+          fill((op ? svr : skr) + s * TILE, bar(!op ? &sh.kfull[s] : i < first_masked ? &sh.vfull[s] : &sh.vraw[s]), TILE, t,
+               page);
+        }
+        page = page_of(i + 1);
       }
-    };
-    bool ok = true;
-    int page = page_of(0), i = 0;
-    for (; i < count; ++i) {
-      const int t = w.t0 + i * span;
-      if constexpr (L::RAW) {
-        const int s = i % RSLOTS;
-        if (i >= RSLOTS && !tc_wait_warp(bar(&sh.rempty[op][s]), (uint32_t)((i / RSLOTS - 1) & 1), abort_flag)) {
-          ok = false;
-          break;
-        }
-        fill(sbase + L::OFF_RAW + (uint32_t)(op * RSLOTS + s) * L::RAWB, bar(&sh.rfull[op][s]), L::RAWB, t, page);
-      } else {
-        const int s = i % SLOTS;
-        if (i >= SLOTS && !tc_wait_warp(bar(op ? &sh.vempty[s] : &sh.kempty[s]), (uint32_t)((i / SLOTS - 1) & 1), abort_flag)) {
-          ok = false;
-          break;
-        }
-        fill((op ? svr : skr) + s * TILE, bar(!op ? &sh.kfull[s] : i < first_masked ? &sh.vfull[s] : &sh.vraw[s]), TILE, t,
-             page);
+      if (!ok && lane == 0) {
+        atomicOr(&g_kvfb_chunk_error, 1u);
+        *abort_flag = 1;
       }
-      page = page_of(i + 1);
-    }
-    if (!ok && lane == 0) {
-      atomicOr(&g_kvfb_chunk_error, 1u);
-      *abort_flag = 1;
-    }
-    // Never leave with copies in flight: the last item of each slot has landed.
-    constexpr int RING = L::RAW ? RSLOTS : SLOTS;
-    for (int k = max(0, i - RING); k < i; ++k) {
-      const int s = k % RING;
-      const bool fixed = !L::RAW && op && k >= first_masked;
-      const uint32_t full = L::RAW ? bar(&sh.rfull[op][s]) : bar(!op ? &sh.kfull[s] : fixed ? &sh.vraw[s] : &sh.vfull[s]);
-      if (!ptx::mbar_wait(full, (uint32_t)(((fixed ? k - first_masked : k) / RING) & 1)) && lane == 0) atomicOr(&g_kvfb_chunk_error, 1u);
-    }
-    // ----------------------------------------------------------- MMA issue
+      // Never leave with copies in flight: the last item of each slot has landed.
+      constexpr int RING = L::RAW ? RSLOTS : SLOTS;
+      for (int k = max(0, i - RING); k < i; ++k) {
+        const int s = k % RING;
+        const bool fixed = !L::RAW && op && k >= first_masked;
+        const uint32_t full = L::RAW ? bar(&sh.rfull[op][s]) : bar(!op ? &sh.kfull[s] : fixed ? &sh.vraw[s] : &sh.vfull[s]);
+        if (!ptx::mbar_wait(full, (uint32_t)(((fixed ? k - first_masked : k) / RING) & 1)) && lane == 0) atomicOr(&g_kvfb_chunk_error, 1u);
+      }
     } else {
+      // --------------------------------------------------------- MMA issue
       const int g = warp == LAST ? 0 : 1;  // the softmax group that this warp issues for
       constexpr uint32_t ID_S = tc::idesc_f16(false, false, 128, 64), ID_O = tc::idesc_f16(false, true, 128, D);
       bool ok = true;
