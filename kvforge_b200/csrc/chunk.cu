@@ -58,8 +58,8 @@ __global__ void __launch_bounds__(128) chunk_merge(const ChunkArgs a) {
 template <int DT, int D> void *merge_fn() { return reinterpret_cast<void *>(&chunk_merge<DT, D>); }
 
 template <int FMT> void *mma_fn(int d) {
-  return d == 128 ? reinterpret_cast<void *>(&chunk_mma_kernel<FMT, KVF_DT_F32, 128>)
-                  : reinterpret_cast<void *>(&chunk_mma_kernel<FMT, KVF_DT_F32, 64>);
+  return d == 128 ? reinterpret_cast<void *>(&chunk_mma_kernel<FMT, 128>)
+                  : reinterpret_cast<void *>(&chunk_mma_kernel<FMT, 64>);
 }
 struct TcVariant {
   void *fn;

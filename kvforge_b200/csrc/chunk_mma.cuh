@@ -1,5 +1,5 @@
-// chunk_mma.cuh - attention of a chunk on mma.sync in fp32 accuracy: every type
-// of query, every cache format, both head widths.
+// chunk_mma.cuh - attention of a chunk on mma.sync in fp32 accuracy, for fp32
+// queries: every cache format, both head widths.
 //
 // Each operand x is split into two tf32 numbers, hi = tf32(x) and lo = x - hi
 // (11 significant bits each, the exponent range of fp32, so nothing has to be
@@ -58,7 +58,7 @@ __device__ __forceinline__ void put8(float *p, const float (&x)[8]) {
   reinterpret_cast<float4 *>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
 }
 
-template <int FMT, int DT, int D>
+template <int FMT, int D>
 __global__ void __launch_bounds__(kChunkThreads) chunk_mma_kernel(const ChunkArgs a) {
   constexpr int QS = D + 8, KS = D + 8, VS = D + 4;
   constexpr bool LO = FMT != KVF_FMT_F16;  // K and V need their lo halves
@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(kChunkThreads) chunk_mma_kernel(const ChunkArg
   for (int i = tid; i < kChunkRows * (D / 8); i += kChunkThreads) {
     const int r = i / (D / 8), li = i % (D / 8);
     float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (r < w.rows) load8<DT>(chunk_row(a.q, a, w, r) + 8 * li * dtype_bytes(DT), a.q.vec, x);
+    if (r < w.rows) load8<KVF_DT_F32>(chunk_row(a.q, a, w, r) + 32 * li, a.q.vec, x);
     put8(sq + r * QS + 8 * li, x);
   }
 
@@ -264,12 +264,11 @@ __global__ void __launch_bounds__(kChunkThreads) chunk_mma_kernel(const ChunkArg
     // a row that sees nothing: zeros and -inf
     const float inv = m == -INFINITY ? 0.f : 1.f / l;
     if (a.lse && t4 == 0) a.lse[at] = m == -INFINITY ? -INFINITY : m + log2f(l);
-    using E = Elem<DT>;
-    typename E::T *out = reinterpret_cast<typename E::T *>(chunk_row(a.out, a, w, r));
+    float *out = reinterpret_cast<float *>(chunk_row(a.out, a, w, r));
 #pragma unroll
     for (int n = 0; n < D / 8; ++n) {
-      out[8 * n + 2 * t4] = E::from(o[n][2 * half] * inv);
-      out[8 * n + 2 * t4 + 1] = E::from(o[n][2 * half + 1] * inv);
+      out[8 * n + 2 * t4] = o[n][2 * half] * inv;
+      out[8 * n + 2 * t4 + 1] = o[n][2 * half + 1] * inv;
     }
   }
 }
