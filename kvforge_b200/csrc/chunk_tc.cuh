@@ -348,8 +348,11 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
         sum += weigh<masked>(sb, m, c, at + 32, seen, p + 16);
         // Weights are taken against the maximum as it stands; only where their
         // sum is past kTcLazySum is it raised, the output so far rescaled, and
-        // the scores of the half read and weighed again.
-        if (__any_sync(0xffffffffu, !(sum <= kTcLazySum) || (m == -INFINITY && at < seen))) {
+        // the scores of the half read and weighed again. The warp goes along, but
+        // a row that need not be raised keeps its maximum and so its weights: its
+        // output does not depend on the rows beside it.
+        const bool raise = !(sum <= kTcLazySum) || (m == -INFINITY && at < seen);
+        if (__any_sync(0xffffffffu, raise)) {
           float mx = -INFINITY;
 #pragma unroll 1
           for (int u = 0; u < 4; ++u) {
@@ -360,7 +363,7 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
             for (int k = 0; k < 16; ++k)
               if (at + 16 * u + k < seen) mx = fmaxf(mx, __uint_as_float(s[k]) * c);
           }
-          const float mn = fmaxf(m, mx);
+          const float mn = raise ? fmaxf(m, mx) : m;
           const float f = m == mn ? 1.f : exp2f(m - mn);
           m = mn;
           l *= f;
