@@ -25,8 +25,11 @@
 //          scores, and V read MN-major. The other two are the producers of K and of V:
 //          TMA boxes per page. A box of tokens that nobody sees, or of a block mapped
 //          to a negative page, is asked for at page -1, which TMA fills with zeros.
-// The running maximum a row's weights are taken against is raised only when 64
-// of them add up to more than 256 (weights up to that fit fp16, and their sum
+// A row's weights are taken against a reference 7 below its running maximum (log2),
+// so that the largest is 2^7: fp16 then holds weights down to 2^-32 of it, where
+// against the maximum itself those below 2^-25 would be lost, and many small ones
+// can outweigh one large one whose value is small. The reference is raised only when
+// 64 weights add up to more than 2^15 (weights up to that fit fp16, and their sum
 // fp32), so the output in tensor memory is rescaled rarely, a step's scores are
 // read once, and their maximum is not needed before.
 // Waits are bounded in time; tensor memory is released before exit.
@@ -51,7 +54,8 @@ namespace {
 constexpr int kTcRows = 128;    // rows of a tile
 constexpr int kTcStep = 128;    // tokens of a step
 constexpr int kTcHalf = 64;     // tokens of a raw half step
-constexpr float kTcLazySum = 256.f;  // most that 64 weights may add up to before the maximum is raised
+constexpr float kTcTop = 7.f;          // log2 of a row's largest weight when its reference is raised
+constexpr float kTcLazySum = 32768.f;  // most that 64 weights may add up to before that
 
 __host__ __device__ constexpr int cache_row_bytes(int fmt, int d) {
   return fmt == KVF_FMT_F16 ? 2 * d : fmt == KVF_FMT_INT8 ? d : d / 2;
@@ -323,7 +327,7 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
     const uint32_t ts = tbase + lanes + S_COL + 128u * grp, to = tbase + lanes + O_COL + (uint32_t)(D * grp);
     const int steps = nw[grp];
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = 0.f;           // reference (log2) and sum of the weights taken against it
     bool early = false;
     uint32_t sa[32], sb[32];                // scores of the half at hand, or (early) of the next
     for (int j = 0; j < steps && ok; ++j) {
@@ -346,10 +350,10 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
         tc::wait_ld32(sb);
         float sum = weigh<masked>(sa, m, c, at, seen, p);
         sum += weigh<masked>(sb, m, c, at + 32, seen, p + 16);
-        // Weights are taken against the maximum as it stands; only where their
+        // Weights are taken against the reference as it stands; only where their
         // sum is past kTcLazySum is it raised, the output so far rescaled, and
         // the scores of the half read and weighed again. The warp goes along, but
-        // a row that need not be raised keeps its maximum and so its weights: its
+        // a row that need not be raised keeps its reference and so its weights: its
         // output does not depend on the rows beside it.
         const bool raise = !(sum <= kTcLazySum) || (m == -INFINITY && at < seen);
         if (__any_sync(0xffffffffu, raise)) {
@@ -363,7 +367,7 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
             for (int k = 0; k < 16; ++k)
               if (at + 16 * u + k < seen) mx = fmaxf(mx, __uint_as_float(s[k]) * c);
           }
-          const float mn = raise ? fmaxf(m, mx) : m;
+          const float mn = raise ? fmaxf(m, mx - kTcTop) : m;
           const float f = m == mn ? 1.f : exp2f(m - mn);
           m = mn;
           l *= f;

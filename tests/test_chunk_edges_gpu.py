@@ -33,6 +33,43 @@ def _attend(q, cache, splits, lse=None, **kw):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("far", [17.0, 18.0])
+@pytest.mark.parametrize("sink", [0, 20000, -1])
+def test_many_small_weights_beside_a_large_one(cuda, dtype, far, sink):
+    """One token takes nearly all of the softmax and its value is zero; 32768
+    others, each e^-far of it, make the output.
+
+    Bound: fp16 weights are taken against a largest one of at least 2^7 (a row's
+    reference lies 7 below its maximum), and below fp16's normal range they are off by at most
+    2^-25 absolute, 2^-32 of the largest; above it by 2^-11 relative. fp32
+    queries: 2^-20 relative, from the products' and scores' halves. Scores are
+    one product with 1, exact; exponentials, sums over n tokens and the merge
+    add (n + 32) 2^-24 relative, and the output is rounded once."""
+    g = _gen(cuda, 1)
+    n, d, T, H = 32769, 128, 2, 2
+    K = torch.zeros((1, 1, n, d), device=cuda)
+    K[..., 0] = -far + _randn((1, 1, n), g) / 8
+    K[0, 0, sink, 0] = 0
+    V = _randn((1, 1, n, d), g) + 1
+    V[0, 0, sink] = 0
+    cache = api.KVCache.from_logical(K, V, fmt=FMT_F16, place=TOKEN)
+    q = torch.zeros((1, T, H, d), dtype=dtype, device=cuda)
+    q[..., 0] = 1
+    k, v = (x[0, :, 0].double() for x in api.gather(cache, n))
+    w = (k[:, 0]).exp()
+    out = (w @ v) / w.sum()
+    small = 2.0 ** -32 * v.abs().sum(0) / w.sum() if dtype != torch.float32 else 0.0
+    rel = (2.0 ** -11 if dtype != torch.float32 else 2.0 ** -20) + (n + 32) * 2.0 ** -24
+    tol = small + rel * (w @ v.abs()) / w.sum()
+    tol = tol + torch.finfo(dtype).eps / 2 * (out.abs() + tol)
+    for splits in (1, 2, 5):
+        got = _attend(q, cache, splits, causal=False, scale=1.0).double()
+        err = (got - out).abs()
+        assert bool((err <= tol).all()), f"splits {splits}: off by {float((err / tol).max()):.3g} times the bound, " \
+                                         f"{float((err / out.abs()).median()):.3g} relative"
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("fmt,group", [(FMT_F16, 0), (FMT_INT8, 64)])
 @pytest.mark.parametrize("rows", [5, 90])
 def test_rows_do_not_depend_on_their_neighbours(cuda, dtype, fmt, group, rows):
