@@ -26,7 +26,7 @@
 //          TMA boxes per page. A box of tokens that nobody sees, or of a block mapped
 //          to a negative page, is asked for at page -1, which TMA fills with zeros.
 // A row's weights are taken against a reference 7 below its running maximum (log2),
-// so that the largest is 2^7: fp16 then holds weights down to 2^-32 of it, where
+// so that the largest is about 2^7: fp16 then holds weights down to 2^-32 of it, where
 // against the maximum itself those below 2^-25 would be lost, and many small ones
 // can outweigh one large one whose value is small. The reference is raised only when
 // 64 weights add up to more than 2^15 (weights up to that fit fp16, and their sum
@@ -41,7 +41,6 @@
 #include <cuda.h>
 
 #include <cstddef>
-#include <type_traits>
 
 namespace kvfb {
 
@@ -56,6 +55,10 @@ constexpr int kTcStep = 128;    // tokens of a step
 constexpr int kTcHalf = 64;     // tokens of a raw half step
 constexpr float kTcTop = 7.f;          // log2 of a row's largest weight when its reference is raised
 constexpr float kTcLazySum = 32768.f;  // most that 64 weights may add up to before that
+// A reference of 2^24 and more (log2) is rounded so coarsely that the largest weight,
+// 2^7 above it but for that, may come out as infinity or 0: from there on a row's
+// reference is its largest score as it is, taken off before the scale.
+constexpr float kTcFar = 16777216.f;
 
 __host__ __device__ constexpr int cache_row_bytes(int fmt, int d) {
   return fmt == KVF_FMT_F16 ? 2 * d : fmt == KVF_FMT_INT8 ? d : d / 2;
@@ -267,8 +270,8 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
 
     // Query rows, scaled, into their tile: a warp takes its own 32 rows, each by
     // D / 8 lanes, all loads in flight at once. A bf16 row is scaled by 2^(14 -
-    // exponent of its largest magnitude), within what fp32 holds; by 1 if that
-    // is zero, infinite or NaN.
+    // exponent of its largest magnitude), or the largest power that fp32 holds for
+    // rows below 2^-100; by 1 if that is zero, infinite or NaN.
     if (TWO || grp == 0) {
       constexpr int LPR = D / 8, RPW = 32 / LPR, N = 32 / RPW;
       const int li = lane % LPR, r0 = 32 * (warp & 3) + lane / LPR;
@@ -302,7 +305,7 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
           for (int off = 1; off < LPR; off <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, off));
           float f = 1.f;
           if (mx > 0u && mx < 0x7f80u) {
-            ex = min(max((int)(mx >> 7), 27), 240);
+            ex = max((int)(mx >> 7), 27);
             f = __uint_as_float((uint32_t)(127 + 14 + 127 - ex) << 23);
           }
 #pragma unroll
@@ -327,7 +330,9 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
     const uint32_t ts = tbase + lanes + S_COL + 128u * grp, to = tbase + lanes + O_COL + (uint32_t)(D * grp);
     const int steps = nw[grp];
-    float m = -INFINITY, l = 0.f;           // reference (log2) and sum of the weights taken against it
+    // Reference (log2) of the row's weights and their sum; where the reference is
+    // past kTcFar it is the raw score `base`, and m is NaN so that every half is raised.
+    float m = -INFINITY, l = 0.f, base = 0.f;
     bool early = false;
     uint32_t sa[32], sb[32];                // scores of the half at hand, or (early) of the next
     for (int j = 0; j < steps && ok; ++j) {
@@ -335,10 +340,10 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
       // Half a step at a time (64 tokens), each half with scores, weights and
       // barriers of its own: while one half is weighed, the tensor cores take the
       // other's value product and its next scores. Whole steps and steps that some
-      // row does not see to the end are code of their own: the comparisons would
-      // cost the first a third of its instructions.
-      auto half = [&](int h, auto is_masked) {
-        constexpr bool masked = decltype(is_masked)::value;
+      // row does not see to the end are weighed by code of their own: the
+      // comparisons would cost the first a third of its instructions.
+      const bool masked = __any_sync(0xffffffffu, t + kTcStep > seen);
+      auto half = [&](int h) {
         const int at = t + 64 * h;
         const uint32_t tsh = ts + 64u * h;
         uint32_t p[32];
@@ -348,8 +353,14 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
         }
         tc::wait_ld32(sa);
         tc::wait_ld32(sb);
-        float sum = weigh<masked>(sa, m, c, at, seen, p);
-        sum += weigh<masked>(sb, m, c, at + 32, seen, p + 16);
+        float sum;
+        if (masked) {
+          sum = weigh<true>(sa, m, c, at, seen, p);
+          sum += weigh<true>(sb, m, c, at + 32, seen, p + 16);
+        } else {
+          sum = weigh<false>(sa, m, c, at, seen, p);
+          sum += weigh<false>(sb, m, c, at + 32, seen, p + 16);
+        }
         // Weights are taken against the reference as it stands; only where their
         // sum is past kTcLazySum is it raised, the output so far rescaled, and
         // the scores of the half read and weighed again. The warp goes along, but
@@ -357,6 +368,9 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
         // output does not depend on the rows beside it.
         const bool raise = !(sum <= kTcLazySum) || (m == -INFINITY && at < seen);
         if (__any_sync(0xffffffffu, raise)) {
+          // scores times the sign of the scale, and its magnitude
+          const float ac = fabsf(c);
+          const uint32_t flip = __float_as_uint(c) & 0x80000000u;
           float mx = -INFINITY;
 #pragma unroll 1
           for (int u = 0; u < 4; ++u) {
@@ -365,11 +379,24 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
             tc::wait_ld16(s);
 #pragma unroll
             for (int k = 0; k < 16; ++k)
-              if (at + 16 * u + k < seen) mx = fmaxf(mx, __uint_as_float(s[k]) * c);
+              if (at + 16 * u + k < seen) mx = fmaxf(mx, __uint_as_float(s[k] ^ flip));
           }
-          const float mn = raise ? fmaxf(m, mx - kTcTop) : m;
-          const float f = m == mn ? 1.f : exp2f(m - mn);
-          m = mn;
+          float f = 1.f;
+          if (raise && m == m) {
+            const float mn = fmaxf(m, fmaf(mx, ac, -kTcTop));
+            if (fabsf(mn) >= kTcFar && mn != -INFINITY) {
+              f = exp2f(kTcTop - fmaf(mx, ac, -m));
+              base = mx;
+              m = NAN;
+            } else {
+              f = m == mn ? 1.f : exp2f(m - mn);
+              m = mn;
+            }
+          } else if (raise) {
+            const float top = fmaxf(base, mx);
+            f = base == top ? 1.f : exp2f((base - top) * ac);
+            base = top;
+          }
           l *= f;
           if (2 * j + h > 0 && __any_sync(0xffffffffu, f != 1.f)) {
             // the half before this one; those before it were done when the scores came
@@ -389,12 +416,26 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
             }
           }
           sum = 0.f;
+          if (__any_sync(0xffffffffu, m != m)) {
+            // rows with a raw reference: it is taken off where the scores lie
+#pragma unroll 1
+            for (int u = 0; u < 4; ++u) {
+              uint32_t s[16];
+              tc::ld16(tsh + 16u * u, s);
+              tc::wait_ld16(s);
+#pragma unroll
+              for (int k = 0; k < 16; ++k)
+                if (m != m) s[k] = __float_as_uint(__uint_as_float(s[k] ^ flip) - base);
+              tc::st16(tsh + 16u * u, s);
+            }
+            tc::wait_st();
+          }
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             uint32_t s[32];
             tc::ld32(tsh + 32u * u, s);
             tc::wait_ld32(s);
-            sum += weigh<true>(s, m, c, at + 32 * u, seen, p + 16 * u);
+            sum += weigh<true>(s, m != m ? -kTcTop : m, m != m ? ac : c, at + 32 * u, seen, p + 16 * u);
           }
         }
         l += sum;
@@ -410,7 +451,6 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
         tc::wait_st();
         tc::fence_before();
       };
-      const bool masked = __any_sync(0xffffffffu, t + kTcStep > seen);
 #pragma unroll 1
       for (int h = 0; h < 2; ++h) {
         if (!early && !tc_wait_warp(bar(&sh.sfull[grp][h]), (uint32_t)(j & 1), abort_flag)) {
@@ -419,10 +459,7 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
         }
         if (!idle) {
           tc::fence_after();
-          if (masked)
-            half(h, std::true_type{});
-          else
-            half(h, std::false_type{});
+          half(h);
           if (!ok) break;
           __syncwarp();
         }
@@ -438,6 +475,7 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
     }
     // ------------------------------------------------------------ epilogue
     const bool none = m == -INFINITY && l == 0.f;
+    if (m != m) m = fmaf(base, fabsf(c), -kTcTop);
     const bool odd = *reinterpret_cast<volatile int *>(&sh.odd) != 0;
     const long long at = live ? chunk_index(a, w, row) : 0;
     const long long part = at * a.splits + (TWO ? w.split : 2 * w.split + grp);

@@ -70,6 +70,53 @@ def test_many_small_weights_beside_a_large_one(cuda, dtype, far, sink):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", [1e9, 1e35])
+def test_scores_far_past_the_usual_range(cuda, dtype, size):
+    """Scores of 1e5 to 1e36: the softmax is the token with the largest score, or
+    the mean of the values of tokens whose keys are equal. fp16 queries reach
+    as far as their type allows, against large keys."""
+    g = _gen(cuda, 2)
+    B, T, H, Hkv, n, d = 2, 70, 4, 2, 300, 128
+    K, V = _randn((B, Hkv, n, d), g), _randn((B, Hkv, n, d), g)
+    q = _randn((B, T, H, d), g)
+    if dtype == torch.float16:
+        K *= 4e3 if size > 1e20 else 30.0  # three times a key of this size is still below 65504
+        q *= 1e4 if size > 1e20 else 3e3
+    else:
+        q *= size
+    for b in range(B):  # equal keys in other halves of a step, and in other steps
+        K[b, :, 5], K[b, :, 100], K[b, :, 201] = 3 * K[b, :, 40], 3 * K[b, :, 40], 3 * K[b, :, 40]
+    cache = api.KVCache.from_logical(K, V, fmt=FMT_F16, place=TOKEN16)
+    k, v = (x.double() for x in api.gather(cache, n))
+    q = q.to(dtype)
+    g2 = H // Hkv
+    seen_gap = 0
+    for splits in (1, 2, 3):
+        lse = torch.zeros((B, T, H), device=cuda)
+        got = _attend(q, cache, splits, lse=lse)
+        assert bool(got.isfinite().all()) and bool(lse.isfinite().all()), f"splits {splits}"
+        for b in range(B):
+            for h in range(H):
+                s = q[b, :, h].double() @ k[b, :, h // g2].T / math.sqrt(d)
+                last = n - T + torch.arange(T, device=cuda)
+                s.masked_fill_(torch.arange(n, device=cuda) > last[:, None], -math.inf)
+                p = torch.softmax(s, -1)
+                # fp32 scores are off by at most (d + 4) 2^-24 + 2^-21 of what they add; rows whose
+                # runner-up is nearer than that (and 30 for the weights) have no answer in fp32
+                mag = (q[b, :, h].double().abs() @ k[b, :, h // g2].abs().T / math.sqrt(d)).amax(-1)
+                top = s.amax(-1)
+                rest = torch.where(s == top[:, None], -math.inf, s).amax(-1)
+                clear = top - rest > 2 * mag * ((d + 4) * 2.0 ** -24 + 2.0 ** -21) + 30
+                seen_gap += int(clear.sum())
+                err = (got[b, :, h].double() - p @ v[b, :, h // g2]).abs()[clear]
+                tol = (2.0 ** -18 if dtype == torch.float32 else 2.0 ** -10 + torch.finfo(dtype).eps) * 5
+                assert bool((err <= tol).all()), f"splits {splits}: {float(err.max()):.3g}"
+                want = top * math.log2(math.e)
+                assert bool(((lse[b, :, h].double() - want).abs()[clear] <= 1 + 1e-4 * want.abs()[clear]).all())
+    assert seen_gap > 3 * B * T * H // 2  # most rows are clear
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("fmt,group", [(FMT_F16, 0), (FMT_INT8, 64)])
 @pytest.mark.parametrize("rows", [5, 90])
 def test_rows_do_not_depend_on_their_neighbours(cuda, dtype, fmt, group, rows):
