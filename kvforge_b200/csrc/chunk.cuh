@@ -111,10 +111,15 @@ __device__ __forceinline__ long long chunk_index(const ChunkArgs &a, const Chunk
   return ((long long)w.b * a.T + w.j0) * a.H + w.h * a.g + (long long)j * a.H + head;
 }
 
-// Eight channels of cache row `row` (from channel 8 * li) as fp32.
+// Whether one of a word's two fp16 numbers is infinite or NaN: an exponent of ones
+// carries into the sign's place.
+__device__ __forceinline__ uint32_t odd_halves(uint32_t w) { return ((w & 0x7C007C00u) + 0x04000400u) & 0x80008000u; }
+
+// Eight channels of cache row `row` (from channel 8 * li) as fp32. Nonzero if one
+// of them can be infinite or NaN (of a quantized cache: its scale or zero is).
 template <int FMT, int D>
-__device__ __forceinline__ void cache8(const uint8_t *data, const uint32_t *meta, const ChunkArgs &a, long long row,
-                                       int li, float (&x)[8]) {
+__device__ __forceinline__ uint32_t cache8(const uint8_t *data, const uint32_t *meta, const ChunkArgs &a, long long row,
+                                           int li, float (&x)[8]) {
   if (FMT == KVF_FMT_F16) {
     const uint4 r = __ldg(reinterpret_cast<const uint4 *>(data + row * (2 * D)) + li);
     const uint32_t w[4] = {r.x, r.y, r.z, r.w};
@@ -124,7 +129,7 @@ __device__ __forceinline__ void cache8(const uint8_t *data, const uint32_t *meta
       x[2 * k] = f.x;
       x[2 * k + 1] = f.y;
     }
-    return;
+    return odd_halves(w[0]) | odd_halves(w[1]) | odd_halves(w[2]) | odd_halves(w[3]);
   }
   uint2 r;
   if (FMT == KVF_FMT_INT8) {
@@ -141,6 +146,7 @@ __device__ __forceinline__ void cache8(const uint8_t *data, const uint32_t *meta
     const uint32_t c = FMT == KVF_FMT_INT8 ? ((k < 4 ? r.x : r.y) >> (8 * (k & 3))) & 255u : (r.x >> (4 * k)) & 15u;
     x[k] = __fmaf_rn((float)c, sc, zero);
   }
+  return odd_halves(m);
 }
 
 } // namespace

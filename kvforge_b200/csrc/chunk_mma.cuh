@@ -9,6 +9,12 @@
 // one step of an output): they round towards zero, and what they leave is added
 // in fp32 to nearest.
 //
+// Infinities and NaN cannot go through halves (lo * inf is NaN where lo is 0 or of
+// the other sign, and 0 * inf would reach rows that do not see the token), so zeros
+// stand in for those of a K or V tile, and the tokens that held them are noted: their
+// scores are then worked out in fp32 from the cache, for the rows that see them,
+// and their infinite or NaN values added channel by channel.
+//
 // Four warps of 16 rows share tiles of 64 tokens, dequantised to fp32 in shared
 // memory. Scores stay in registers: the fragment that the score product leaves
 // (rows x two adjacent tokens) is taken as it is for the operand of the value
@@ -27,6 +33,7 @@ constexpr int kChunkThreads = 128;
 
 __host__ __device__ constexpr int chunk_mma_smem(int d) {
   // q and k rows of d + 8 floats (conflict-free 8-byte reads), v rows of d + 4
+  // and two masks of 64 tokens
   return (kChunkRows * (d + 8) + kChunkTokens * (d + 8) + kChunkTokens * (d + 4)) * 4 + 16;
 }
 
@@ -36,7 +43,7 @@ __device__ __forceinline__ void split(float x, uint32_t &hi, uint32_t &lo) {
   hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
   lo = __float_as_uint(__fsub_rn(x, __uint_as_float(hi)));
 }
-// K and V of an f16 cache are tf32 numbers as they are (infinities stay so).
+// K and V of an f16 cache are tf32 numbers as they are.
 template <bool LO> __device__ __forceinline__ void split_if(float x, uint32_t &hi, uint32_t &lo) {
   if (LO) {
     split(x, hi, lo);
@@ -58,13 +65,56 @@ __device__ __forceinline__ void put8(float *p, const float (&x)[8]) {
   reinterpret_cast<float4 *>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
 }
 
+// Infinities and NaN of the step's tiles, seldom there: out of line, so that the
+// loops around them stay as they are without.
+
+// Zeros for those that this thread stored, their tokens into `odd`: K's in words 0
+// and 1, V's in 2 and 3.
+template <int D> __device__ __noinline__ void odd_tokens(float *sk, float *sv, unsigned *odd) {
+  constexpr int KS = D + 8, VS = D + 4;
+  for (int i = threadIdx.x; i < kChunkTokens * (D / 8); i += kChunkThreads) {
+    const int r = i / (D / 8), li = i % (D / 8);
+    for (int k = 0; k < 16; ++k) {
+      float *x = k < 8 ? sk + r * KS + 8 * li + k : sv + r * VS + 8 * li + k - 8;
+      if (fabsf(*x) < INFINITY) continue;
+      *x = 0.f;
+      atomicOr(odd + (k < 8 ? 0 : 2) + (r >> 5), 1u << (r & 31));
+    }
+  }
+}
+// Products of two query rows with the K row of a token.
 template <int FMT, int D>
-__global__ void __launch_bounds__(kChunkThreads) chunk_mma_kernel(const ChunkArgs a) {
+__device__ __noinline__ float2 odd_scores(const ChunkArgs &a, long long row, const float *q_lo, const float *q_hi) {
+  float2 s = make_float2(0.f, 0.f);
+  for (int li = 0; li < D / 8; ++li) {
+    float x[8];
+    cache8<FMT, D>(a.k, a.km, a, row, li, x);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      s.x = fmaf(q_lo[8 * li + k], x[k], s.x);
+      s.y = fmaf(q_hi[8 * li + k], x[k], s.y);
+    }
+  }
+  return s;
+}
+// Channels 8 n + 2 t4 and the next of the V row of a token.
+template <int FMT, int D> __device__ __noinline__ float2 odd_values(const ChunkArgs &a, long long row, int n, int t4) {
+  float x[8];
+  cache8<FMT, D>(a.v, a.vm, a, row, n, x);
+  return t4 == 0   ? make_float2(x[0], x[1])
+         : t4 == 1 ? make_float2(x[2], x[3])
+         : t4 == 2 ? make_float2(x[4], x[5])
+                   : make_float2(x[6], x[7]);
+}
+
+template <int FMT, int D>
+__global__ void __launch_bounds__(kChunkThreads) chunk_mma_kernel(const __grid_constant__ ChunkArgs a) {
   constexpr int QS = D + 8, KS = D + 8, VS = D + 4;
   constexpr bool LO = FMT != KVF_FMT_F16;  // K and V need their lo halves
   extern __shared__ __align__(16) float sm[];
   float *sq = sm, *sk = sq + kChunkRows * QS, *sv = sk + kChunkTokens * KS;
-  int *odd = reinterpret_cast<int *>(sv + kChunkTokens * VS);  // V rows of the step hold an infinity or NaN
+  // Tokens of the step whose K (words 0, 1) or V (2, 3) rows hold an infinity or NaN.
+  unsigned *odd = reinterpret_cast<unsigned *>(sv + kChunkTokens * VS);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g4 = lane >> 2, t4 = lane & 3;
 
   ChunkWork w;
@@ -74,9 +124,13 @@ __global__ void __launch_bounds__(kChunkThreads) chunk_mma_kernel(const ChunkArg
     const int r = i / (D / 8), li = i % (D / 8);
     float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (r < w.rows) load8<KVF_DT_F32>(chunk_row(a.q, a, w, r) + 32 * li, a.q.vec, x);
+    // halved, and the scale doubled: rounding to 11 bits cannot make the greatest numbers infinite
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] *= 0.5f;
     put8(sq + r * QS + 8 * li, x);
   }
 
+  const float scale = 2.f * a.scale_log2;
   const int r_lo = warp * 16 + g4, r_hi = r_lo + 8;
   const int seen_lo = r_lo < w.rows ? chunk_seen(a, w, r_lo) : 0;
   const int seen_hi = r_hi < w.rows ? chunk_seen(a, w, r_hi) : 0;
@@ -89,9 +143,9 @@ __global__ void __launch_bounds__(kChunkThreads) chunk_mma_kernel(const ChunkArg
 
   for (int t = w.t0; t < w.t1; t += kChunkTokens) {
     __syncthreads();
-    if (tid == 0) *odd = 0;
+    if (tid < 4) odd[tid] = 0u;
+    uint32_t any = 0u;
     __syncthreads();
-    const bool masked = t + kChunkTokens > w.seen0;  // some row of the tile does not see all of the step
 #pragma unroll 4
     for (int i = tid; i < kChunkTokens * (D / 8); i += kChunkThreads) {
       const int r = i / (D / 8), li = i % (D / 8);
@@ -99,18 +153,14 @@ __global__ void __launch_bounds__(kChunkThreads) chunk_mma_kernel(const ChunkArg
       // rows past the last that anyone sees are zero, whatever the cache holds there
       const long long row = t + r < w.t1 ? a.cache.row(w.b, w.h, t + r) : -1;
       if (row >= 0) {
-        cache8<FMT, D>(a.k, a.km, a, row, li, x);
-        cache8<FMT, D>(a.v, a.vm, a, row, li, y);
+        any |= cache8<FMT, D>(a.k, a.km, a, row, li, x) | cache8<FMT, D>(a.v, a.vm, a, row, li, y);
       }
       put8(sk + r * KS + 8 * li, x);
       put8(sv + r * VS + 8 * li, y);
-      if (masked) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (!(fabsf(y[k]) < INFINITY)) *odd = 1;
-      }
     }
+    if (any) odd_tokens<D>(sk, sv, odd);
     __syncthreads();
+    unsigned long long odd_k = odd[0] | (unsigned long long)odd[1] << 32, odd_v = odd[2] | (unsigned long long)odd[3] << 32;
 
     float s[kChunkTokens / 8][4];
 #pragma unroll
@@ -147,14 +197,29 @@ __global__ void __launch_bounds__(kChunkThreads) chunk_mma_kernel(const ChunkArg
       }
     }
 
+#pragma unroll 1
+    for (; odd_k; odd_k &= odd_k - 1) {
+      const int u = __ffsll(odd_k) - 1;
+      // the token's score for this thread's rows, if the thread holds it
+      const float2 x = odd_scores<FMT, D>(a, a.cache.row(w.b, w.h, t + u), sq + r_lo * QS, sq + r_hi * QS);
+#pragma unroll
+      for (int n = 0; n < kChunkTokens / 8; ++n)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          if (8 * n + 2 * t4 + k == u) {
+            s[n][k] = x.x;
+            s[n][2 + k] = x.y;
+          }
+    }
+
     float mx_lo = -INFINITY, mx_hi = -INFINITY;
 #pragma unroll
     for (int n = 0; n < kChunkTokens / 8; ++n)
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const int tok = t + 8 * n + 2 * t4 + k;
-        s[n][k] = tok < seen_lo ? s[n][k] * a.scale_log2 : -INFINITY;
-        s[n][2 + k] = tok < seen_hi ? s[n][2 + k] * a.scale_log2 : -INFINITY;
+        s[n][k] = tok < seen_lo ? s[n][k] * scale : -INFINITY;
+        s[n][2 + k] = tok < seen_hi ? s[n][2 + k] * scale : -INFINITY;
         mx_lo = fmaxf(mx_lo, s[n][k]);
         mx_hi = fmaxf(mx_hi, s[n][2 + k]);
       }
@@ -180,38 +245,47 @@ __global__ void __launch_bounds__(kChunkThreads) chunk_mma_kernel(const ChunkArg
         l_lo += s[n][k];
         l_hi += s[n][2 + k];
       }
-    if (*reinterpret_cast<volatile int *>(odd)) {
+    // Rows that see such a value are rescaled before it is added; the others as ever.
+    float g_lo = f_lo, g_hi = f_hi;
+    if (odd_v) {
+      const int first = t + __ffsll(odd_v) - 1;
+      if (first < seen_lo) g_lo = 1.f;
+      if (first < seen_hi) g_hi = 1.f;
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          if (first < seen_lo) o[n][k] *= f_lo;
+          if (first < seen_hi) o[n][2 + k] *= f_hi;
+        }
+    }
+#pragma unroll 1
+    for (; odd_v; odd_v &= odd_v - 1) {
+      const int u = __ffsll(odd_v) - 1;
+      // the token's weights, from the lanes that hold them
+      float p_lo = 0.f, p_hi = 0.f;
+      const int src = (lane & ~3) + ((u & 7) >> 1);
+#pragma unroll
+      for (int n = 0; n < kChunkTokens / 8; ++n) {
+        const float x0 = __shfl_sync(0xffffffffu, (u & 1) ? s[n][1] : s[n][0], src);
+        const float x1 = __shfl_sync(0xffffffffu, (u & 1) ? s[n][3] : s[n][2], src);
+        if (n == (u >> 3)) {
+          p_lo = x0;
+          p_hi = x1;
+        }
+      }
+      const long long row = a.cache.row(w.b, w.h, t + u);
 #pragma unroll
       for (int n = 0; n < D / 8; ++n) {
-        o[n][0] *= f_lo;
-        o[n][1] *= f_lo;
-        o[n][2] *= f_hi;
-        o[n][3] *= f_hi;
-      }
-      // 0 * inf would carry an infinity or NaN into rows that do not see its
-      // token: such a step is added token by token, each row what it sees.
-      for (int u = 0; u < kChunkTokens; ++u) {
-        const int src = (lane & ~3) + ((u & 7) >> 1);
-        float p_lo = 0.f, p_hi = 0.f;
+        const float2 x = odd_values<FMT, D>(a, row, n, t4);
 #pragma unroll
-        for (int n = 0; n < kChunkTokens / 8; ++n) {
-          const float x0 = __shfl_sync(0xffffffffu, (u & 1) ? s[n][1] : s[n][0], src);
-          const float x1 = __shfl_sync(0xffffffffu, (u & 1) ? s[n][3] : s[n][2], src);
-          if (n == (u >> 3)) {
-            p_lo = x0;
-            p_hi = x1;
-          }
+        for (int k = 0; k < 2; ++k) {
+          const float v = k ? x.y : x.x;
+          if (fabsf(v) < INFINITY) continue;
+          if (t + u < seen_lo) o[n][k] = fmaf(p_lo, v, o[n][k]);
+          if (t + u < seen_hi) o[n][2 + k] = fmaf(p_hi, v, o[n][2 + k]);
         }
-#pragma unroll
-        for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const float v = sv[u * VS + 8 * n + 2 * t4 + k];
-            if (t + u < seen_lo) o[n][k] = fmaf(p_lo, v, o[n][k]);
-            if (t + u < seen_hi) o[n][2 + k] = fmaf(p_hi, v, o[n][2 + k]);
-          }
       }
-      continue;
     }
     uint32_t ph[kChunkTokens / 8][4], pl[kChunkTokens / 8][4];
 #pragma unroll
@@ -234,10 +308,10 @@ __global__ void __launch_bounds__(kChunkThreads) chunk_mma_kernel(const ChunkArg
         if (LO) mma_tf32(acc, ph[u], vl);
         mma_tf32(acc, ph[u], vh);
       }
-      o[n][0] = fmaf(o[n][0], f_lo, acc[0]);
-      o[n][1] = fmaf(o[n][1], f_lo, acc[1]);
-      o[n][2] = fmaf(o[n][2], f_hi, acc[2]);
-      o[n][3] = fmaf(o[n][3], f_hi, acc[3]);
+      o[n][0] = fmaf(o[n][0], g_lo, acc[0]);
+      o[n][1] = fmaf(o[n][1], g_lo, acc[1]);
+      o[n][2] = fmaf(o[n][2], g_hi, acc[2]);
+      o[n][3] = fmaf(o[n][3], g_hi, acc[3]);
     }
   }
 

@@ -117,6 +117,97 @@ def test_scores_far_past_the_usual_range(cuda, dtype, size):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [2, 70])
+def test_infinite_keys_and_values(cuda, dtype, rows):
+    """A key whose score is -inf has weight 0 and no other effect; a value that is
+    infinite makes its column infinite for the rows that see it; a key whose
+    score is +inf makes the row NaN. In whole steps and in masked ones."""
+    g = _gen(cuda, 3)
+    B, T, H, Hkv, n, d = 1, rows, 4, 2, 700, 128
+    K, V = _randn((B, Hkv, n, d), g), _randn((B, Hkv, n, d), g)
+    q = _randn((B, T, H, d), g).abs().add(0.01)
+    q[..., 1] *= -1
+    q = q.to(dtype)
+    gone = [3, 300, n - T - 1, n - T + 1 if T > 2 else n - T]
+    want_v = V.clone()
+    for t in gone:
+        K[..., t, 0] = -math.inf
+        K[..., t, 1] = math.inf if t == 300 else 1.0  # negative queries: also -inf
+    cols = {17: (200, math.inf), 18: (n - T, -math.inf), 19: (n - 1, math.inf), 64: (0, -math.inf)}
+    for c, (t, x) in cols.items():
+        want_v[..., t, c] = 0
+        V[..., t, c] = x
+    for place in (HEAD, TOKEN16):
+        cache = api.KVCache.from_logical(K, V, fmt=FMT_F16, place=place)
+        k, v = (x.double() for x in api.gather(cache, n))
+        plain = v.clone().nan_to_num(0.0, 0.0, 0.0)
+        for splits in (1, 2, 3):
+            got = _attend(q, cache, splits)
+            for h in range(H):
+                s = (q[0, :, h].double() @ k[0, :, h // 2].T).div(math.sqrt(d))
+                last = n - T + torch.arange(T, device=cuda)
+                hidden = torch.arange(n, device=cuda) > last[:, None]
+                p = torch.softmax(s.masked_fill(hidden, -math.inf), -1)
+                assert not p.isnan().any() and not p[:, gone].any()
+                want = p @ plain[0, :, h // 2]
+                for c, (t, x) in cols.items():
+                    want[last >= t, c] = x if t not in gone else math.nan
+                fine, inf = want.isfinite(), want.isinf()
+                mine = got[0, :, h].double()
+                assert torch.equal(mine.isfinite(), fine), f"splits {splits}"
+                tol = 2.0 ** -14 if dtype == torch.float32 else 2.0 ** -7
+                assert bool(((mine - want)[fine].abs() <= tol).all())
+                if dtype == torch.float32:  # 16-bit queries: infinite or NaN, since their weights are rounded (0 * inf)
+                    assert torch.equal(mine[inf], want[inf]) and torch.equal(mine.isnan(), want.isnan())
+    K[..., 400, 0] = math.inf
+    cache = api.KVCache.from_logical(K, V, fmt=FMT_F16, place=TOKEN16)
+    for splits in (1, 2):
+        assert bool(_attend(q, cache, splits).isnan().all())
+    assert api.device_errors() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("fmt,group,d", [(FMT_INT8, 64, 128), (FMT_INT4, 32, 128), (FMT_INT8, 64, 64), (FMT_INT4, 64, 64)])
+@pytest.mark.parametrize("rows", [3, 70])
+def test_quantized_values_past_fp16(cuda, dtype, fmt, group, d, rows):
+    """Groups of a quantized cache that hold values past 65504, or whose scale or
+    zero is infinite, at late tokens: rows that do not see them are those of a
+    cache without them, bit for bit or in another order of the same sums."""
+    g = _gen(cuda, 4)
+    B, T, H, Hkv, n = 2, rows, 4, 2, 500
+    K, V = _randn((B, Hkv, n, d), g), _randn((B, Hkv, n, d), g)
+    lens = [500, 389]
+    K2, V2 = K.clone(), V.clone()
+    first = []
+    for b, kv in enumerate(lens):
+        K2[b, :, kv:], V2[b, :, kv:] = 1e30, -1e30            # nobody's
+        V2[b, 0, kv - 1, : group] = torch.linspace(0, 2e5, group, device=cuda)   # finite, past fp16
+        V2[b, 1, kv - 1, : group] = torch.linspace(-1e30, 1e30, group, device=cuda)  # scale and zero infinite
+        K2[b, 1, kv - 1, d - group:] = torch.linspace(-1e30, 1e30, group, device=cuda)
+        first.append(kv - 1)
+    for place in (HEAD, TOKEN16):
+        a = api.KVCache.from_logical(K, V, fmt=fmt, group=group, place=place)
+        c = api.KVCache.from_logical(K2, V2, fmt=fmt, group=group, place=place)
+        a.seq_lens = c.seq_lens = torch.tensor(lens, dtype=torch.int32, device=cuda)
+        q = _randn((B, T, H, d), g, dtype)
+        for splits in (1, 2, 3, 4):
+            x, y = _attend(q, a, splits), _attend(q, c, splits)
+            tol = 2.0 ** -7 if dtype == torch.bfloat16 else 2.0 ** -9 if dtype == torch.float16 else 2.0 ** -17
+            early, late = slice(0, T - 1), T - 1
+            assert bool(y[:, early].isfinite().all()), f"splits {splits}"
+            assert bool(((x - y)[:, early].abs() <= tol * (x[:, early].abs() + 1)).all()), f"splits {splits}"
+            # the last row of heads 0, 1 sees values up to 2e5, heads 2, 3 a NaN key
+            assert bool(y[:, late, 2:].isnan().all())
+            big = y[:, late, :2, : group]
+            assert bool(y[:, late, :2, group:].isfinite().all())
+            if dtype == torch.float32:
+                assert bool(big.isfinite().all()) and bool((big[..., -1] > 0).all())
+            else:
+                assert bool((big[..., -1] == math.inf).all()) and bool(big[..., 0].isfinite().all())
+    assert api.device_errors() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("fmt,group", [(FMT_F16, 0), (FMT_INT8, 64)])
 @pytest.mark.parametrize("rows", [5, 90])
 def test_rows_do_not_depend_on_their_neighbours(cuda, dtype, fmt, group, rows):
@@ -133,3 +224,19 @@ def test_rows_do_not_depend_on_their_neighbours(cuda, dtype, fmt, group, rows):
             y = _attend(torch.where(other[..., None], q * mul, q), cache, splits, lse=lse2)
             assert torch.equal(x[~other], y[~other]) and torch.equal(lse[~other], lse2[~other])
     assert api.device_errors() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("fmt,group", [(FMT_F16, 0), (FMT_INT8, 64)])
+def test_the_greatest_query(cuda, dtype, fmt, group):
+    """A channel of the type's greatest number against zero keys adds nothing."""
+    g = _gen(cuda, 8)
+    B, T, H, Hkv, n, d = 1, 9, 4, 2, 200, 64
+    K = _randn((B, Hkv, n, d), g).abs()  # a group's least value is its zero point: zero is stored as zero
+    K[..., 5] = 0
+    cache = api.KVCache.from_logical(K, _randn((B, Hkv, n, d), g), fmt=fmt, group=group, place=TOKEN)
+    q = _randn((B, T, H, d), g, dtype)
+    q[..., 5] = 0
+    want = api.chunk_attention(q, cache)
+    q[..., 5] = torch.finfo(dtype).max
+    assert torch.equal(api.chunk_attention(q, cache), want)
