@@ -335,9 +335,10 @@ __global__ void __launch_bounds__(kChunkThreads) chunk_mma_kernel(const __grid_c
         *reinterpret_cast<float2 *>(po + 8 * n + 2 * t4) = make_float2(o[n][2 * half], o[n][2 * half + 1]);
       continue;
     }
-    // a row that sees nothing: zeros and -inf
-    const float inv = m == -INFINITY ? 0.f : 1.f / l;
-    if (a.lse && t4 == 0) a.lse[at] = m == -INFINITY ? -INFINITY : m + log2f(l);
+    // a row that sees nothing: zeros and -inf (NaN scores leave m at -inf too, but not l at 0)
+    const bool none = m == -INFINITY && l == 0.f;
+    const float inv = none ? 0.f : 1.f / l;
+    if (a.lse && t4 == 0) a.lse[at] = none ? -INFINITY : m + log2f(l);
     float *out = reinterpret_cast<float *>(chunk_row(a.out, a, w, r));
 #pragma unroll
     for (int n = 0; n < D / 8; ++n) {

@@ -240,3 +240,25 @@ def test_the_greatest_query(cuda, dtype, fmt, group):
     want = api.chunk_attention(q, cache)
     q[..., 5] = torch.finfo(dtype).max
     assert torch.equal(api.chunk_attention(q, cache), want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("splits", [1, 2, 3])
+def test_nan_queries(cuda, dtype, splits):
+    """A NaN query's row is NaN, and so is its lse (-inf is for rows that see nothing)."""
+    g = _gen(cuda, 5)
+    B, T, H, Hkv, n, d = 2, 5, 4, 2, 300, 64
+    cache = api.KVCache.from_logical(_randn((B, Hkv, n, d), g), _randn((B, Hkv, n, d), g), fmt=FMT_INT8, group=64, place=TOKEN16)
+    cache.seq_lens = torch.tensor([300, 3], dtype=torch.int32, device=cuda)
+    q = _randn((B, T, H, d), g, dtype)
+    clean_lse = torch.zeros((B, T, H), device=cuda)
+    clean = _attend(q, cache, splits, lse=clean_lse)
+    bad = torch.zeros((B, T, H), dtype=torch.bool, device=cuda)
+    bad[0, 1, 2] = bad[1, 4, 0] = bad[1, 0, 1] = True  # the last one sees nothing
+    q[bad] = math.nan
+    lse = torch.zeros((B, T, H), device=cuda)
+    got = _attend(q, cache, splits, lse=lse)
+    sees = clean_lse > -math.inf
+    assert bool(got[bad & sees].isnan().all()) and bool(lse[bad & sees].isnan().all())
+    assert not got[bad & ~sees].any() and bool((lse[bad & ~sees] == -math.inf).all())
+    assert torch.equal(got[~bad], clean[~bad]) and torch.equal(lse[~bad], clean_lse[~bad])
