@@ -445,7 +445,8 @@ cudaError_t kvf_b200_chunk_attention(const kvf_args *a, int fmt, int d, int ord,
 
 /* The splits of each sequence's tokens that kvf_b200_chunk_attention runs best
  * with for this shape (dtype: KVF_DT_* of the queries; n: the longest
- * sequence). At least 1. */
+ * sequence). At least 1; more than 1 only where their partials take at most
+ * 512 MiB and the model of their cost says that they pay. */
 int kvf_b200_chunk_splits(int B, int T, int H, int Hkv, int n, int fmt, int d, int dtype);
 
 /* Bytes of device scratch behind kvf_b200_decode_noalloc (8 MiB). */

@@ -108,10 +108,18 @@ ChunkRows chunk_rows(const kvf_heads &r) {
                    rows_aligned(r) ? 1 : 0};
 }
 
-// Splits of each tile's tokens. Tensor-core kernel: the blocks run one per SM,
-// a block costs its steps and about six more to start and end, and writing and
-// merging partials about sixteen; the count that makes the waves shortest.
-int pick_splits(int B, int T, int H, int Hkv, int n, int dtype) {
+// Splits of each tile's tokens. Tensor-core kernel: the blocks run one per SM, and
+// a block costs its steps and about six more to start and end. Splits cost a merge,
+// about sixteen steps for its launch and one for each 8 MB of partials written or
+// read. One row tile without splits leaves a softmax group idle: its steps take
+// 1.15 times as long. The count that makes the whole shortest, the least of equals,
+// with at most kPartialBytes of partials. Measured against the neighbouring counts
+// (int8, 128 channels): 64 x 4 tokens of 64 heads over 16384: 768 us with 4,
+// 886 with 1, 816 with 2, 831 with 6; 512 x 16 over 1024: 774 with 1, 962 with 2;
+// 64 x 512 over 65536: 74.9 ms with 1, 76.0 with 2; 1 x 2048 tokens of 32 heads
+// over 131072: 4.28 ms with 4, 4.57 with 1.
+constexpr double kPartialBytes = 512.0 * (1 << 20);
+int pick_splits(int B, int T, int H, int Hkv, int n, int d, int dtype) {
   const long long rows = (long long)T * (H / Hkv);
   const int sms = device_sm_count();
   if (dtype == KVF_DT_F32) {
@@ -123,16 +131,20 @@ int pick_splits(int B, int T, int H, int Hkv, int n, int dtype) {
   const bool one = rows <= kTcRows;
   const long long blocks = (rows + 2 * kTcRows - 1) / (2 * kTcRows) * B * Hkv;
   const int steps = (n + kTcStep - 1) / kTcStep;
-  long long best = -1;
-  int s = 1;
+  auto waves = [&](int k) { return (double)((blocks * k + sms - 1) / sms); };
+  int best = 1;
+  double cost = waves(1) * (one ? 1.15 * steps + 6 : steps + 6.0);
   for (int k = 1; k <= std::min(64, std::max(1, steps / 2)); ++k) {
-    const long long cost = (blocks * k + sms - 1) / sms * ((steps + k - 1) / k + 6) + (k > 1 ? 16 : 0);
-    if (best < 0 || cost < best) {
-      best = cost;
-      s = k;
+    const int s = one ? 2 * k : k;
+    const double bytes = (double)B * T * H * s * (d + 2) * 4;
+    if (s == 1 || bytes > kPartialBytes) continue;
+    const double x = waves(k) * ((steps + k - 1) / k + 6) + 16 + 2 * bytes / 8e6;
+    if (x < cost) {
+      cost = x;
+      best = s;
     }
   }
-  return one ? 2 * s : s;
+  return best;
 }
 
 } // namespace
@@ -156,7 +168,7 @@ extern "C" int kvf_b200_chunk_splits(int B, int T, int H, int Hkv, int n, int fm
   if (B <= 0 || T <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || n <= 0 || fmt < 0 || fmt > 2 || (d != 64 && d != 128) ||
       dtype < KVF_DT_F32 || dtype > KVF_DT_BF16)
     return 1;
-  return pick_splits(B, T, H, Hkv, n, dtype);
+  return pick_splits(B, T, H, Hkv, n, d, dtype);
 }
 
 extern "C" cudaError_t kvf_b200_chunk_attention(const kvf_args *args, int fmt, int d, int ord, int paged,
