@@ -457,13 +457,17 @@ class ChunkWorkspace:
     part_ml: Optional[torch.Tensor]
 
     @classmethod
-    def allocate(cls, cache: KVCache, T: int, H: int, dtype: torch.dtype, splits: Optional[int] = None) -> "ChunkWorkspace":
+    def allocate(cls, cache: KVCache, T: int, H: int, dtype: torch.dtype, splits: Optional[int] = None,
+                 n: Optional[int] = None) -> "ChunkWorkspace":
         """For chunks of at most T tokens with H query heads of `dtype`; splits
-        defaults to kvf_b200_chunk_splits."""
+        defaults to kvf_b200_chunk_splits for sequences of n tokens (default: as
+        many as the cache has room for). A cache that is mostly empty is split
+        for nothing: give the longest length there is to come. Longer sequences
+        are right too."""
         dev, B, d = cache.k.device, cache.B, cache.d
         if splits is None:
             with torch.cuda.device(dev):
-                splits = int(lib().kvf_b200_chunk_splits(B, T, H, cache.Hkv, cache.n, cache.fmt, d, DTYPES[dtype]))
+                splits = int(lib().kvf_b200_chunk_splits(B, T, H, cache.Hkv, n or cache.n, cache.fmt, d, DTYPES[dtype]))
         if splits <= 1:
             return cls(1, None, None)
         return cls(splits, torch.empty((B, T, H, splits, d), dtype=torch.float32, device=dev),

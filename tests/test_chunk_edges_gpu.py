@@ -262,3 +262,20 @@ def test_nan_queries(cuda, dtype, splits):
     assert bool(got[bad & sees].isnan().all()) and bool(lse[bad & sees].isnan().all())
     assert not got[bad & ~sees].any() and bool((lse[bad & ~sees] == -math.inf).all())
     assert torch.equal(got[~bad], clean[~bad]) and torch.equal(lse[~bad], clean_lse[~bad])
+
+
+def test_workspace_for_what_is_stored(cuda):
+    """A long cache that holds little: splits by the lengths that are to come, and
+    right for longer ones."""
+    g = _gen(cuda, 9)
+    B, T, H, Hkv, n, d = 1, 16, 8, 2, 20000, 128
+    cache = api.KVCache.from_logical(_randn((B, Hkv, n, d), g), _randn((B, Hkv, n, d), g), fmt=FMT_F16, place=TOKEN)
+    q = _randn((B, T, H, d), g, torch.bfloat16)
+    assert api.ChunkWorkspace.allocate(cache, T, H, q.dtype).splits > 4
+    ws = api.ChunkWorkspace.allocate(cache, T, H, q.dtype, n=100)
+    assert ws.splits == 1 and ws.part_o is None
+    for length in (100, n):
+        cache.seq_lens = torch.tensor([length], dtype=torch.int32, device=cuda)
+        a, b = api.chunk_attention(q, cache, workspace=ws), api.chunk_attention(q, cache)
+        # weights and their sums are rounded alike, but summed in another order: a step of bf16 apart at most
+        assert bool(((a.float() - b.float()).abs() <= 2.0 ** -7 * b.float().abs() + 2.0 ** -10).all())
