@@ -44,7 +44,9 @@ enum { KVF_ORD_HEAD = 0, KVF_ORD_TOKEN = 1 };
  *                byte c/2, odd columns in the high nibble)
  *   k_meta,v_meta [rows][D/group] words, each (scale | zero << 16) as fp16
  *                (a __half2 with .x = scale); quantized formats only
- *   block_table  [B][max_blocks] page ids, paged layouts only
+ *   block_table  [B][max_blocks] page ids, paged layouts only; negative where no
+ *                page is mapped. Blocks that hold stored tokens must be mapped
+ *                (decode reads page 0 in place of one that is not)
  *   out          [B][H][D] fp32
  *   part_o       [B][H][splits][D] fp32 workspace, used when splits > 1
  *   part_ml      [B][H][splits][2] fp32 workspace (running max in log2 units,

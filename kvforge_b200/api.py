@@ -99,7 +99,11 @@ class KVCache:
     @classmethod
     def from_logical(cls, K: torch.Tensor, V: torch.Tensor, *, fmt: int, group: int = 0,
                      place: Placement, seq_lens=None, table_seed: int = 18) -> "KVCache":
-        """Build a cache from logical float32 K, V [B][Hkv][n][D] on a CUDA device."""
+        """Build a cache from logical float32 K, V [B][Hkv][n][D] on a CUDA device.
+
+        Paged with seq_lens: only the blocks that hold stored tokens get a page;
+        the others' table entries are -1, and tokens appended there are skipped and
+        reported until the caller maps them."""
         B, Hkv, n, d = K.shape
         dev = K.device
         kq, km = quantize(K, fmt, group)

@@ -564,6 +564,8 @@ decode_kernel(const kvf_args a, const Plan p, const __grid_constant__ CUtensorMa
     const int h0 = hgi * p.hh;
     const uint32_t *kmeta = reinterpret_cast<const uint32_t *>(a.k_meta);
     const uint32_t *vmeta = reinterpret_cast<const uint32_t *>(a.v_meta);
+    // A negative page (none mapped) is read as page 0, so that lengths past the
+    // mapped blocks stay inside the cache.
     // Block-table window: pages of blocks [win, win + 96) in three registers
     // per lane, loaded one window ahead of use, so a stage's page lookup is
     // two shuffles and never waits for memory.
@@ -618,7 +620,7 @@ decode_kernel(const kvf_args a, const Plan p, const __grid_constant__ CUtensorMa
         const int idx = blk0 - win + (lane < p.npg ? lane : 0);  // < 32 + 4
         const int from_cur = __shfl_sync(0xffffffffu, pg_cur, idx & 31);
         const int from_nxt = __shfl_sync(0xffffffffu, pg_nxt, idx & 31);
-        lanepage = idx < 32 ? from_cur : from_nxt;
+        lanepage = max(idx < 32 ? from_cur : from_nxt, 0);
       }
       if (lane == 0) ptx::mbar_arrive_expect_tx(bar_full + 8u * s, p.tx_bytes);
 #pragma unroll

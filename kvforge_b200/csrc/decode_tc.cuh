@@ -261,7 +261,8 @@ decode_tc_kernel(const kvf_args a, const TcPlan p, const __grid_constant__ CUten
     const int nblk_valid = p.paged ? min(a.max_blocks, (nb + bmask) >> p.bt_shift) : 0;
     const long long tab0 = (long long)b * a.max_blocks;
     // Block-table window: pages of blocks [win, win + 96) in three registers
-    // per lane, loaded one window ahead of use.
+    // per lane, loaded one window ahead of use; a negative page (none mapped) is
+    // read as page 0, so that lengths past the mapped blocks stay inside the cache.
     int win = p.paged ? (t0 >> p.bt_shift) : 0;
     int pg_cur = 0, pg_nxt = 0, pg_nn = 0;
     if (p.paged) {
@@ -288,7 +289,7 @@ decode_tc_kernel(const kvf_args a, const TcPlan p, const __grid_constant__ CUten
         const int idx = blk0 - win + (lane < p.npg ? lane : 0);  // < 32 + 8
         const int from_cur = __shfl_sync(0xffffffffu, pg_cur, idx & 31);
         const int from_nxt = __shfl_sync(0xffffffffu, pg_nxt, idx & 31);
-        lanepage = idx < 32 ? from_cur : from_nxt;
+        lanepage = max(idx < 32 ? from_cur : from_nxt, 0);
       }
       // Metadata rows of tokens lane + 32k of the stage (null past the chunk,
       // where the row is zero-filled instead).

@@ -33,7 +33,9 @@ def page_table(B: int, n: int, bt: int, seed: int, seq_lens=None) -> tuple[np.nd
 
     Without seq_lens every sequence owns ceil(n/bt) pages (upload_cache,
     kvf_host.h:157-165). With seq_lens a sequence owns ceil(n_b/bt) pages and the
-    unused table entries are 0. The pages are a seeded random permutation."""
+    unused table entries are -1: no page, so that a token appended there is
+    skipped and reported instead of landing in another sequence's page. The pages
+    are a seeded random permutation."""
     max_blocks = (n + bt - 1) // bt
     if seq_lens is None:
         need = np.full(B, max_blocks, dtype=np.int64)
@@ -41,7 +43,7 @@ def page_table(B: int, n: int, bt: int, seed: int, seq_lens=None) -> tuple[np.nd
         need = (np.asarray(seq_lens, dtype=np.int64) + bt - 1) // bt
     pages = int(need.sum())
     perm = np.random.default_rng(seed).permutation(pages).astype(np.int32)
-    table = np.zeros((B, max(max_blocks, 1)), dtype=np.int32)
+    table = np.full((B, max(max_blocks, 1)), -1, dtype=np.int32)
     off = 0
     for b in range(B):
         table[b, : need[b]] = perm[off : off + need[b]]
