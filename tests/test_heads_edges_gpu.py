@@ -23,6 +23,94 @@ def _randn(shape, g, dtype=torch.float32):
     return torch.randn(shape, generator=g, device=g.device).to(dtype)
 
 
+def _rotated(x, pos, rope, weight):
+    """norm_rope in fp32 torch operations, one rounding each, the squares in a tree of neighbours."""
+    x = x.float()
+    T, d = x.shape[1], x.shape[-1]
+    if weight is not None:
+        s = x * x
+        while s.shape[-1] > 1:
+            s = s[..., 0::2] + s[..., 1::2]
+        x = x * (1.0 / torch.sqrt(s / d + 1e-6)) * weight.float()
+    if rope is None:
+        return x
+    y, r = x.clone(), 2 * rope.cos.shape[1]
+    at = pos[:, None].long() + torch.arange(T, device=x.device)
+    c, s = rope.cos[at][:, :, None], rope.sin[at][:, :, None]
+    u, w = x[..., : r // 2], x[..., r // 2: r]
+    y[..., : r // 2], y[..., r // 2: r] = u * c - w * s, u * s + w * c
+    return y
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,heads,d,rot", [
+    (2100, 8, 128, 128), (2100, 8, 128, 64), (5000, 16, 128, 128), (5000, 16, 128, 64), (5000, 15, 128, 128),
+    (2100, 16, 64, 64), (5000, 32, 64, 64), (5000, 32, 64, 32), (5000, 31, 64, 64), (1, 3, 128, 128)])
+def test_every_number_of_rows_per_lane(cuda, dtype, T, heads, d, rot):
+    """Long calls take two, four (fp32) or eight (16-bit) rows per lane group, by how
+    many heads fill them; rotated whole or in part, normed or not."""
+    g = _gen(cuda, 1)
+    B = 3
+    x = _randn((B, T, heads, d), g, dtype)
+    w = (1 + 0.1 * _randn((d,), g)).to(dtype)
+    rope = api.Rope.build(T + 50, rot, device=cuda)
+    pos = torch.tensor([0, 49, 7], dtype=torch.int32, device=cuda)
+    for weight, r in ((None, rope), (w, rope), (w, None)):
+        got = api.norm_rope(x, None if r is None else pos, r, weight=weight)
+        assert torch.equal(got, _rotated(x, pos, r, weight).to(dtype))
+    assert api.device_errors() == 0
+
+
+def test_rows_beside_a_position_outside_the_table(cuda):
+    """What is inside is rotated as ever, in every row."""
+    g = _gen(cuda, 2)
+    rope = api.Rope.build(10, 64, device=cuda)
+    x = _randn((3, 4, 2, 64), g)
+    pos = torch.tensor([8, -2, 3], dtype=torch.int32, device=cuda)
+    out = torch.full_like(x, 7.0)
+    api.norm_rope(x, pos, rope, out=out)
+    assert api.device_errors() == 4 and api.device_errors() == 0
+    for b in range(3):
+        for t in range(4):
+            p = int(pos[b]) + t
+            want = torch.full_like(x[b, t], 7.0)
+            if 0 <= p < 10:
+                want = _rotated(x[b: b + 1, t: t + 1], torch.tensor([p], device=cuda), rope, None)[0, 0]
+            assert torch.equal(out[b, t], want)
+
+@pytest.mark.parametrize("fmt,group", FORMATS)
+@pytest.mark.parametrize("order", [ORD_HEAD, ORD_TOKEN])
+def test_append_past_the_mapped_blocks(cuda, fmt, group, order):
+    """A cache built with lengths maps the blocks of stored tokens only: tokens
+    appended past those are skipped and reported, and no other sequence's page is
+    touched."""
+    g = _gen(cuda, 3)
+    B, Hkv, n, d = 3, 2, 80, 64
+    lens = [33, 1, 16]
+    K, V = _randn((B, Hkv, n, d), g), _randn((B, Hkv, n, d), g)
+    group = min(group, d)
+    for call in ("append", "append_rope"):
+        cache = api.KVCache.from_logical(K, V, fmt=fmt, group=group, place=Placement(order, True, 16), seq_lens=lens)
+        before = api.gather(cache, n)
+        T = 20
+        k, v = _randn((B, T, Hkv, d), g), _randn((B, T, Hkv, d), g)
+        if call == "append":
+            api.append(cache, k.transpose(1, 2), v.transpose(1, 2))
+        else:
+            api.append_rope(cache, k, v)
+        assert api.device_errors() == 4
+        # the mapped blocks hold 48, 16 and 16 tokens: 15, 15 and 0 of the 20 fit
+        cache.seq_lens = torch.tensor([48, 16, 16], dtype=torch.int32, device=cuda)
+        after = api.gather(cache, n)
+        assert api.device_errors() == 0
+        kq, vq = (api.KVCache.from_logical(x.transpose(1, 2).contiguous(), x.transpose(1, 2).contiguous(), fmt=fmt, group=group,
+                                           place=Placement(ORD_TOKEN, False, 0)) for x in (k, v))
+        for was, now, new in zip(before, after, (api.gather(kq, T)[0], api.gather(vq, T)[0])):
+            for b, (m, fit) in enumerate(zip(lens, (15, 15, 0))):
+                assert torch.equal(now[b, :m], was[b, :m])
+                assert torch.equal(now[b, m: m + fit], new[b, :fit])
+
+
 @pytest.mark.parametrize("fmt,group", FORMATS)
 def test_decode_of_blocks_without_a_page_stays_in_the_cache(cuda, fmt, group):
     """Lengths past the mapped blocks (an append that was reported, whose error
