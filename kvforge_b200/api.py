@@ -137,6 +137,28 @@ class KVCache:
         return cache
 
 
+    @classmethod
+    def empty(cls, B: int, Hkv: int, n: int, d: int, *, fmt: int, group: int = 0, place: Placement, device="cuda",
+              table_seed: int = 18) -> "KVCache":
+        """A cache that holds no tokens yet, with room for n of every sequence: every
+        block has a page, every length is 0. append_rope and append fill it."""
+        table, max_blocks, pages = None, 0, 0
+        if place.paged:
+            table, max_blocks, pages = layout.page_table(B, n, place.block_tokens, table_seed)
+            table = torch.from_numpy(table).to(device)
+        rows, gpr = layout.rows_alloc(B, Hkv, n, place, pages), groups_per_row(fmt, d, group)
+
+        def zeros(width, dtype):
+            return torch.zeros((rows, width), dtype=dtype, device=device)
+
+        return cls(
+            fmt=fmt, d=d, group=group, place=place, B=B, Hkv=Hkv, n=n,
+            k=zeros(row_bytes(fmt, d), torch.uint8), v=zeros(row_bytes(fmt, d), torch.uint8),
+            k_meta=zeros(gpr, torch.int32) if gpr else None, v_meta=zeros(gpr, torch.int32) if gpr else None,
+            block_table=table, max_blocks=max_blocks, seq_lens=torch.zeros(B, dtype=torch.int32, device=device),
+        )
+
+
 @dataclass
 class Workspace:
     """Split partials: part_o [B][H][splits][D] and part_ml [B][H][splits][2].

@@ -131,3 +131,32 @@ def test_decode_of_blocks_without_a_page_stays_in_the_cache(cuda, fmt, group):
             rest = [0, 1, 2, 4, 5, 7]
             assert float((got[rest] - want[rest]).abs().max()) < 1e-4
         assert api.device_errors() == 0
+
+
+@pytest.mark.parametrize("fmt,group", FORMATS)
+@pytest.mark.parametrize("place", [Placement(ORD_HEAD, False, 0), Placement(ORD_TOKEN, True, 16)], ids=lambda p: p.name)
+def test_an_empty_cache_is_filled(cuda, fmt, group, place):
+    """KVCache.empty holds no tokens and room for n of every sequence: filled by
+    append_rope it is the cache that from_logical makes."""
+    g = _gen(cuda, 5)
+    B, H, Hkv, n, d = 3, 8, 2, 50, 128
+    cache = api.KVCache.empty(B, Hkv, n, d, fmt=fmt, group=group, place=place, device=cuda)
+    assert cache.seq_lens.tolist() == [0] * B and cache.payload_bytes() == 0
+    q = _randn((B, H, d), g)
+    assert not api.decode(q, cache).any()
+    k, v = _randn((B, n, Hkv, d), g), _randn((B, n, Hkv, d), g)
+    lens = torch.tensor([17, 0, 50], dtype=torch.int32, device=cuda)
+    api.append_rope(cache, k, v, lens=lens)
+    assert cache.seq_lens.tolist() == [17, 0, 50]
+    rest = [(17, 33), (0, 50), (50, 0)]
+    pad = torch.zeros_like(k), torch.zeros_like(v)
+    for b, (m, r) in enumerate(rest):
+        for x, y in zip(pad, (k, v)):
+            x[b, :r] = y[b, m:]
+    api.append_rope(cache, *pad, lens=torch.tensor([r for _, r in rest], dtype=torch.int32, device=cuda))
+    assert cache.seq_lens.tolist() == [n] * B and api.device_errors() == 0
+    full = api.KVCache.from_logical(k.transpose(1, 2).contiguous(), v.transpose(1, 2).contiguous(), fmt=fmt, group=group,
+                                    place=place)
+    for x, y in zip(api.gather(cache, n), api.gather(full, n)):
+        assert torch.equal(x, y)
+    assert float((api.decode(q, cache) - api.decode(q, full)).abs().max()) < 1e-5
