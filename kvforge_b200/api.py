@@ -306,6 +306,14 @@ def _launch(fn: str, device: torch.device, stream, *args) -> None:
     check(fn, getattr(lib(), fn)(*args, s))
 
 
+def _no_graph(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Refuses tensors whose gradients would be lost: these calls build no autograd graph."""
+    if torch.is_grad_enabled():
+        for x in tensors:
+            if x is not None and x.requires_grad:
+                raise ValueError(f"{what} has no backward pass: call it under torch.no_grad(), or with detached tensors")
+
+
 def _heads(x: torch.Tensor, what: str, device: torch.device, shape=None) -> KvfHeads:
     size = x.shape
     if len(size) != 4 or (shape is not None and size != shape):
@@ -386,6 +394,7 @@ def norm_rope(x: torch.Tensor, pos: Optional[torch.Tensor], rope: Optional[Rope]
     not read, and in `out` left as they were. out (default: a new tensor,
     zero there) may be x. A position outside the table leaves its rows unwritten
     and sets bit 2 of device_errors()."""
+    _no_graph("norm_rope", x, weight, out)
     xs = _heads(x, "x", x.device)
     B, T, H, d = x.shape
     if weight is None and rope is None:
@@ -420,6 +429,7 @@ def append_rope(cache: KVCache, k: torch.Tensor, v: torch.Tensor, rope: Optional
     stream); a given pos leaves seq_lens alone. Tokens outside the cache or the
     table are skipped and set bit 2 of device_errors()."""
     dev = cache.k.device
+    _no_graph("append_rope", k, v, q, k_weight, q_weight, q_out)
     if k.dim() != 4 or (k.shape[0], k.shape[2], k.shape[3]) != (cache.B, cache.Hkv, cache.d):
         raise ValueError(f"k must be [B][T][Hkv][D] with B={cache.B}, Hkv={cache.Hkv}, D={cache.d}")
     B, T, Hkv, d = k.shape
@@ -464,6 +474,7 @@ def gather(cache: KVCache, T: int, *, pos: Optional[torch.Tensor] = None, lens: 
     if out is None:
         out = tuple(_output(cache.k, shape, dtype, stream) for _ in range(2))
     k, v = out
+    _no_graph("gather", k, v)
     if k.dtype != v.dtype:
         raise ValueError("both outputs must have one type")
     _launch("kvf_b200_gather", dev, stream, ctypes.byref(_cache_args(cache)), cache.fmt, cache.d, cache.place.order,
@@ -515,6 +526,7 @@ def chunk_attention(q: torch.Tensor, cache: KVCache, *, q_lens: Optional[torch.T
     lse (float32 [B][T][H], contiguous) receives log2 of each softmax
     denominator. workspace (ChunkWorkspace.allocate) saves its allocation here."""
     dev = cache.k.device
+    _no_graph("chunk_attention", q, out)
     qs = _heads(q, "q", dev)
     B, T, H, d = q.shape
     if (B, d) != (cache.B, cache.d) or H == 0 or H % cache.Hkv:

@@ -160,3 +160,33 @@ def test_an_empty_cache_is_filled(cuda, fmt, group, place):
     for x, y in zip(api.gather(cache, n), api.gather(full, n)):
         assert torch.equal(x, y)
     assert float((api.decode(q, cache) - api.decode(q, full)).abs().max()) < 1e-5
+
+
+def test_tensors_that_want_gradients_are_refused(cuda):
+    """No call around the cache has a backward pass: a graph would end here without a word."""
+    g = _gen(cuda, 6)
+    B, T, H, Hkv, n, d = 1, 3, 4, 2, 16, 64
+    cache = api.KVCache.empty(B, Hkv, n, d, fmt=FMT_F16, place=Placement(ORD_TOKEN, False, 0), device=cuda)
+    q, k, v = _randn((B, T, H, d), g), _randn((B, T, Hkv, d), g), _randn((B, T, Hkv, d), g)
+    w = torch.ones(d, device=cuda)
+    pos = torch.zeros(B, dtype=torch.int32, device=cuda)
+
+    def wants(x):
+        return x.clone().requires_grad_()
+
+    calls = [lambda f: api.norm_rope(f(q), None, weight=w), lambda f: api.norm_rope(q, None, weight=f(w)),
+             lambda f: api.norm_rope(q, None, weight=w, out=f(q)),
+             lambda f: api.append_rope(cache, f(k), v, pos=pos), lambda f: api.append_rope(cache, k, f(v), pos=pos),
+             lambda f: api.append_rope(cache, k, v, pos=pos, k_weight=f(w)),
+             lambda f: api.append_rope(cache, k, v, pos=pos, q=f(q), q_weight=w),
+             lambda f: api.append_rope(cache, k, v, pos=pos, q=q, q_weight=f(w)),
+             lambda f: api.append_rope(cache, k, v, pos=pos, q=q, q_out=f(q)),
+             lambda f: api.gather(cache, T, out=(f(k), v)),
+             lambda f: api.chunk_attention(f(q), cache), lambda f: api.chunk_attention(q, cache, out=f(q))]
+    for call in calls:
+        with pytest.raises(ValueError, match="backward"):
+            call(wants)
+        call(lambda x: x)
+        with torch.no_grad():
+            call(wants)
+    assert api.device_errors() == 0
