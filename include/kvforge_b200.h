@@ -438,7 +438,9 @@ cudaError_t kvf_b200_gather(const kvf_args *a, int fmt, int d, int ord, int page
  * [B][T][H][splits][d] (16-byte aligned) and part_ml [B][T][H][splits][2].
  * q, out, split_sem and max-splits rules of kvf_b200_decode do not apply. Blocks
  * that hold seen tokens must be mapped (a negative page's tokens count as
- * zero keys and values); pages hold 16 to 128 tokens. Products of fp32 queries have fp32 accuracy (about
+ * zero keys and values); pages hold 16 to 128 tokens. k_meta and v_meta are
+ * aligned to a row's words, 4 * (d / group) bytes, for fp16 and bf16 queries
+ * (else cudaErrorMisalignedAddress), to 4 bytes for fp32. Products of fp32 queries have fp32 accuracy (about
  * 2^-21 relative). For fp16 and bf16 queries keys, values and softmax weights
  * are rounded to fp16 and the products accumulated in fp32: stored values past
  * 65504 (which a quantized group can hold) count as infinities there. */

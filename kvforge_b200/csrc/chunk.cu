@@ -183,8 +183,10 @@ extern "C" cudaError_t kvf_b200_chunk_attention(const kvf_args *args, int fmt, i
   if (args->B == 0 || T == 0) return cudaSuccess;
   if ((e = check_heads(q)) != cudaSuccess || (e = check_heads(out)) != cudaSuccess) return e;
   if (q->heads != args->H || out->heads != args->H || q->dtype != out->dtype) return cudaErrorInvalidValue;
-  if (group && ((reinterpret_cast<uintptr_t>(args->k_meta) | reinterpret_cast<uintptr_t>(args->v_meta)) &
-                (uintptr_t)(4 * (d / group) - 1)))
+  // 16-bit queries: a row's metadata is copied as one piece (fp32 queries read words)
+  if (group && q->dtype != KVF_DT_F32 &&
+      ((reinterpret_cast<uintptr_t>(args->k_meta) | reinterpret_cast<uintptr_t>(args->v_meta)) &
+       (uintptr_t)(4 * (d / group) - 1)))
     return cudaErrorMisalignedAddress;
   if (paged && (args->block_shift < 4 || args->block_shift > 7 ||
                 (long long)args->max_blocks << args->block_shift < args->n))

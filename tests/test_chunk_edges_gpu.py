@@ -264,6 +264,25 @@ def test_nan_queries(cuda, dtype, splits):
     assert torch.equal(got[~bad], clean[~bad]) and torch.equal(lse[~bad], clean_lse[~bad])
 
 
+@pytest.mark.parametrize("fmt,group,d", [(FMT_INT8, 64, 128), (FMT_INT4, 32, 128)])
+def test_metadata_on_odd_words(cuda, fmt, group, d):
+    """fp32 queries read metadata by words: any 4-byte address will do. 16-bit
+    queries need a row's words on their own alignment."""
+    g = _gen(cuda, 6)
+    B, T, H, Hkv, n = 1, 3, 2, 1, 50
+    cache = api.KVCache.from_logical(_randn((B, Hkv, n, d), g), _randn((B, Hkv, n, d), g), fmt=fmt, group=group, place=TOKEN)
+    q = _randn((B, T, H, d), g)
+    want = api.chunk_attention(q, cache)
+    for name in ("k_meta", "v_meta"):
+        m = getattr(cache, name)
+        odd = torch.zeros(m.numel() + 1, dtype=m.dtype, device=cuda)[1:].view(m.shape)
+        odd.copy_(m)
+        setattr(cache, name, odd)
+    assert torch.equal(api.chunk_attention(q, cache), want)
+    with pytest.raises(api.KvfError):
+        api.chunk_attention(q.half(), cache)
+
+
 def test_workspace_for_what_is_stored(cuda):
     """A long cache that holds little: splits by the lengths that are to come, and
     right for longer ones."""
