@@ -549,8 +549,8 @@ def chunk_attention(q: torch.Tensor, cache: KVCache, *, q_lens: Optional[torch.T
     a.splits = workspace.splits if workspace is not None else 1
     if a.splits > 1:
         for x, e in ((workspace.part_o, d), (workspace.part_ml, 2)):
-            if x.device != dev or x.numel() < B * T * H * a.splits * e:
-                raise ValueError("workspace is too small for this chunk, or on another device")
+            if x.device != dev or x.dtype != torch.float32 or not x.is_contiguous() or x.numel() < B * T * H * a.splits * e:
+                raise ValueError("workspace must be contiguous float32 on the cache's device, and hold this chunk")
         a.part_o, a.part_ml = workspace.part_o.data_ptr(), workspace.part_ml.data_ptr()
     _launch("kvf_b200_chunk_attention", dev, stream, ctypes.byref(a), cache.fmt, d, cache.place.order,
             int(cache.place.paged), ctypes.byref(qs), ctypes.byref(_heads(out, "out", dev, q.shape)), T,

@@ -298,3 +298,18 @@ def test_workspace_for_what_is_stored(cuda):
         a, b = api.chunk_attention(q, cache, workspace=ws), api.chunk_attention(q, cache)
         # weights and their sums are rounded alike, but summed in another order: a step of bf16 apart at most
         assert bool(((a.float() - b.float()).abs() <= 2.0 ** -7 * b.float().abs() + 2.0 ** -10).all())
+
+
+def test_workspaces_that_do_not_hold_the_partials(cuda):
+    """Of another type, with gaps, or too small: refused, since the kernels write all of it."""
+    g = _gen(cuda, 10)
+    B, T, H, Hkv, n, d = 1, 8, 4, 2, 500, 64
+    cache = api.KVCache.from_logical(_randn((B, Hkv, n, d), g), _randn((B, Hkv, n, d), g), fmt=FMT_F16, place=TOKEN)
+    q = _randn((B, T, H, d), g, torch.bfloat16)
+    good = api.ChunkWorkspace.allocate(cache, T, H, q.dtype, splits=4)
+    wide = torch.zeros((*good.part_o.shape[:-1], 2 * d), device=cuda)
+    for part_o, part_ml in ((good.part_o.half(), good.part_ml), (good.part_o, good.part_ml.half()), (wide[..., ::2], good.part_ml),
+                            (good.part_o[:, :-1], good.part_ml), (good.part_o.cpu(), good.part_ml)):
+        with pytest.raises(ValueError):
+            api.chunk_attention(q, cache, workspace=api.ChunkWorkspace(4, part_o, part_ml))
+    assert bool(api.chunk_attention(q, cache, workspace=good).isfinite().all()) and api.device_errors() == 0
