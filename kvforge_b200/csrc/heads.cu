@@ -23,6 +23,8 @@ namespace kvfb {
 // (reported as bit 2 of kvf_b200_device_errors).
 __device__ unsigned g_kvfb_heads_error;
 
+int device_sm_count();  // decode.cu
+
 namespace {
 
 struct Rows {
@@ -376,8 +378,9 @@ cudaError_t launch_heads(HeadsArgs a, cudaStream_t st) {
   const bool cache = a.k.heads > 0;
   auto units = [](int heads, int r) { return (heads + r * RPW - 1) / (r * RPW); };
   const long long pairs = units(a.q.heads, 1) + units(a.k.heads, 1) + units(a.v.heads, 1);
-  int r = tokens * pairs >= 2 * 148 * 32 ? 2 : 1;
-  if (!cache && tokens * pairs >= BIG * 148 * 32 && 4 * a.q.heads >= 3 * units(a.q.heads, BIG) * BIG * RPW) r = BIG;
+  const long long filled = 32LL * device_sm_count();
+  int r = tokens * pairs >= 2 * filled ? 2 : 1;
+  if (!cache && tokens * pairs >= BIG * filled && 4 * a.q.heads >= 3 * units(a.q.heads, BIG) * BIG * RPW) r = BIG;
   a.q_units = units(a.q.heads, r);
   a.k_units = units(a.k.heads, r);
   a.units = a.q_units + a.k_units + units(a.v.heads, r);
