@@ -403,9 +403,10 @@ cudaError_t kvf_b200_norm_rope(const kvf_heads *x, const kvf_heads *out, int B, 
  * stores their fp32 rows, at tokens pos[b] .. pos[b] + lens[b] - 1 of the cache
  * `a` describes (the fields that kvf_b200_append reads). q (NULL = none) takes
  * the same tokens' query heads through q_norm and the rotation into q_out in
- * the same launch. k, v, q and q_out have one type. A token at or past n, past
- * max_blocks, in a block mapped to a negative page, or outside the rotation
- * table is not written and sets bit 2 of kvf_b200_device_errors(). Two tokens
+ * the same launch. k, v, q and q_out have one type. Keys and values of a token at
+ * or past n, past max_blocks or in a block mapped to a negative page are not
+ * written, nor is anything of a token outside the rotation table (or before
+ * position 0); either sets bit 2 of kvf_b200_device_errors(). Two tokens
  * of one call that fall on the same physical row (a page that two sequences
  * share) leave it undefined. */
 cudaError_t kvf_b200_append_rope(const kvf_args *a, int fmt, int d, int ord, int paged, const kvf_heads *k,
@@ -428,8 +429,12 @@ cudaError_t kvf_b200_gather(const kvf_args *a, int fmt, int d, int ord, int page
  * are in the cache already) and ql = q_lens[b] (NULL = T) new tokens: token j
  * is the sequence's token kv - ql + j and sees kv - ql + j + 1 tokens
  * (causal = 1), or all kv (causal = 0: cross attention, or a chunk that sees
- * itself whole). A row that sees nothing gets zeros. What lies in the cache
- * at tokens a row does not see has no effect on it, infinities and NaN included.
+ * itself whole). A row that sees nothing, or scores of -inf alone, gets zeros
+ * (lse -inf). What lies in the cache at tokens a row does not see has no effect on
+ * it, infinities and NaN included, nor have the rows beside it. Of what it does
+ * see, a key whose score is -inf has no weight, one whose score is +inf or NaN
+ * makes the row NaN, and an infinite value makes its column infinite (fp16 and
+ * bf16 queries: infinite, or NaN where its weight rounds to 0).
  * q and out have H heads and one type, any multiple of Hkv query heads (at
  * most 32768 times), and may not overlap; their strides between tokens and
  * heads are at most 2^29 - 1 elements. Read from `a`: the cache, H, seq_lens, scale_log2, lse
@@ -443,7 +448,8 @@ cudaError_t kvf_b200_gather(const kvf_args *a, int fmt, int d, int ord, int page
  * (else cudaErrorMisalignedAddress), to 4 bytes for fp32. Products of fp32 queries have fp32 accuracy (about
  * 2^-21 relative). For fp16 and bf16 queries keys, values and softmax weights
  * are rounded to fp16 and the products accumulated in fp32: stored values past
- * 65504 (which a quantized group can hold) count as infinities there. */
+ * 65504 (which a quantized group can hold) count as infinities there, and weights
+ * are kept down to 2^-32 of a row's largest. Scores may be as large as fp32 holds. */
 cudaError_t kvf_b200_chunk_attention(const kvf_args *a, int fmt, int d, int ord, int paged, const kvf_heads *q,
                                      const kvf_heads *out, int T, const int *q_lens, int causal, cudaStream_t stream);
 

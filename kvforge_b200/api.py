@@ -306,12 +306,10 @@ def _launch(fn: str, device: torch.device, stream, *args) -> None:
     check(fn, getattr(lib(), fn)(*args, s))
 
 
-def _no_graph(what: str, *tensors: Optional[torch.Tensor]) -> None:
-    """Refuses tensors whose gradients would be lost: these calls build no autograd graph."""
+def _no_graph(x: torch.Tensor, what: str) -> None:
+    """Refuses a tensor whose gradient would be lost: these calls build no autograd graph."""
     if torch.is_grad_enabled():
-        for x in tensors:
-            if x is not None and x.requires_grad:
-                raise ValueError(f"{what} has no backward pass: call it under torch.no_grad(), or with detached tensors")
+        raise ValueError(f"{what} wants a gradient, and there is no backward pass: call under torch.no_grad(), or detach it")
 
 
 def _heads(x: torch.Tensor, what: str, device: torch.device, shape=None) -> KvfHeads:
@@ -321,6 +319,8 @@ def _heads(x: torch.Tensor, what: str, device: torch.device, shape=None) -> KvfH
     dtype = DTYPES.get(x.dtype)
     if dtype is None or x.device != device or not x.is_cuda:
         raise ValueError(f"{what} must be float32, float16 or bfloat16 on {device}")
+    if x.requires_grad:
+        _no_graph(x, what)
     sb, st, sh, sc = x.stride()
     if sc != 1 and size[3] > 1:
         raise ValueError(f"{what}: the channels of a head must be adjacent")
@@ -349,6 +349,8 @@ def _norm(weight: Optional[torch.Tensor], what: str, d: int, eps: float, device:
         return None
     if weight.dtype not in DTYPES or weight.shape != (d,) or weight.device != device or not weight.is_contiguous():
         raise ValueError(f"{what} must be a contiguous tensor [{d}] on {device}")
+    if weight.requires_grad:
+        _no_graph(weight, what)
     return ctypes.byref(KvfNorm(weight.data_ptr(), DTYPES[weight.dtype], eps))
 
 
@@ -394,7 +396,6 @@ def norm_rope(x: torch.Tensor, pos: Optional[torch.Tensor], rope: Optional[Rope]
     not read, and in `out` left as they were. out (default: a new tensor,
     zero there) may be x. A position outside the table leaves its rows unwritten
     and sets bit 2 of device_errors()."""
-    _no_graph("norm_rope", x, weight, out)
     xs = _heads(x, "x", x.device)
     B, T, H, d = x.shape
     if weight is None and rope is None:
@@ -425,11 +426,11 @@ def append_rope(cache: KVCache, k: torch.Tensor, v: torch.Tensor, rope: Optional
     q [B][T][H][D] takes the same tokens' query heads through q_weight and the
     rotation in the same launch; returned (q_out, or a new tensor), else None.
     lens (int32 [B]) defaults to all T. pos (int32 [B]) defaults to
-    cache.seq_lens, which is then raised by what was appended (on the call's
-    stream); a given pos leaves seq_lens alone. Tokens outside the cache or the
-    table are skipped and set bit 2 of device_errors()."""
+    cache.seq_lens, which is then raised by lens (on the call's stream, tokens
+    that were skipped included); a given pos leaves seq_lens alone. Keys and
+    values of tokens outside the cache, in a block without a page or outside the
+    table are skipped, and set bit 2 of device_errors()."""
     dev = cache.k.device
-    _no_graph("append_rope", k, v, q, k_weight, q_weight, q_out)
     if k.dim() != 4 or (k.shape[0], k.shape[2], k.shape[3]) != (cache.B, cache.Hkv, cache.d):
         raise ValueError(f"k must be [B][T][Hkv][D] with B={cache.B}, Hkv={cache.Hkv}, D={cache.d}")
     B, T, Hkv, d = k.shape
@@ -474,7 +475,6 @@ def gather(cache: KVCache, T: int, *, pos: Optional[torch.Tensor] = None, lens: 
     if out is None:
         out = tuple(_output(cache.k, shape, dtype, stream) for _ in range(2))
     k, v = out
-    _no_graph("gather", k, v)
     if k.dtype != v.dtype:
         raise ValueError("both outputs must have one type")
     _launch("kvf_b200_gather", dev, stream, ctypes.byref(_cache_args(cache)), cache.fmt, cache.d, cache.place.order,
@@ -526,7 +526,6 @@ def chunk_attention(q: torch.Tensor, cache: KVCache, *, q_lens: Optional[torch.T
     lse (float32 [B][T][H], contiguous) receives log2 of each softmax
     denominator. workspace (ChunkWorkspace.allocate) saves its allocation here."""
     dev = cache.k.device
-    _no_graph("chunk_attention", q, out)
     qs = _heads(q, "q", dev)
     B, T, H, d = q.shape
     if (B, d) != (cache.B, cache.d) or H == 0 or H % cache.Hkv:
