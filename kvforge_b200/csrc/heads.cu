@@ -101,7 +101,7 @@ template <int DT> __device__ __forceinline__ void store4(void *p, const float *e
 // 4 li .. 4 li + 3 of both halves, so that a pair is one lane's and the rotation
 // needs no shuffles (of which the other layout has eight a row, and the
 // shared-memory pipe that carries them was as busy as the schedulers: 4 x 4001
-// tokens of 64 heads 123 us with them, 88 us without, 81 us at the copy peak). The sum of squares keeps its tree: four
+// tokens of 64 heads 127 us with them, 98 us without, 81 us at the copy peak). The sum of squares keeps its tree: four
 // channels in the lane, neighbours by lane, the halves last.
 template <int DT, int D, int R>
 __device__ __forceinline__ void paired_rows(const HeadsArgs &a, int b, int j, long long t, int r0, int li) {
@@ -371,7 +371,7 @@ cudaError_t launch_heads(HeadsArgs a, cudaStream_t st) {
   // Rows per lane group. One in short calls, whose time is that of one row; more
   // where that still gives every SM some 32 warps. Queries alone: eight (four of
   // fp32), if a token's heads fill three quarters of such units (4 x 4001 tokens of
-  // 64 heads: 88 us with eight, 97 with four, 129 with two). With keys and values
+  // 64 heads: 98 us with eight, 113 with four, 132 with two). With keys and values
   // the quantizer needs the registers: two (8 ragged chunks of 2048 tokens into
   // int8: 111 us with two, 123 with four, 148 with eight).
   constexpr int BIG = DT == KVF_DT_F32 ? 4 : 8;
@@ -531,8 +531,8 @@ __global__ void __launch_bounds__(256) gather_kernel(const GatherArgs a) {
 template <int FMT, int DT, int D>
 cudaError_t launch_gather(GatherArgs a, cudaStream_t st) {
   // Rows per lane group: as many as keep three quarters of the lanes busy, four,
-  // or eight of the short int4 rows (65536 tokens of 8 heads: 72 us with eight,
-  // 79 with four; a ragged f16 batch 62 us with four, 65 with eight).
+  // or eight of the short int4 rows (65536 tokens of 8 heads: 75 us with eight,
+  // 80 with four; a ragged f16 batch 64 us with four, 67 with eight).
   constexpr int RPW = 32 / (D / 8), BIG = FMT == KVF_FMT_INT4 ? 8 : 4;
   const int rows = 2 * a.k.heads;
   auto units = [&](int r) { return (rows + r * RPW - 1) / (r * RPW); };
