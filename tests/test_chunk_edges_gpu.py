@@ -313,3 +313,73 @@ def test_workspaces_that_do_not_hold_the_partials(cuda):
         with pytest.raises(ValueError):
             api.chunk_attention(q, cache, workspace=api.ChunkWorkspace(4, part_o, part_ml))
     assert bool(api.chunk_attention(q, cache, workspace=good).isfinite().all()) and api.device_errors() == 0
+
+
+def _softmax_rows(q, cache):
+    """Causal attention over the stored values in 64 bits, whole sequences of n tokens."""
+    B, T, H, d = q.shape
+    k, v = (x.double() for x in api.gather(cache, cache.n))
+    g, n = H // cache.Hkv, cache.n
+    k, v = (x.repeat_interleave(g, 2).transpose(1, 2) for x in (k, v))
+    s = q.double().transpose(1, 2) @ k.transpose(-1, -2) / math.sqrt(d)
+    last = n - T + torch.arange(T, device=q.device)
+    s.masked_fill_(torch.arange(n, device=q.device) > last[:, None], -math.inf)
+    return (torch.softmax(s, -1) @ v).transpose(1, 2)
+
+
+def _near(got, want):
+    """Normal inputs of 128 channels or fewer. 16-bit queries: keys off by 2^-11 move a
+    score by at most 2^-11 sum |q k| / sqrt(d), about 2^-11 * 8, and the output by twice
+    that times its |values| (about 1): 2^-7; weights, values and the output's rounding add
+    2^-9 at most. fp32: 2^-21 in place of 2^-11, and sums over the tokens."""
+    tol = 2.0 ** -14 if got.dtype == torch.float32 else 2.0 ** -6
+    return bool(((got.double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("fmt,group", [(FMT_F16, 0), (FMT_INT8, 64), (FMT_INT4, 32)])
+@pytest.mark.parametrize("order", [ORD_HEAD, ORD_TOKEN])
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+def test_every_page_size(cuda, dtype, fmt, group, order, page):
+    g = _gen(cuda, 11)
+    B, T, H, Hkv, n, d = 2, 40, 6, 3, 300, 128
+    cache = api.KVCache.from_logical(_randn((B, Hkv, n, d), g), _randn((B, Hkv, n, d), g), fmt=fmt, group=group,
+                                     place=Placement(order, True, page))
+    q = _randn((B, T, H, d), g, dtype)
+    want = _softmax_rows(q, cache)
+    for splits in (1, 2, 3):
+        assert _near(_attend(q, cache, splits), want)
+    assert api.device_errors() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads", [100, 129, 300, 5000])
+def test_many_query_heads_for_a_kv_head(cuda, dtype, heads):
+    """Tiles that end inside a token's heads, and tokens of many tiles."""
+    g = _gen(cuda, 12)
+    B, T, Hkv, n, d = 1, 3, 2, 150, 64
+    cache = api.KVCache.from_logical(_randn((B, Hkv, n, d), g), _randn((B, Hkv, n, d), g), fmt=FMT_INT8, group=64, place=TOKEN16)
+    q = _randn((B, T, heads * Hkv, d), g, dtype)
+    want = _softmax_rows(q, cache)
+    for splits in (1, 2):
+        assert _near(_attend(q, cache, splits), want)
+    assert api.device_errors() == 0
+
+
+def test_calls_on_two_streams_at_once(cuda):
+    """Chunks of two batches on streams of their own, default workspaces: the bits of calls one by one."""
+    g = _gen(cuda, 13)
+    B, T, H, Hkv, n, d = 4, 16, 16, 4, 3000, 128
+    sets = []
+    for fmt, group, dtype in ((FMT_INT8, 64, torch.bfloat16), (FMT_F16, 0, torch.float32)):
+        cache = api.KVCache.from_logical(_randn((B, Hkv, n, d), g), _randn((B, Hkv, n, d), g), fmt=fmt, group=group, place=TOKEN16)
+        q = _randn((B, T, H, d), g, dtype)
+        assert api.ChunkWorkspace.allocate(cache, T, H, dtype).splits > 1
+        sets.append((q, cache, api.chunk_attention(q, cache), torch.cuda.Stream(cuda)))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        outs = [api.chunk_attention(q, cache, stream=st) for q, cache, _, st in sets]
+        torch.cuda.synchronize()
+        for x, (_, _, want, _) in zip(outs, sets):
+            assert torch.equal(x, want)
+    assert api.device_errors() == 0

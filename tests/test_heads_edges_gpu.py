@@ -190,3 +190,37 @@ def test_tensors_that_want_gradients_are_refused(cuda):
         with torch.no_grad():
             call(wants)
     assert api.device_errors() == 0
+
+
+def test_a_step_in_a_graph(cuda):
+    """append_rope that raises the lengths itself, and attention with a workspace of the
+    graph's own, replayed: the bits of calls one by one."""
+    g = _gen(cuda, 7)
+    B, T, H, Hkv, n, d = 3, 2, 8, 2, 64, 128
+    place = Placement(ORD_TOKEN, True, 16)
+    a, b = (api.KVCache.empty(B, Hkv, n, d, fmt=FMT_INT8, group=64, place=place, device=cuda) for _ in range(2))
+    rope = api.Rope.build(n, d, device=cuda)
+    qkv = _randn((B, T, H + 2 * Hkv, d), g, torch.bfloat16)
+    q, k, v = qkv.split((H, Hkv, Hkv), 2)
+    lens = torch.tensor([2, 1, 2], dtype=torch.int32, device=cuda)
+
+    def step(cache):
+        return api.chunk_attention(api.append_rope(cache, k, v, rope, q=q, lens=lens), cache, q_lens=lens)
+
+    step(a)  # kernels' attributes are set outside the capture
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(a)
+    a.seq_lens.zero_()
+    for x in (a.k, a.v, a.k_meta, a.v_meta):
+        x.zero_()
+    for new in ([2, 1, 2], [1, 0, 2], [2, 2, 2], [0, 1, 1]):
+        qkv.copy_(_randn(qkv.shape, g, qkv.dtype))
+        lens.copy_(torch.tensor(new, dtype=torch.int32))
+        graph.replay()
+        assert torch.equal(out, step(b))
+        assert torch.equal(a.seq_lens, b.seq_lens)
+    for x, y in zip((a.k, a.v, a.k_meta, a.v_meta), (b.k, b.v, b.k_meta, b.v_meta)):
+        assert torch.equal(x, y)
+    assert api.device_errors() == 0
