@@ -21,7 +21,6 @@ namespace {
 // Splits that saw nothing have m = -inf and no output.
 template <int DT, int D>
 __global__ void __launch_bounds__(128) chunk_merge(const ChunkArgs a) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int lane = threadIdx.x & 31;
   const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (at >= (long long)a.B * a.T * a.H) return;
@@ -85,7 +84,7 @@ bool one_tile(long long rows, int splits) { return rows <= kTcRows && splits % 2
 
 // Launches fn(a) or fn(a, maps[0], maps[1]).
 cudaError_t launch(void *fn, long long blocks, int threads, uint32_t smem, const ChunkArgs &a, CUtensorMap *maps,
-                   bool dependent, cudaStream_t st) {
+                   cudaStream_t st) {
   if (blocks <= 0) return cudaSuccess;
   if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
   cudaLaunchConfig_t cfg{};
@@ -93,11 +92,6 @@ cudaError_t launch(void *fn, long long blocks, int threads, uint32_t smem, const
   cfg.blockDim = dim3((unsigned)threads, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = dependent ? 1 : 0;
   void *params[] = {const_cast<ChunkArgs *>(&a), maps, maps ? maps + 1 : nullptr};
   return cudaLaunchKernelExC(&cfg, fn, params);
 }
@@ -227,7 +221,7 @@ extern "C" cudaError_t kvf_b200_chunk_attention(const kvf_args *args, int fmt, i
     const uint32_t smem = (uint32_t)chunk_mma_smem(d);
     a.tiles = (T * a.g + kChunkRows - 1) / kChunkRows;
     if ((e = ensure_kernel_smem(fn, smem)) != cudaSuccess) return e;
-    e = launch(fn, (long long)a.tiles * a.B * a.cache.Hkv * a.splits, kChunkThreads, smem, a, nullptr, false, stream);
+    e = launch(fn, (long long)a.tiles * a.B * a.cache.Hkv * a.splits, kChunkThreads, smem, a, nullptr, stream);
   } else {
     const bool two = !one_tile((long long)T * a.g, a.splits);
     const TcVariant x = fmt == KVF_FMT_F16    ? tc_variant<KVF_FMT_F16>(q->dtype, d, two)
@@ -239,7 +233,7 @@ extern "C" cudaError_t kvf_b200_chunk_attention(const kvf_args *args, int fmt, i
     if ((e = encode_cache_maps(args, fmt, d, ord, paged, tbox, maps[0], maps[1])) != cudaSuccess) return e;
     if ((e = ensure_kernel_smem(x.fn, x.smem)) != cudaSuccess) return e;
     e = launch(x.fn, (long long)a.tiles * a.B * a.cache.Hkv * (two ? a.splits : a.splits / 2), x.threads, x.smem, a, maps,
-               false, stream);
+               stream);
   }
   if (e != cudaSuccess || a.splits == 1) return e;
   void *mf = d == 128 ? (q->dtype == KVF_DT_F32   ? merge_fn<KVF_DT_F32, 128>()
@@ -248,5 +242,5 @@ extern "C" cudaError_t kvf_b200_chunk_attention(const kvf_args *args, int fmt, i
                       : (q->dtype == KVF_DT_F32   ? merge_fn<KVF_DT_F32, 64>()
                          : q->dtype == KVF_DT_F16 ? merge_fn<KVF_DT_F16, 64>()
                                                   : merge_fn<KVF_DT_BF16, 64>());
-  return launch(mf, ((long long)a.B * T * a.H + 3) / 4, 128, 0, a, nullptr, true, stream);
+  return launch(mf, ((long long)a.B * T * a.H + 3) / 4, 128, 0, a, nullptr, stream);
 }

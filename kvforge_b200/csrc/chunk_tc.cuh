@@ -23,8 +23,8 @@
 //          neither waits on the other's weights: S = Q K^T into tensor memory, O += P V
 //          with P read from tensor memory, where the softmax group writes it over its
 //          scores, and V read MN-major. The other two are the producers of K and of V:
-//          TMA boxes per page. A box of tokens that nobody sees, or of a block mapped
-//          to a negative page, is asked for at page -1, which TMA fills with zeros.
+//          TMA boxes per page, none for tokens that nobody sees or for a block
+//          without a page.
 // A row's weights are taken against a reference 7 below its running maximum (log2),
 // so that the largest is about 2^7: fp16 then holds weights down to 2^-32 of it, where
 // against the maximum itself those below 2^-25 would be lost, and many small ones
@@ -229,17 +229,12 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
   const int n = (w.t1 - w.t0 + kTcStep - 1) / kTcStep;
 
   // Steps of each softmax group.
-  int nw[2];
-#pragma unroll
-  for (int g = 0; g < 2; ++g) {
-    if (TWO) {
-      const int rows = min(w.rows - g * kTcRows, kTcRows);
-      const int seen = rows > 0 ? chunk_seen(a, w, g * kTcRows + rows - 1) : 0;
-      nw[g] = seen > w.t0 ? min(n, (seen - w.t0 + kTcStep - 1) / kTcStep) : 0;
-    } else {
-      nw[g] = (n + 1 - g) / 2;
-    }
-  }
+  auto group_steps = [&](int g) -> int {
+    if (!TWO) return (n + 1 - g) / 2;
+    const int rows = min(w.rows - g * kTcRows, kTcRows);
+    const int seen = rows > 0 ? chunk_seen(a, w, g * kTcRows + rows - 1) : 0;
+    return seen > w.t0 ? min(n, (seen - w.t0 + kTcStep - 1) / kTcStep) : 0;
+  };
 
   // First step that some row of the block does not see whole. From there on V
   // tiles must not carry infinities or NaN into such rows (0 * inf): zeros stand
@@ -329,7 +324,7 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
     const bool idle = __all_sync(0xffffffffu, !live);
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
     const uint32_t ts = tbase + lanes + S_COL + 128u * grp, to = tbase + lanes + O_COL + (uint32_t)(D * grp);
-    const int steps = nw[grp];
+    const int steps = group_steps(grp);
     // Reference (log2) of the row's weights and their sum; where the reference is
     // past kTcFar it is the raw score `base`, and m is NaN so that every half is raised.
     float m = -INFINITY, l = 0.f, base = 0.f;
@@ -764,7 +759,6 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
       // ----------------------------------------------------------- producers
       const int op = warp - LAST - 1;  // 0: K, 1: V
       const CUtensorMap *map = op ? &tmv : &tmk;
-      if (lane == 0) ptx::prefetch_tmap(map);
       const uint64_t pol = ptx::policy_evict_last();
       const bool paged = a.cache.paged != 0;
       const int bts = paged ? a.cache.bt_shift : 30, bmask = (1 << bts) - 1;
@@ -782,15 +776,40 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
         return page;
       };
       // One elected lane issues an item's boxes; coordinates come from the lanes
-      // that hold them.
+      // that hold them. A box with no page is not asked for. What its rows hold is
+      // of no account where nobody sees them (scores are masked, values cleared),
+      // nor in a quantized cache (codes of no scale and no zero); rows of an f16
+      // cache that are seen all the same, in a block without a page, are zeros.
       auto fill = [&](uint32_t dst, uint32_t full, uint32_t bytes, int t, int page) {
-        const int my = max(page, -1);
+        const uint32_t there = __ballot_sync(0xffffffffu, lane < boxes && page >= 0);
+        if constexpr (!L::RAW) {
+          uint32_t blank = __ballot_sync(0xffffffffu, lane < boxes && page < 0 && t + (lane << tbs) < w.t1);
+          if (blank) {
+            for (; blank; blank &= blank - 1) {
+              const uint32_t at = dst + ((uint32_t)(__ffs(blank) - 1) << tbs) * 128u;
+              for (int k = lane; k < KB * (8 << tbs); k += 32)
+                asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(at + (uint32_t)(k / (8 << tbs)) * BLK +
+                                                                         (uint32_t)(k % (8 << tbs)) * 16u),
+                             "r"(0)
+                             : "memory");
+            }
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+          }
+        }
+        bytes = bytes / (uint32_t)boxes * (uint32_t)__popc(there);
+        if (tc::elect_one()) {
+          if (bytes)
+            ptx::mbar_arrive_expect_tx(full, bytes);
+          else
+            ptx::mbar_arrive(full);
+        }
+        __syncwarp();
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
-          if (x < boxes) {
-            const int pg = __shfl_sync(0xffffffffu, my, x);
+          if (there >> x & 1u) {
+            const int pg = __shfl_sync(0xffffffffu, page, x);
             if (tc::elect_one()) {
-              if (x == 0) ptx::mbar_arrive_expect_tx(full, bytes);
               const int c1 = paged ? (t + (x << tbs)) & bmask : t + (x << tbs);
               if (L::RAW) {
                 ptx::tma_g2s_4d(dst + ((uint32_t)x << tbs) * RB, map, 0, c1, w.h, pg, full, pol);
@@ -841,6 +860,7 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
     } else {
       // --------------------------------------------------------- MMA issue
       const int g = warp == LAST ? 0 : 1;  // the softmax group that this warp issues for
+      const int nw = group_steps(g);
       constexpr uint32_t ID_S = tc::idesc_f16(false, false, 128, 64), ID_O = tc::idesc_f16(false, true, 128, D);
       bool ok = true;
       // Waits for K or V tile i.
@@ -896,7 +916,7 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
       int i = TWO ? 0 : g;
       ok = tc_wait_warp(bar(&sh.qready), 0u, abort_flag);
       if (ok && i < n && take_k(i)) {
-        if (nw[g] > 0)
+        if (nw > 0)
           for (int h = 0; h < 2; ++h) scores(i, h);
         release(&sh.kempty[i % SLOTS]);
       }
@@ -906,17 +926,17 @@ chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tmk, cons
         const bool more = next < n;
         // The first half's next scores go between the two products, unless the
         // K tile is late: the second product does not wait for it.
-        if (j < nw[g] && !values(i, j, 0)) break;
+        if (j < nw && !values(i, j, 0)) break;
         const bool between = more && __all_sync(0xffffffffu, ptx::mbar_test_wait(bar(&sh.kfull[next % SLOTS]),
                                                                                (uint32_t)((next / SLOTS) & 1)));
         if (between) {
           tc::fence_after();
-          if (j + 1 < nw[g]) scores(next, 0);
+          if (j + 1 < nw) scores(next, 0);
         }
-        if (j < nw[g] && !values(i, j, 1)) break;
+        if (j < nw && !values(i, j, 1)) break;
         release(&sh.vempty[i % SLOTS]);
         if (more && (between || take_k(next))) {
-          if (j + 1 < nw[g]) {
+          if (j + 1 < nw) {
             if (!between) scores(next, 0);
             scores(next, 1);
           }

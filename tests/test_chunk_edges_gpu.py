@@ -383,3 +383,49 @@ def test_calls_on_two_streams_at_once(cuda):
         for x, (_, _, want, _) in zip(outs, sets):
             assert torch.equal(x, want)
     assert api.device_errors() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("fmt,group,d", [(FMT_F16, 0, 128), (FMT_F16, 0, 64), (FMT_INT8, 64, 128), (FMT_INT4, 32, 64)])
+@pytest.mark.parametrize("page", [16, 64, 128])
+def test_seen_blocks_without_a_page_are_zeros(cuda, dtype, fmt, group, d, page):
+    """In the middle and at the end of a sequence, whatever earlier steps left behind."""
+    g = _gen(cuda, 14)
+    B, T, H, Hkv, n = 2, 30, 4, 2, 500
+    cache = api.KVCache.from_logical(_randn((B, Hkv, n, d), g), _randn((B, Hkv, n, d), g), fmt=fmt, group=group,
+                                     place=Placement(ORD_HEAD, True, page))
+    cache.block_table[0, 1] = cache.block_table[1, 0] = cache.block_table[1, -1] = -1
+    q = _randn((B, T, H, d), g, dtype)
+    want = _softmax_rows(q, cache)  # reads such blocks back as zeros, and reports them
+    assert api.device_errors() == 4
+    for splits in (1, 2, 3):
+        assert _near(_attend(q, cache, splits), want)
+    assert api.device_errors() == 0
+
+
+def test_a_stream_of_small_calls(cuda):
+    """Many short calls of all kinds, one behind the other: sequences of no, one and
+    few tokens, splits without tokens, pages that end inside a tile."""
+    import random
+
+    g, rng = _gen(cuda, 15), random.Random(15)
+    results = []
+    for _ in range(150):
+        d, fmt = rng.choice((64, 128)), rng.choice((FMT_F16, FMT_INT8, FMT_INT4))
+        B, T, Hkv, heads, n = rng.choice((1, 2, 5)), rng.randint(1, 40), rng.choice((1, 2, 3)), rng.choice((1, 2, 5)), rng.randint(1, 200)
+        page = rng.choice((0, 16, 64, 128))
+        cache = api.KVCache.empty(B, Hkv, n, d, fmt=fmt, group=0 if fmt == FMT_F16 else 64,
+                                  place=Placement(rng.choice((ORD_HEAD, ORD_TOKEN)), page > 0, page), device=cuda)
+        k, v = (_randn((B, n, Hkv, d), g, torch.float16) for _ in range(2))
+        kv = torch.randint(0, n + 1, (B,), generator=g, device=cuda, dtype=torch.int32)
+        api.append_rope(cache, k, v, lens=kv)
+        q = _randn((B, T, heads * Hkv, d), g, rng.choice(DTYPES))
+        lens = torch.randint(0, T + 1, (B,), generator=g, device=cuda, dtype=torch.int32)
+        outs = [_attend(q, cache, s, q_lens=lens) for s in (1, 2, 4, 7)]
+        results.append((outs, d))
+    for outs, d in results:
+        for x in outs[1:]:
+            # rows of one token or a few: values up to about 5, rounded alike or one step of the type apart
+            tol = 1e-4 if x.dtype == torch.float32 else 2.0 ** -8 if x.dtype == torch.float16 else 2.0 ** -5
+            assert bool(x.isfinite().all()) and bool(((x.float() - outs[0].float()).abs() <= tol).all())
+    assert api.device_errors() == 0
