@@ -549,7 +549,7 @@ decode_kernel(const kvf_args a, const Plan p, const __grid_constant__ CUtensorMa
 
   if (warp == p.hh) {
     // ------------------------------------------------------------ producer
-    if (lane == 0) {
+    if (lane == 0 && t0 < t1) {  // only where loads follow, which are waited for
       ptx::prefetch_tmap(&tmk);
       ptx::prefetch_tmap(&tmv);
       if (GPR > 0 && p.meta_tma) {

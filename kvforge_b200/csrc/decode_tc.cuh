@@ -254,7 +254,7 @@ decode_tc_kernel(const kvf_args a, const TcPlan p, const __grid_constant__ CUten
     const int pw = warp - kTcProducerWarp;
     const CUtensorMap *tmap = pw ? &tmv : &tmk;
     const uint32_t *meta = reinterpret_cast<const uint32_t *>(pw ? a.v_meta : a.k_meta);
-    if (lane == 0) ptx::prefetch_tmap(tmap);
+    if (lane == 0 && ntiles > 0) ptx::prefetch_tmap(tmap);  // only where loads follow, which are waited for
     const uint64_t pol = ptx::policy_evict_first();
     const int tbs = p.tbox_shift;
     const int bmask = (1 << p.bt_shift) - 1;
